@@ -125,9 +125,43 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32,  # m, n, k, gated, eager
         _p, _p,                     # workspace, stream
     ]),
+    "bvllm_tree_range_steps": (ctypes.c_int32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64]),
+    "bvllm_tree_workspace_bytes": (ctypes.c_int64, [_i32, _i32, _i32, _i32]),
+    "bvllm_paged_tree_attention": (ctypes.c_int, [
+        _p, _i64, _i64,             # q
+        _p, _p, _i64, _i64, _i64,   # caches + strides
+        _i32,                       # num_blocks
+        _p, _i64, _i32,             # block_tables, bt_stride, max_blocks
+        _p, _p, _p,                 # query_start_loc, seq_lens, context_lens
+        _p, _i64, _i32, _f32,       # tree_mask, stride, words, scale
+        _p, _i64, _i64,             # out
+        _i32, _i32, _i32,           # num_seqs, num_tokens, max_query_len
+        _i32, _i32, _i32, _i32,     # H, Hkv, D, block_size
+        _p, _i32, _i32, _p,         # workspace, range_steps, num_ranges, stream
+    ]),
+    "bvllm_commit_draft_tree": (ctypes.c_int, [
+        _p, _p, _i32,               # k_caches, v_caches, num_layers
+        _i64, _i64, _i64, _i32, _i32, _i32, _i32,  # strides, num_blocks, Hkv, D, block_size
+        _p, _i64, _i32,             # block_tables, bt_stride, max_blocks
+        _p, _p, _p, _p, _p,         # query_start_loc, context_lens, draft, target, parents
+        _p, _p, _p,                 # path, accepted, following
+        _i32, _i32, _p,             # num_seqs, max_path, stream
+    ]),
+    "bvllm_beam_workspace_bytes": (ctypes.c_int64, [_i32, _i32]),
+    "bvllm_beam_select": (ctypes.c_int, [
+        _p, _i64, _i32, _p,         # logits, row_stride, logits_fp32, scores
+        _i32, _i32, _i32, _i32,     # num_groups, num_beams, vocab, num_candidates
+        _p, _p, _p, _p, _p,         # workspace, out scores, beams, tokens, stream
+    ]),
+    "bvllm_reorder_beams": (ctypes.c_int, [
+        _p, _p, _i32,               # k_caches, v_caches, num_layers
+        _i64, _i64, _i64, _i32, _i32, _i32, _i32,  # strides, num_blocks, Hkv, D, block_size
+        _p, _i64, _i32,             # block_tables, bt_stride, max_blocks
+        _p, _p, _i32, _i32, _p,     # seq_lens, beams, num_groups, num_beams, stream
+    ]),
 }
 
-ABI_VERSION = 10
+ABI_VERSION = 11
 
 
 # Pages (rows · table width) that the balanced launches take.

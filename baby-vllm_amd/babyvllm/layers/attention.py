@@ -1,9 +1,10 @@
-"""Paged attention layer: routes a step to the decode or the prefill HIP kernel.
+"""Paged attention layer: routes a step to the decode, the prefill or the draft tree HIP kernel.
 
 Mirrors ``Attention`` of babyvllm/layers/attention.py:35-68: with a forward
 context and a cache, a step whose ``max_query_len == 1`` runs
 ``paged_decode_attention`` (with ``max_seq_len`` = the step's context bucket),
-any longer step runs ``paged_prefill_attention``. This build has no torch
+any longer step runs ``paged_prefill_attention``; a step with a ``tree_mask`` (drafted
+token trees, not in the reference) runs ``paged_tree_attention``. This build has no torch
 attention path: a call on a non-ROCm tensor, without a KV cache or without a
 forward context raises instead of silently computing elsewhere.
 
@@ -47,6 +48,9 @@ class Attention(nn.Module):
         if not q.is_cuda:
             raise RuntimeError(f"Attention runs only on a ROCm device, got {q.device}")
         md = ctx.attn_metadata
+        if getattr(md, "tree_mask", None) is not None:
+            from babyvllm.kernels.tree_attn import paged_tree_attention
+            return paged_tree_attention(q, self.kv_cache, md, self.scale)
         if md.max_query_len == 1 and self.kv_cache.shape[2] >= 16:
             from babyvllm.kernels.paged_attn import paged_decode_attention
             return paged_decode_attention(q, self.kv_cache, md.block_tables, md.seq_lens,

@@ -4,7 +4,9 @@ Same fields and meaning as the reference: ``slot_mapping`` int64 ``[T]``,
 ``block_tables`` int32 ``[S, W]``, ``query_start_loc`` int32 ``[S+1]``,
 ``seq_lens`` / ``context_lens`` int32 ``[S]``, their host-side lists, and the
 host ints ``max_query_len`` (1 for a pure decode step) and ``max_seq_len``
-(the context bucket under a captured graph).
+(the context bucket under a captured graph). ``tree_mask`` has no counterpart there: the
+visibility words of a step whose rows are drafted token trees (``kernels/tree_attn.py``),
+else None.
 """
 
 from __future__ import annotations
@@ -27,6 +29,7 @@ class AttentionMetadata:
     context_lens_cpu: list[int]
     max_query_len: int
     max_seq_len: int
+    tree_mask: torch.Tensor | None = None  # int64 [T, W]
 
 
 @dataclass

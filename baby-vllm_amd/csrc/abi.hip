@@ -417,3 +417,157 @@ extern "C" int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t v
   a.rows = rows; a.hidden = hidden; a.head_dim = head_dim;
   return (int)embed_rows(a, (hipStream_t)stream);
 }
+
+extern "C" int32_t bvllm_tree_range_steps(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t max_blocks, int64_t key_steps, int64_t longest_steps) {
+  if (num_seqs < 1 || num_tokens < 1 || max_query_len < 1 || max_blocks < 1) return 0;
+  if (!valid_heads(num_heads, num_kv_heads) || (head_dim != 64 && head_dim != 128)) return 0;
+  TreeArgs a{};
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.max_query_len = max_query_len;
+  a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.max_blocks = max_blocks;
+  return tree_range_steps(a, key_steps, longest_steps);
+}
+
+extern "C" int64_t bvllm_tree_workspace_bytes(int32_t num_tokens, int32_t num_heads, int32_t head_dim,
+                                              int32_t num_ranges) {
+  if (num_tokens < 1 || num_heads < 1 || head_dim < 1 || num_ranges < 2) return 0;
+  return tree_range_bytes(num_ranges, num_tokens, num_heads, head_dim);
+}
+
+extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                                          const void* k_cache, const void* v_cache,
+                                          int64_t cache_stride_block, int64_t cache_stride_tok,
+                                          int64_t cache_stride_head, int32_t num_blocks,
+                                          const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                                          const int32_t* query_start_loc, const int32_t* seq_lens,
+                                          const int32_t* context_lens,
+                                          const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words,
+                                          float scale,
+                                          void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                          int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                          int32_t block_size, void* workspace, int32_t range_steps,
+                                          int32_t num_ranges, void* stream) {
+  if (num_seqs < 0 || num_tokens < 0 || max_query_len < 0) return kBad;
+  if (!valid_heads(num_heads, num_kv_heads)) return kBad;
+  if (head_dim != 64 && head_dim != 128) return kBad;
+  if (block_size != 16) return kBad;
+  if (!(scale > 0.f) || scale * kLog2e > 3.4e38f) return kBad;
+  if (num_tokens == 0 || num_seqs == 0 || max_query_len == 0) return 0;
+  if (!q || !out || !block_tables || !query_start_loc || !seq_lens || !context_lens || !tree_mask) return kBad;
+  if (!cache_ok(k_cache, v_cache, cache_stride_block, cache_stride_tok, cache_stride_head, num_blocks)) return kBad;
+  if (!aligned16(q) || !aligned16(out) || q_stride_t % 8 || q_stride_h % 8 || out_stride_t % 8 || out_stride_h % 8)
+    return kBad;
+  if (max_blocks < 1 || bt_stride < max_blocks) return kBad;
+  // Offsets inside one page are 32-bit, and so are (token, head) pairs.
+  if ((int64_t)16 * cache_stride_tok > 0x3fffffff || (int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
+  if (mask_words < 1 || (int64_t)mask_words * 64 < max_query_len || mask_stride < mask_words) return kBad;
+  if (range_steps < 0 || range_steps > (1 << 28)) return kBad;
+  if (range_steps > 0 && (num_ranges < 1 || num_ranges > tree_max_ranges(max_blocks, range_steps))) return kBad;
+  const int32_t ranges = range_steps > 0 ? num_ranges : 1;
+  if (ranges > 1 && (!workspace || !aligned16(workspace))) return kBad;
+  TreeArgs a{};
+  a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
+  a.k_cache = k_cache; a.v_cache = v_cache;
+  a.c_sb = cache_stride_block; a.c_st = cache_stride_tok; a.c_sh = cache_stride_head;
+  a.num_pages = num_blocks;
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.max_blocks = max_blocks;
+  a.query_start_loc = query_start_loc; a.seq_lens = seq_lens; a.context_lens = context_lens;
+  a.tree_mask = tree_mask; a.mask_stride = mask_stride; a.mask_words = mask_words;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.max_query_len = max_query_len;
+  a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.range_steps = range_steps > 0 ? range_steps : 1 << 28;
+  a.num_ranges = ranges;
+  if (ranges > 1) {
+    a.part_out = reinterpret_cast<float*>(workspace);
+    a.part_ml = a.part_out + (int64_t)ranges * num_tokens * num_heads * head_dim;
+  }
+  return (int)paged_tree_attention(a, (hipStream_t)stream);
+}
+
+// The layers' pointers and their common shape (num_layers may be 0).
+static bool cache_set_ok(void* const* k, void* const* v, int32_t layers, int64_t sb, int64_t st, int64_t sh,
+                         int32_t nb, int32_t hkv, int32_t d, int32_t block_size) {
+  if (layers < 0 || hkv < 1 || d < 8 || d % 8 || block_size != 16 || (layers > 0 && (!k || !v))) return false;
+  if ((int64_t)hkv * d > 1 << 20) return false;  // chunks of 64 layers' rows are numbered in 32 bits
+  for (int32_t i = 0; i < layers; ++i)
+    if (!cache_ok(k[i], v[i], sb, st, sh, nb)) return false;
+  return true;
+}
+
+extern "C" int bvllm_commit_draft_tree(void* const* k_caches, void* const* v_caches, int32_t num_layers,
+                                       int64_t cache_stride_block, int64_t cache_stride_tok,
+                                       int64_t cache_stride_head, int32_t num_blocks, int32_t num_kv_heads,
+                                       int32_t head_dim, int32_t block_size,
+                                       const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                                       const int32_t* query_start_loc, const int32_t* context_lens,
+                                       const int64_t* draft_tokens, const int64_t* target_tokens,
+                                       const int32_t* parents,
+                                       int32_t* path, int32_t* accepted, int64_t* following,
+                                       int32_t num_seqs, int32_t max_path, void* stream) {
+  if (num_seqs < 0 || num_seqs > 65535 || max_path < 1 || max_path > 4096) return kBad;
+  if (!cache_set_ok(k_caches, v_caches, num_layers, cache_stride_block, cache_stride_tok, cache_stride_head,
+                    num_blocks, num_kv_heads, head_dim, block_size))
+    return kBad;
+  if (num_seqs == 0) return 0;
+  if (!block_tables || max_blocks < 1 || bt_stride < max_blocks || !query_start_loc || !context_lens) return kBad;
+  if (!draft_tokens || !target_tokens || !parents || !path || !accepted || !following) return kBad;
+  CommitArgs a{};
+  a.cache = {cache_stride_block, cache_stride_tok, cache_stride_head, num_blocks, num_kv_heads, head_dim};
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.max_blocks = max_blocks;
+  a.query_start_loc = query_start_loc; a.context_lens = context_lens;
+  a.draft_tokens = draft_tokens; a.target_tokens = target_tokens; a.parents = parents;
+  a.path = path; a.accepted = accepted; a.following = following;
+  a.num_seqs = num_seqs; a.max_path = max_path;
+  return (int)commit_draft_tree(a, k_caches, v_caches, num_layers, (hipStream_t)stream);
+}
+
+extern "C" int64_t bvllm_beam_workspace_bytes(int32_t rows, int32_t vocab) {
+  if (rows < 1 || vocab < 1) return 0;
+  return (int64_t)rows * ((vocab + (int64_t)kBeamPiece - 1) / kBeamPiece) * 2 * (int64_t)sizeof(float);
+}
+
+extern "C" int bvllm_beam_select(const void* logits, int64_t row_stride, int32_t logits_fp32, const float* scores,
+                                 int32_t num_groups, int32_t num_beams, int32_t vocab, int32_t num_candidates,
+                                 void* workspace, float* out_scores, int64_t* out_beams, int64_t* out_tokens,
+                                 void* stream) {
+  if (num_groups < 0 || num_beams < 1 || num_beams > kBeamMaxBeams || vocab < 1) return kBad;
+  if (num_candidates < 1 || num_candidates > kBeamMaxCandidates) return kBad;
+  if ((int64_t)num_beams * vocab < num_candidates || (logits_fp32 != 0 && logits_fp32 != 1)) return kBad;
+  if (((int64_t)vocab + kBeamPiece - 1) / kBeamPiece * num_beams > kBeamMaxPieces) return kBad;
+  if (num_groups == 0) return 0;
+  if ((int64_t)num_groups * num_beams > 0x7fffffff) return kBad;
+  if (!logits || !scores || !workspace || !out_scores || !out_beams || !out_tokens || row_stride < vocab) return kBad;
+  if (((uintptr_t)workspace & 7u) != 0 || ((uintptr_t)logits & (logits_fp32 ? 3u : 1u)) != 0) return kBad;
+  BeamSelectArgs a{};
+  a.logits = logits; a.row_stride = row_stride; a.fp32 = logits_fp32;
+  a.scores = scores;
+  a.num_groups = num_groups; a.num_beams = num_beams; a.vocab = vocab; a.num_candidates = num_candidates;
+  a.stats = reinterpret_cast<float*>(workspace);
+  a.out_scores = out_scores; a.out_beams = out_beams; a.out_tokens = out_tokens;
+  return (int)beam_select(a, (hipStream_t)stream);
+}
+
+extern "C" int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches, int32_t num_layers,
+                                   int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
+                                   int32_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                                   int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                                   const int32_t* seq_lens, const int64_t* beams,
+                                   int32_t num_groups, int32_t num_beams, void* stream) {
+  if (num_groups < 0 || num_groups > 65535 || num_beams < 1 || num_beams > kBeamMaxBeams) return kBad;
+  if (!cache_set_ok(k_caches, v_caches, num_layers, cache_stride_block, cache_stride_tok, cache_stride_head,
+                    num_blocks, num_kv_heads, head_dim, block_size))
+    return kBad;
+  if (num_groups == 0) return 0;
+  if (!block_tables || max_blocks < 1 || bt_stride < max_blocks || !seq_lens || !beams) return kBad;
+  ReorderArgs a{};
+  a.cache = {cache_stride_block, cache_stride_tok, cache_stride_head, num_blocks, num_kv_heads, head_dim};
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens; a.beams = beams;
+  a.num_groups = num_groups; a.num_beams = num_beams;
+  return (int)reorder_beams(a, k_caches, v_caches, num_layers, (hipStream_t)stream);
+}

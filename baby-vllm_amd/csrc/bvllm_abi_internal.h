@@ -133,6 +133,91 @@ struct EmbedArgs {
 };
 hipError_t embed_rows(const EmbedArgs& a, hipStream_t stream);
 
+// Attention of drafted token trees (tree_attn.hip).
+struct TreeArgs {
+  const void* q;  int64_t q_st, q_sh;      // [T, H, D]
+  const void* k_cache; const void* v_cache;
+  int64_t c_sb, c_st, c_sh;
+  int32_t num_pages;
+  const int32_t* block_tables; int64_t bt_stride; int32_t max_blocks;
+  const int32_t* query_start_loc;          // [S+1]
+  const int32_t* seq_lens;                 // [S]
+  const int32_t* context_lens;             // [S]
+  const int64_t* tree_mask; int64_t mask_stride; int32_t mask_words;  // [T, words]
+  float scale_log2;
+  void* out;      int64_t o_st, o_sh;      // [T, H, D]
+  int32_t num_seqs, num_tokens, max_query_len;
+  int32_t num_heads, num_kv_heads, head_dim;
+  // Key ranges: 32-key steps per range, their number (the last one runs to the row's end)
+  // and, with more than one, their fp32 partials.
+  int32_t range_steps, num_ranges;
+  float* part_out;                         // [num_ranges, T, H, D], unnormalized
+  float* part_ml;                          // [num_ranges, T, H, 2]: maximum (log2 units), sum
+};
+hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
+// 32-key steps per range for the batch's shape, 0 for whole rows (key_steps: those of all
+// sequences, longest_steps: of the longest; < 0 if unknown).
+int32_t tree_range_steps(const TreeArgs& a, int64_t key_steps, int64_t longest_steps);
+inline int64_t tree_range_bytes(int32_t num_ranges, int32_t num_tokens, int32_t num_heads, int32_t head_dim) {
+  return (int64_t)num_ranges * num_tokens * num_heads * (head_dim + 2) * (int64_t)sizeof(float);
+}
+// Ranges of range_steps steps that a table of max_blocks pages can hold.
+inline int32_t tree_max_ranges(int32_t max_blocks, int32_t range_steps) {
+  return (int32_t)((((int64_t)max_blocks + 1) / 2 + range_steps - 1) / range_steps);
+}
+
+// The K and V caches of several layers, all of one shape.
+constexpr int kCacheSetLayers = 64;        // of one launch
+struct CacheSet {
+  void* k[kCacheSetLayers];
+  void* v[kCacheSetLayers];
+};
+struct CacheShape {
+  int64_t stride_page, stride_token, stride_head;
+  int32_t num_pages, num_kv_heads, head_dim;
+};
+// A verified draft tree's path and its rows in the cache (cache_moves.hip).
+struct CommitArgs {
+  CacheShape cache;
+  const int32_t* block_tables; int64_t bt_stride; int32_t max_blocks;
+  const int32_t* query_start_loc;          // [S+1]
+  const int32_t* context_lens;             // [S]
+  const int64_t* draft_tokens;             // [T]
+  const int64_t* target_tokens;            // [T]
+  const int32_t* parents;                  // [T], within the sequence
+  int32_t* path;                           // [S, max_path]
+  int32_t* accepted;                       // [S]
+  int64_t* following;                      // [S]
+  int32_t num_seqs, max_path;
+};
+hipError_t commit_draft_tree(const CommitArgs& a, void* const* k, void* const* v, int layers, hipStream_t stream);
+// Beams that continue others: tables and partial pages (cache_moves.hip).
+struct ReorderArgs {
+  CacheShape cache;
+  int32_t* block_tables; int64_t bt_stride; int32_t max_blocks;  // [groups * beams, max_blocks]
+  const int32_t* seq_lens;                 // [groups * beams]
+  const int64_t* beams;                    // [groups * beams], within the group
+  int32_t num_groups, num_beams;
+};
+hipError_t reorder_beams(const ReorderArgs& a, void* const* k, void* const* v, int layers, hipStream_t stream);
+
+// Beam search's selection (beam_select.hip).
+constexpr int kBeamPiece = 2048;           // columns per piece
+constexpr int kBeamMaxPieces = 8192;       // pieces of one group's rows
+constexpr int kBeamMaxBeams = 32;
+constexpr int kBeamMaxCandidates = 64;
+struct BeamSelectArgs {
+  const void* logits; int64_t row_stride;  // [groups * beams, vocab], unit column stride
+  int32_t fp32;                            // 1: fp32 logits, 0: bf16
+  const float* scores;                     // [groups * beams]
+  int32_t num_groups, num_beams, vocab, num_candidates;
+  float* stats;                            // [groups * beams, pieces, 2]: maximum, sum of exponentials
+  float* out_scores;                       // [groups, candidates]
+  int64_t* out_beams;
+  int64_t* out_tokens;
+};
+hipError_t beam_select(const BeamSelectArgs& a, hipStream_t stream);
+
 // How a linear layer of a few tokens runs (skinny_linear.hip).
 struct LinearPlan {
   int32_t rw, kw;          // row waves x k slabs of a work-group; rw = 0: not a shape for this kernel

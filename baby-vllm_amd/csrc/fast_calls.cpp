@@ -42,6 +42,13 @@ struct Entry {
   decltype(&bvllm_silu_mul) silu = nullptr;
   decltype(&bvllm_linear_workspace_bytes) linear_bytes = nullptr;
   decltype(&bvllm_linear) linear = nullptr;
+  decltype(&bvllm_tree_range_steps) tree_steps = nullptr;
+  decltype(&bvllm_tree_workspace_bytes) tree_bytes = nullptr;
+  decltype(&bvllm_paged_tree_attention) tree = nullptr;
+  decltype(&bvllm_commit_draft_tree) commit = nullptr;
+  decltype(&bvllm_beam_workspace_bytes) beam_bytes = nullptr;
+  decltype(&bvllm_beam_select) beam = nullptr;
+  decltype(&bvllm_reorder_beams) reorder = nullptr;
 } g;
 
 struct BindName {
@@ -64,6 +71,13 @@ const BindName kNames[] = {
     {"bvllm_silu_mul", (void**)&g.silu},
     {"bvllm_linear_workspace_bytes", (void**)&g.linear_bytes},
     {"bvllm_linear", (void**)&g.linear},
+    {"bvllm_tree_range_steps", (void**)&g.tree_steps},
+    {"bvllm_tree_workspace_bytes", (void**)&g.tree_bytes},
+    {"bvllm_paged_tree_attention", (void**)&g.tree},
+    {"bvllm_commit_draft_tree", (void**)&g.commit},
+    {"bvllm_beam_workspace_bytes", (void**)&g.beam_bytes},
+    {"bvllm_beam_select", (void**)&g.beam},
+    {"bvllm_reorder_beams", (void**)&g.reorder},
 };
 
 // The wrappers' own error for a return code (babyvllm.kernels._lib.check), bound with the addresses.
@@ -451,6 +465,211 @@ PyObject* fast_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (q, kv_cache, block_tables, query_start_loc, seq_lens, context_lens, tree_mask, seq_lens list, max_query_len, scale,
+//  device, stream)
+PyObject* fast_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) return none();
+  const int64_t dev = PyLong_AsLongLong(a[10]);
+  const at::Tensor* q = plain(a[0], at::kBFloat16, dev);
+  const at::Tensor* c = plain(a[1], at::kBFloat16, dev);
+  const at::Tensor* bt = plain(a[2], at::kInt, dev);
+  const at::Tensor* qsl = plain(a[3], at::kInt, dev);
+  const at::Tensor* seq = plain(a[4], at::kInt, dev);
+  const at::Tensor* ctx = plain(a[5], at::kInt, dev);
+  const at::Tensor* mask = plain(a[6], at::kLong, dev);
+  if (!rows_of(q, 3) || !plain_cache(c) || !rows_of(bt, 2) || !rows_of(mask, 2)) return none();
+  for (const at::Tensor* v : {qsl, seq, ctx})
+    if (!v || v->dim() != 1 || !v->is_contiguous()) return none();
+  const int64_t tokens = q->size(0), heads = q->size(1), d = q->size(2), hkv = c->size(3), seqs = seq->size(0);
+  const int64_t width = bt->size(1), words = mask->size(1);
+  if (tokens == 0 || seqs == 0 || width == 0 || c->size(4) != d || c->size(2) != kPage) return none();
+  if (qsl->size(0) != seqs + 1 || ctx->size(0) != seqs || bt->size(0) < seqs || mask->size(0) < tokens) return none();
+  if (!small(tokens) || !small(heads) || !small(seqs) || !small(width) || !small(words)) return none();
+  if (!PyLong_CheckExact(a[8]) || !PyFloat_CheckExact(a[9])) return none();
+  const int64_t max_q = clamped(a[8]);
+  const float scale = (float)PyFloat_AsDouble(a[9]);
+  void* stream = PyLong_AsVoidPtr(a[11]);
+  if (PyErr_Occurred()) return nullptr;
+  if (max_q < 1 || !small(max_q) || words * 64 < max_q) return none();
+  int64_t total = -1, longest = -1;
+  if (PyList_CheckExact(a[7]) && PyList_GET_SIZE(a[7]) == seqs) {
+    total = longest = 0;
+    for (int64_t i = 0; i < seqs; ++i) {
+      PyObject* l = PyList_GET_ITEM(a[7], i);
+      if (!PyLong_CheckExact(l)) return none();
+      const int64_t len = clamped(l);
+      if (!small(len)) return none();
+      total += cdiv(len, 32);
+      longest = std::max(longest, cdiv(len, 32));
+    }
+  }
+  int32_t steps = g.tree_steps((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv, (int32_t)d,
+                               (int32_t)width, total, longest);
+  const int64_t widest = cdiv(width, 2);
+  int32_t ranges = steps > 0 ? (int32_t)cdiv(longest >= 0 ? std::min(longest, widest) : widest, steps) : 1;
+  at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16), ws;
+  if (ranges > 1) {
+    ws = optional_scratch(g.tree_bytes((int32_t)tokens, (int32_t)heads, (int32_t)d, ranges), *q);
+    if (!ws.defined()) ranges = 1;
+  }
+  if (ranges <= 1) steps = 0;
+  return launch(out, "bvllm_paged_tree_attention", [&] {
+    return g.tree(ptr(*q), q->stride(0), q->stride(1), ptr(*c), v_half(*c), c->stride(1), c->stride(2), c->stride(3),
+                  (int32_t)c->size(1), bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width,
+                  qsl->const_data_ptr<int32_t>(), seq->const_data_ptr<int32_t>(), ctx->const_data_ptr<int32_t>(),
+                  mask->const_data_ptr<int64_t>(), mask->stride(0), (int32_t)words, scale, ptr(out), out.stride(0),
+                  out.stride(1), (int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv,
+                  (int32_t)d, (int32_t)kPage, ws.defined() ? ptr(ws) : nullptr, steps, ranges, stream);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// The layers' caches of a list: their pointers, written to, and one of them. False: not plain ones of one shape and layout.
+struct Layers {
+  std::vector<void*> k, v;
+  const at::Tensor* one = nullptr;
+};
+bool plain_layers(PyObject* o, int64_t dev, Layers& l) {
+  if (!PyList_CheckExact(o)) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(o);
+  if (n < 1 || n > 4096) return false;
+  l.k.resize(n);
+  l.v.resize(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    const at::Tensor* c = plain(PyList_GET_ITEM(o, i), at::kBFloat16, dev);
+    if (!plain_cache(c)) return false;
+    if (i == 0) l.one = c;
+    else if (c->sizes() != l.one->sizes() || c->strides() != l.one->strides()) return false;
+  }
+  return l.one->size(2) == kPage && small(l.one->size(4));
+}
+void write_layers(PyObject* o, Layers& l) {
+  for (size_t i = 0; i < l.k.size(); ++i) {
+    const at::Tensor& c = THPVariable_Unpack(PyList_GET_ITEM(o, i));
+    l.k[i] = out_ptr(c);
+    l.v[i] = (char*)l.k[i] + c.stride(0) * 2;
+  }
+}
+
+PyObject* tuple_of(const at::Tensor& x, const at::Tensor& y, const at::Tensor& z) {
+  PyObject *p = THPVariable_Wrap(x), *q = THPVariable_Wrap(y), *r = THPVariable_Wrap(z);
+  PyObject* t = p && q && r ? PyTuple_Pack(3, p, q, r) : nullptr;
+  Py_XDECREF(p);
+  Py_XDECREF(q);
+  Py_XDECREF(r);
+  return t;
+}
+
+// (kv_caches, block_tables, query_start_loc, context_lens, draft, target, parents, max_path, device, stream)
+PyObject* fast_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 10) return none();
+  const int64_t dev = PyLong_AsLongLong(a[8]);
+  Layers l;
+  if (!plain_layers(a[0], dev, l)) return none();
+  const at::Tensor* bt = plain(a[1], at::kInt, dev);
+  const at::Tensor* qsl = plain(a[2], at::kInt, dev);
+  const at::Tensor* ctx = plain(a[3], at::kInt, dev);
+  const at::Tensor* draft = plain(a[4], at::kLong, dev);
+  const at::Tensor* target = plain(a[5], at::kLong, dev);
+  const at::Tensor* parents = plain(a[6], at::kInt, dev);
+  if (!rows_of(bt, 2)) return none();
+  for (const at::Tensor* v : {qsl, ctx, draft, target, parents})
+    if (!v || v->dim() != 1 || !v->is_contiguous()) return none();
+  const int64_t seqs = ctx->size(0), tokens = draft->size(0), width = bt->size(1);
+  if (seqs == 0 || tokens == 0 || width == 0 || qsl->size(0) != seqs + 1 || bt->size(0) < seqs) return none();
+  if (target->size(0) != tokens || parents->size(0) != tokens || !small(seqs) || !small(width)) return none();
+  if (!PyLong_CheckExact(a[7])) return none();
+  const int64_t max_path = clamped(a[7]);
+  void* stream = PyLong_AsVoidPtr(a[9]);
+  if (PyErr_Occurred()) return nullptr;
+  if (max_path < 1 || max_path > 4096) return none();
+  at::Tensor path = new_empty({seqs, max_path}, *ctx, at::kInt), accepted = new_empty({seqs}, *ctx, at::kInt),
+             following = new_empty({seqs}, *ctx, at::kLong);
+  write_layers(a[0], l);
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const at::Tensor& c = *l.one;
+    rc = g.commit(l.k.data(), l.v.data(), (int32_t)l.k.size(), c.stride(1), c.stride(2), c.stride(3),
+                  (int32_t)c.size(1), (int32_t)c.size(3), (int32_t)c.size(4), (int32_t)kPage,
+                  bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width, qsl->const_data_ptr<int32_t>(),
+                  ctx->const_data_ptr<int32_t>(), draft->const_data_ptr<int64_t>(), target->const_data_ptr<int64_t>(),
+                  parents->const_data_ptr<int32_t>(), path.mutable_data_ptr<int32_t>(),
+                  accepted.mutable_data_ptr<int32_t>(), following.mutable_data_ptr<int64_t>(), (int32_t)seqs,
+                  (int32_t)max_path, stream);
+  }
+  return rc == 0 ? tuple_of(path, accepted, following) : failed(rc, "bvllm_commit_draft_tree");
+  END_HANDLE_TH_ERRORS
+}
+
+// (logits, scores, num_beams, num_candidates, max_beams, max_candidates, device, stream)
+PyObject* fast_beam(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) return none();
+  const int64_t dev = PyLong_AsLongLong(a[6]);
+  const at::Tensor* x = plain(a[0], at::kBFloat16, dev);
+  const bool fp32 = x == nullptr;
+  if (fp32) x = plain(a[0], at::kFloat, dev);
+  const at::Tensor* scores = plain(a[1], at::kFloat, dev);
+  if (!rows_of(x, 2) || !scores || !scores->is_contiguous()) return none();
+  if (!PyLong_CheckExact(a[2]) || !PyLong_CheckExact(a[3])) return none();
+  const int64_t rows = x->size(0), vocab = x->size(1), beams = clamped(a[2]), cand = clamped(a[3]);
+  const int64_t max_beams = PyLong_AsLongLong(a[4]), max_cand = PyLong_AsLongLong(a[5]);
+  void* stream = PyLong_AsVoidPtr(a[7]);
+  if (PyErr_Occurred()) return nullptr;
+  if (rows == 0 || vocab == 0 || !small(rows) || !small(vocab) || scores->numel() != rows) return none();
+  if (beams < 1 || beams > max_beams || rows % beams || cand < 1 || cand > std::min(max_cand, beams * vocab)) return none();
+  const int64_t groups = rows / beams, row_stride = rows > 1 ? x->stride(0) : vocab;
+  at::Tensor s = new_empty({groups, cand}, *x, at::kFloat), b = new_empty({groups, cand}, *x, at::kLong),
+             t = new_empty({groups, cand}, *x, at::kLong);
+  at::Tensor ws = new_empty({g.beam_bytes((int32_t)rows, (int32_t)vocab) / 4}, *x, at::kFloat);
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    rc = g.beam(ptr(*x), row_stride, fp32 ? 1 : 0, scores->const_data_ptr<float>(), (int32_t)groups, (int32_t)beams,
+                (int32_t)vocab, (int32_t)cand, ptr(ws), s.mutable_data_ptr<float>(), b.mutable_data_ptr<int64_t>(),
+                t.mutable_data_ptr<int64_t>(), stream);
+  }
+  return rc == 0 ? tuple_of(s, b, t) : failed(rc, "bvllm_beam_select");
+  END_HANDLE_TH_ERRORS
+}
+
+// (kv_caches, block_tables, seq_lens, beams, max_beams, device, stream) -> True or None
+PyObject* fast_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) return none();
+  const int64_t dev = PyLong_AsLongLong(a[5]);
+  Layers l;
+  if (!plain_layers(a[0], dev, l)) return none();
+  const at::Tensor* bt = plain(a[1], at::kInt, dev);
+  const at::Tensor* lens = plain(a[2], at::kInt, dev);
+  const at::Tensor* beams = plain(a[3], at::kLong, dev);
+  if (!rows_of(bt, 2) || !lens || lens->dim() != 1 || !lens->is_contiguous()) return none();
+  if (!beams || beams->dim() != 2 || !beams->is_contiguous()) return none();
+  const int64_t groups = beams->size(0), k = beams->size(1), width = bt->size(1), rows = bt->size(0);
+  const int64_t max_beams = PyLong_AsLongLong(a[4]);
+  void* stream = PyLong_AsVoidPtr(a[6]);
+  if (PyErr_Occurred()) return nullptr;
+  if (groups < 1 || k < 1 || k > max_beams || rows != groups * k || lens->size(0) != rows) return none();
+  if (width == 0 || !small(groups) || !small(width) || (rows > 1 && bt->stride(0) < width)) return none();
+  write_layers(a[0], l);
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const at::Tensor& c = *l.one;
+    rc = g.reorder(l.k.data(), l.v.data(), (int32_t)l.k.size(), c.stride(1), c.stride(2), c.stride(3),
+                   (int32_t)c.size(1), (int32_t)c.size(3), (int32_t)c.size(4), (int32_t)kPage,
+                   bt->mutable_data_ptr<int32_t>(), rows > 1 ? bt->stride(0) : width, (int32_t)width,
+                   lens->const_data_ptr<int32_t>(), beams->const_data_ptr<int64_t>(), (int32_t)groups, (int32_t)k,
+                   stream);
+  }
+  if (rc != 0) return failed(rc, "bvllm_reorder_beams");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // ({name: address}, check): binds the library's entry points and what raises for a return code.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2 || !PyDict_Check(a[0]) || !PyCallable_Check(a[1]))
@@ -485,6 +704,7 @@ PyObject* names(PyObject*, PyObject*) {
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))fast_##name, METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     FAST(norm), FAST(silu), FAST(rope), FAST(auto_plan), FAST(decode), FAST(prefill), FAST(linear),
+    FAST(tree), FAST(commit), FAST(beam), FAST(reorder),
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr}, {"names", names, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast_calls", nullptr, -1, kMethods};

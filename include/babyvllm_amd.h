@@ -40,7 +40,7 @@ extern "C" {
 #endif
 
 /* ABI version of this header; bumped on any signature change. */
-#define BVLLM_ABI_VERSION 10
+#define BVLLM_ABI_VERSION 11
 
 #if defined(__GNUC__)
 #define BVLLM_API __attribute__((visibility("default")))
@@ -336,6 +336,102 @@ BVLLM_API int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t vo
                      const int64_t* positions, const float* cos_table, const float* sin_table,
                      int64_t max_positions, void* cos_out, void* sin_out, int32_t rows, int32_t hidden,
                      int32_t head_dim, void* stream);
+
+/*
+ * Attention of drafted token trees over the paged cache (no counterpart in the
+ * reference): the step of speculative decoding that scores every drafted token at once.
+ * Arguments as bvllm_paged_prefill's, with the rows of sequence s its drafted tokens
+ * (their K/V already appended at positions context_lens[s] + j) and tree_mask int64
+ * [T, mask_words] (row stride mask_stride) in place of the causal rule: row i attends the
+ * positions below context_lens[s], and context_lens[s] + j where bit j mod 64 of its word
+ * j / 64 is set, all below seq_lens[s] and inside the table. Its own bit is not implied. A
+ * row with no visible key outputs zeros; keys that a row does not see do not reach it,
+ * whatever they hold. mask_words must be at least max_query_len / 64 rounded up; scale
+ * must be positive and finite.
+ * range_steps > 0 cuts every sequence's keys into ranges of range_steps 32-key steps, each
+ * on work-groups of its own, with fp32 partials in workspace
+ * (bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, num_ranges) bytes) that a
+ * second launch adds; the last of the num_ranges ranges runs to the row's end. 0: one
+ * launch, no workspace. bvllm_tree_range_steps returns the range_steps to use (0: none)
+ * from host sizes alone: key_steps is ceil(seq_len / 32) summed over the sequences,
+ * longest_steps the largest of them, each -1 if unknown. They steer the choice only;
+ * results agree within the rounding of fp32 sums in another order.
+ */
+BVLLM_API int32_t bvllm_tree_range_steps(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks,
+                     int64_t key_steps, int64_t longest_steps);
+BVLLM_API int64_t bvllm_tree_workspace_bytes(int32_t num_tokens, int32_t num_heads, int32_t head_dim,
+                     int32_t num_ranges);
+BVLLM_API int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void* k_cache, const void* v_cache,
+                     int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
+                     int32_t num_blocks,
+                     const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                     const int32_t* query_start_loc, const int32_t* seq_lens,
+                     const int32_t* context_lens,
+                     const int64_t* tree_mask, int64_t mask_stride, int32_t mask_words, float scale,
+                     void* out, int64_t out_stride_t, int64_t out_stride_h,
+                     int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t block_size, void* workspace, int32_t range_steps, int32_t num_ranges,
+                     void* stream);
+
+/*
+ * Takes over a verified draft tree (no counterpart in the reference). For every sequence:
+ * the path from its node 0 (row query_start_loc[s]), at each node to the first later node
+ * whose parent it is (parents int32 [T], within the sequence, ascending: parents[c] < c;
+ * the root's is -1) and whose draft_tokens entry equals target_tokens at the node (both
+ * int64 [T]), of at most max_path nodes. path int32 [S, max_path] gets its node numbers
+ * (-1 behind them), accepted int32 [S] their number, following int64 [S] target_tokens at
+ * its last node. In every layer the K/V rows at positions context_lens[s] + path[s][i]
+ * then move to context_lens[s] + i. A sequence without rows gets 0 and -1.
+ * k_caches and v_caches are host arrays of num_layers device pointers, read during the
+ * call; all layers share the strides and num_blocks. Rows outside the table or the pool are
+ * not moved. max_path at most 4096.
+ */
+BVLLM_API int bvllm_commit_draft_tree(void* const* k_caches, void* const* v_caches, int32_t num_layers,
+                     int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
+                     int32_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                     const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                     const int32_t* query_start_loc, const int32_t* context_lens,
+                     const int64_t* draft_tokens, const int64_t* target_tokens, const int32_t* parents,
+                     int32_t* path, int32_t* accepted, int64_t* following,
+                     int32_t num_seqs, int32_t max_path, void* stream);
+
+/*
+ * Beam search's selection (no counterpart in the reference): the num_candidates best of
+ * scores[b] + logits[b][v] - logsumexp(logits[b]) over the num_beams rows of each group and
+ * the vocabulary, in descending order, equal ones by b * vocab + v. logits
+ * [num_groups * num_beams, vocab] bf16 (logits_fp32 = 0) or fp32 (1) with unit column
+ * stride, scores fp32. Totals are formed and compared in fp64. out_scores fp32, out_beams
+ * (within the group) and out_tokens int64, each [num_groups, num_candidates]. A beam whose
+ * score is not finite, or whose logits hold a NaN, a +inf or no finite value, gives totals
+ * of -inf. num_beams at most 32, num_candidates at most 64 and num_beams * vocab,
+ * num_beams * ceil(vocab / 2048) at most 8192. workspace holds
+ * bvllm_beam_workspace_bytes(rows, vocab) bytes.
+ */
+BVLLM_API int64_t bvllm_beam_workspace_bytes(int32_t rows, int32_t vocab);
+BVLLM_API int bvllm_beam_select(const void* logits, int64_t row_stride, int32_t logits_fp32, const float* scores,
+                     int32_t num_groups, int32_t num_beams, int32_t vocab, int32_t num_candidates,
+                     void* workspace, float* out_scores, int64_t* out_beams, int64_t* out_tokens,
+                     void* stream);
+
+/*
+ * The paged cache after a selection (no counterpart in the reference): beam b of each group
+ * of num_beams rows continues beam beams[b] of it (int64, within the group; an index outside
+ * it leaves the beam as it is). Beams of a group have one length, seq_lens of its first row.
+ * In block_tables (int32 [num_groups * num_beams, max_blocks], in place) the entries of the
+ * seq_len / 16 full pages are taken from the parent's row; the entry of the page being
+ * filled, which must be the beam's own, stays, and its seq_len mod 16 tokens are copied from
+ * the parent's page in every layer, all read before any is written. Layers as in
+ * bvllm_commit_draft_tree. num_beams at most 32.
+ */
+BVLLM_API int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches, int32_t num_layers,
+                     int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
+                     int32_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t block_size,
+                     int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                     const int32_t* seq_lens, const int64_t* beams,
+                     int32_t num_groups, int32_t num_beams, void* stream);
 
 #ifdef __cplusplus
 }
