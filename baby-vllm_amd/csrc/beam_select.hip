@@ -6,9 +6,9 @@
 // Bound by one pass over the logits (16 groups of 8 beams over 152,064 bf16 tokens are
 // 39 MB). Stage 1, one wave per piece of 2048 columns: the piece's maximum and its sum of
 // exponentials relative to it, nothing else. Stage 2, one work-group per group: the rows'
-// lse from the pieces; then the n best pieces by (total of the maximum, index) hold the n
-// best tokens (each of n better pieces has a better token), so only those are read again,
-// and of them only tokens that reach the n-th piece's maximum compete.
+// lse from the pieces; then a bar that n pieces' maxima reach, so that a token has to reach
+// it too. Only pieces that do are read again, some more than n of them, and few tokens in
+// them compete: each counts the better ones.
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -127,212 +127,267 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 
 constexpr double kNegInf64 = -__builtin_huge_val();
 
+// Candidates of the fast path: more than this many send the group to the exact one.
+constexpr int kMaxCand = kMaxPick * kMaxPick;
+static_assert(kMaxCand >= kMaxPick * kMaxPick, "the exact path: n tokens of n pieces");
+
+struct PickShared {
+  uint64_t keys[kBeamMaxPieces];  // the pieces' maxima as totals
+  uint64_t cand_key[kMaxCand];
+  uint32_t cand[kMaxCand];        // b * vocab + v < 2^24 (at most 8192 pieces of 2048)
+  double base[kBeamMaxBeams];
+  int count;
+};
+
+// Totals of beam b; -inf for a beam without a distribution (base -inf), whatever its logits.
+__device__ __forceinline__ double total_of_logit(double base, float x) {
+  return base == kNegInf64 ? kNegInf64 : (double)x + base;
+}
+
+template <typename T>
+__device__ __forceinline__ void load_piece(const BeamSelectArgs& a, int64_t row, int piece, bool live, Piece<T>& p) {
+  p.load(reinterpret_cast<const T*>(a.logits) + row * a.row_stride + (int64_t)piece * kPiece, a.vocab - piece * kPiece);
+  if (!live) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) p.v[i] = kNegInf;
+  }
+}
+
+// Wave-wide: exclusive prefix sum, and the sum in `all`.
+__device__ __forceinline__ int wave_prefix(int mine, int& all) {
+  int upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int t = __shfl_up(upto, d, 64);
+    if (lane_id() >= d) upto += t;
+  }
+  all = __shfl(upto, 63, 64);
+  return upto - mine;
+}
+
+// The piece's n best tokens that reach the bar, whatever there is of equal ones. The lane's
+// elements to take, as bits.
+template <typename T>
+__device__ __forceinline__ uint32_t best_of_piece(const Piece<T>& p, double base, uint64_t bar, int left, int n) {
+  uint32_t over = 0, even = 0;  // the lane's elements above the bar, and at it
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    if (Piece<T>::column(i) < left) {
+      const uint64_t k = order_of(total_of_logit(base, p.v[i]));
+      over |= (uint32_t)(k > bar) << i;
+      even |= (uint32_t)(k == bar) << i;
+    }
+  }
+  auto wave_count = [&](uint32_t bits) {
+    return wave_reduce(__builtin_popcount(bits), [](int x, int y) { return x + y; });
+  };
+  int n_over = wave_count(over);
+  if (n_over > n) {
+    // The piece alone holds more than n above the bar: its own bar is its n-th logit, found
+    // bit by bit from the top (the largest value that at least n reach).
+    const uint32_t open = over;
+    uint32_t nth = 0;
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t probe = nth | (1u << bit);
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) mine += ((open >> i) & 1) && order_of(p.v[i]) >= probe;
+      const int reach = wave_reduce(mine, [](int x, int y) { return x + y; });
+      if (reach >= n) nth = probe;
+      if (reach == n) break;
+    }
+    over = even = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      over |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) > nth) << i;
+      even |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) == nth) << i;
+    }
+    n_over = wave_count(over);
+  }
+  // Elements at the bar are equal: the first of them by column, as many as could be taken
+  // (vectors in order, lanes in order within one).
+  int want = max(0, n - n_over);
+  if (wave_count(even) > want) {
+    constexpr int VEC = Piece<T>::VEC;
+    uint32_t keep = 0;
+    for (int k = 0; k < Piece<T>::LOADS; ++k) {
+      uint32_t bits = (even >> (k * VEC)) & ((1u << VEC) - 1);
+      int all;
+      int room = max(0, want - wave_prefix(__builtin_popcount(bits), all));
+      while (bits != 0 && room > 0) {
+        keep |= (bits & -bits) << (k * VEC);
+        bits &= bits - 1;
+        --room;
+      }
+      want = max(0, want - all);
+    }
+    even = keep;
+  }
+  return over | even;
+}
+
+// The exact choice of pieces and tokens, for groups whose candidates overflow: many equal
+// totals at the bar (masked vocabularies, few distinct logits), or many good tokens in one piece.
+template <typename T>
+__device__ __forceinline__ void pick_exact(const BeamSelectArgs& a, int pieces, PickShared& sh) {
+  const int lane = lane_id(), w = wave_id();
+  const int n = a.num_candidates, M = a.num_beams * pieces;
+  const int64_t row0 = (int64_t)blockIdx.x * a.num_beams;
+  // The n-th best piece's key (0 with fewer pieces), bit by bit; then pieces above it, and the
+  // first ones at it. Every wave finds the same.
+  uint64_t bar = 0;
+  int above = M;
+  if (M > n) {
+    auto reach = [&](uint64_t k) {
+      int c = 0;
+      for (int i0 = 0; i0 < M; i0 += 64)
+        c += __popcll(__builtin_amdgcn_ballot_w64(i0 + lane < M && sh.keys[min(i0 + lane, M - 1)] >= k));
+      return c;
+    };
+    for (int bit = 63; bit >= 0; --bit) {
+      const uint64_t probe = bar | (1ull << bit);
+      if (reach(probe) >= n) bar = probe;
+    }
+    above = bar == ~0ull ? 0 : reach(bar + 1);
+  }
+  int found = 0, found_even = 0;
+  for (int i0 = 0; i0 < M; i0 += 64) {
+    const uint64_t key = i0 + lane < M ? sh.keys[i0 + lane] : 0;
+    const bool in = i0 + lane < M;
+    uint64_t over = __builtin_amdgcn_ballot_w64(in && (M <= n || key > bar));
+    const uint64_t even = M <= n ? 0 : __builtin_amdgcn_ballot_w64(in && key == bar);
+    for (uint64_t left = over | even; left != 0; left &= left - 1) {
+      const int l = (int)__builtin_ctzll(left);
+      if (((even >> l) & 1) && found_even++ >= n - above) continue;
+      if ((found++ & (kPickWaves - 1)) != w) continue;
+      const int i = i0 + l, b = i / pieces, piece = i - b * pieces;
+      Piece<T> p;
+      load_piece(a, row0 + b, piece, sh.base[b] != kNegInf64, p);
+      const uint32_t taken = best_of_piece(p, sh.base[b], bar, a.vocab - piece * kPiece, n);
+      int all;
+      int at = wave_prefix(__builtin_popcount(taken), all);
+      int start = 0;
+      if (lane == 0) start = atomicAdd(&sh.count, all);
+      at += __shfl(start, 0, 64);
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if ((taken >> e) & 1) {
+          sh.cand_key[at] = order_of(total_of_logit(sh.base[b], p.v[e]));
+          sh.cand[at++] = (uint32_t)(b * a.vocab + piece * kPiece + Piece<T>::column(e));
+        }
+    }
+  }
+}
+
 template <typename T>
 __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs a, int pieces) {
-  constexpr int kMaxKeys = kBeamMaxPieces;
-  // Keys of the pieces, later the competing tokens (key and flat index).
-  __shared__ __attribute__((aligned(16))) uint64_t store[kMaxKeys];
-  static_assert(kMaxKeys >= 2 * kMaxPick * kMaxPick, "n tokens of n pieces");
-  __shared__ uint16_t ahead[kMaxKeys];  // pieces that reach the lane threshold
-  __shared__ double base[kBeamMaxBeams];
-  __shared__ uint64_t lane_key[64];
-  __shared__ int lane_piece[64], lane_rank[64], chosen[kMaxPick], counts[2];
-  uint64_t* keys = store;
-
+  __shared__ PickShared sh;
   const int tid = (int)threadIdx.x, lane = lane_id(), w = wave_id();
   const int K = a.num_beams, n = a.num_candidates, M = K * pieces;
   const int64_t row0 = (int64_t)blockIdx.x * K;
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + row0 * pieces;
-  if (tid < 2) counts[tid] = 0;
-  if (tid < 64) lane_rank[tid] = 0;
+  if (tid == 0) sh.count = 0;
 
-  // base_b = score_b - lse_b, in fp64 from the largest piece maximum on.
+  // A wave per beam: base_b = score_b - lse_b, in fp64 from the pieces' sums on, and the
+  // keys of its pieces.
   for (int b = w; b < K; b += kPickWaves) {
+    const float score = a.scores[row0 + b];
     float m = kNegInf;
     for (int i = lane; i < pieces; i += 64) m = fmax_prop(m, stats[b * pieces + i].x);
     m = wave_max(m);
     double sum = 0.0;
     for (int i = lane; i < pieces; i += 64) {
       const float2 x = stats[b * pieces + i];
-      if (x.x != kNegInf) sum += (double)x.y * exp((double)x.x - (double)m);
+      if (x.x != kNegInf) sum += (double)(x.y * fast_exp2((x.x - m) * kLog2e));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
-    if (lane == 0) {
-      const float score = a.scores[row0 + b];
-      const bool live = fabsf(m) < __builtin_huge_valf() && fabsf(score) < __builtin_huge_valf();
-      base[b] = live ? (double)score - ((double)m + log(sum)) : kNegInf64;
-    }
+    const bool live = fabsf(m) < __builtin_huge_valf() && fabsf(score) < __builtin_huge_valf();
+    const double base = live ? (double)score - ((double)m + log(sum)) : kNegInf64;
+    if (lane == 0) sh.base[b] = base;
+    for (int i = lane; i < pieces; i += 64) sh.keys[b * pieces + i] = order_of(total_of_logit(base, stats[b * pieces + i].x));
   }
   __syncthreads();
-  // (base is -inf for a beam without a distribution, whatever its logits.)
-  auto total = [&](int b, float x) { return base[b] == kNegInf64 ? kNegInf64 : (double)x + base[b]; };
-  for (int i = tid; i < M; i += kPickThreads) keys[i] = order_of(total(i / pieces, stats[i].x));
-  __syncthreads();
 
-  // A threshold that at least n pieces reach and few others: lane l of a wave takes the best
-  // of pieces l, l + 64, ...; the n-th best of those 64.
-  int n_chosen = M;
+  // The bar: a total that at least n pieces reach, and few others. Lane l takes the best of
+  // pieces l, l + 64, ...; the bar is the n-th best of those 64. Every wave finds the same.
+  uint64_t bar = 0;
   if (M > n) {
-    n_chosen = n;
-    if (w == 0) {
-      uint64_t k = 0;
-      int at = 0x7fffffff;
-      for (int i = lane; i < M; i += 64)
-        if (at == 0x7fffffff || keys[i] > k) {
-          k = keys[i];
-          at = i;
-        }
-      lane_key[lane] = k;
-      lane_piece[lane] = at;
-    }
-    __syncthreads();
-    {
-      const uint64_t k = lane_key[lane];
-      const int at = lane_piece[lane];
-      int better = 0;
+    uint64_t best = 0;
+    for (int i = lane; i < M; i += 64) best = max(best, sh.keys[i]);
+    int better = 0;
 #pragma unroll
-      for (int q = 0; q < 64 / kPickWaves; ++q) {
-        const int o = w * (64 / kPickWaves) + q;
-        better += lane_key[o] > k || (lane_key[o] == k && lane_piece[o] < at);
-      }
-      if (better) atomicAdd(&lane_rank[lane], better);
+    for (int o = 0; o < 64; ++o) {
+      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, o);
+      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), o);
+      const uint64_t other = ((uint64_t)hi << 32) | lo;
+      better += other > best || (other == best && o < lane);
     }
-    __syncthreads();
-    const uint64_t at_rank = __builtin_amdgcn_ballot_w64(lane_rank[lane] == n - 1);
-    const int tl = (int)__builtin_ctzll(at_rank);
-    const uint64_t tk = lane_key[tl];
-    const int tp = lane_piece[tl];
-    for (int i = tid; i < M; i += kPickThreads)
-      if (keys[i] > tk || (keys[i] == tk && i <= tp)) ahead[atomicAdd(&counts[0], 1)] = (uint16_t)i;
-    __syncthreads();
-    const int c = counts[0];
-    for (int e = tid; e < c; e += kPickThreads) {
-      const int i = ahead[e];
-      const uint64_t k = keys[i];
-      int rank = 0;
-      for (int o = 0; o < c; ++o) {
-        const int p = ahead[o];
-        rank += keys[p] > k || (keys[p] == k && p < i);
-      }
-      if (rank < n) chosen[rank] = i;
-    }
-  } else if (tid < M) {
-    chosen[tid] = tid;
+    const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(better == n - 1));
+    bar = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), l) << 32) |
+          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, l);
   }
-  __syncthreads();
-  // With n pieces a token has to reach the n-th one's maximum.
-  const uint64_t bar = M > n ? keys[chosen[n - 1]] : 0;
-  __syncthreads();
 
-  // The chosen pieces' tokens that reach the bar: (key, flat index) pairs. At most n of a
-  // piece, its best ones.
-  uint64_t* cand = store;
-  for (int e = w; e < n_chosen; e += kPickWaves) {
-    const int b = chosen[e] / pieces, piece = chosen[e] - b * pieces;
-    Piece<T> p;
-    p.load(reinterpret_cast<const T*>(a.logits) + (row0 + b) * a.row_stride + (int64_t)piece * kPiece,
-           a.vocab - piece * kPiece);
-    const int left = a.vocab - piece * kPiece;
-    if (base[b] == kNegInf64) {  // no distribution: all alike, whatever they hold
+  // The pieces that reach it, dealt to the waves; their tokens that do are candidates. A
+  // conservative fp32 threshold sorts out nearly all others.
+  const double bar_total = bar == 0 ? kNegInf64 : total_of(bar);
+  int found = 0;
+  for (int i0 = 0; i0 < M; i0 += 64) {
+    const bool in = i0 + lane < M && sh.keys[min(i0 + lane, M - 1)] >= bar;
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(in); left != 0; left &= left - 1) {
+      if ((found++ & (kPickWaves - 1)) != w) continue;
+      const int i = i0 + (int)__builtin_ctzll(left), b = i / pieces, piece = i - b * pieces;
+      const int columns = a.vocab - piece * kPiece;
+      const double base = sh.base[b];
+      Piece<T> p;
+      load_piece(a, row0 + b, piece, base != kNegInf64, p);
+      const float at_bar = base == kNegInf64 ? kNegInf : (float)(bar_total - base);
+      const float threshold = at_bar - fabsf(at_bar) * 0x1p-22f - 0x1p-126f;
+      int all = 0;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) p.v[i] = kNegInf;
-    }
-    uint32_t over = 0, even = 0;  // the lane's elements above the bar, and at it
+      for (int e = 0; e < 32; ++e) all += __popcll(__builtin_amdgcn_ballot_w64(p.v[e] >= threshold));
+      int at = 0;
+      if (lane == 0) at = atomicAdd(&sh.count, all);
+      at = uniform(at);
+      if (at + all > kMaxCand) continue;  // (the count tells everybody)
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      if (Piece<T>::column(i) < left) {
-        const uint64_t k = order_of(total(b, p.v[i]));
-        over |= (uint32_t)(k > bar) << i;
-        even |= (uint32_t)(k == bar) << i;
-      }
-    }
-    auto wave_count = [&](uint32_t bits) {
-      return wave_reduce(__builtin_popcount(bits), [](int x, int y) { return x + y; });
-    };
-    int n_over = wave_count(over);
-    if (n_over > n) {
-      // The piece alone holds more than n above the bar: its own bar is its n-th logit, found
-      // bit by bit from the top (the largest value that at least n reach).
-      const uint32_t open = over;
-      uint32_t nth = 0;
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t probe = nth | (1u << bit);
-        int mine = 0;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) mine += ((open >> i) & 1) && order_of(p.v[i]) >= probe;
-        const int reach = wave_reduce(mine, [](int x, int y) { return x + y; });
-        if (reach >= n) nth = probe;
-        if (reach == n) break;
-      }
-      over = even = 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        over |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) > nth) << i;
-        even |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) == nth) << i;
-      }
-      n_over = wave_count(over);
-      if (n_over == n) even = 0;
-    }
-    // Elements at the bar are equal: the first of them by column, as many as could be taken.
-    int want_even = n_over >= n ? 0 : n - n_over;
-    if (wave_count(even) > want_even) {
-      // Vectors in order, lanes in order within one.
-      uint32_t keep = 0;
-#pragma unroll
-      for (int k = 0; k < Piece<T>::LOADS; ++k) {
-        constexpr int VEC = Piece<T>::VEC;
-        uint32_t bits = (even >> (k * VEC)) & ((1u << VEC) - 1);
-        const int mine = __builtin_popcount(bits);
-        int before = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-          const int t = __shfl_up(before, d, 64);
-          if (lane >= d) before += t;
+      for (int e = 0; e < 32; ++e) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(p.v[e] >= threshold);
+        if (hit != 0) {
+          if ((hit >> lane) & 1) {
+            // Columns behind the row's end, which read as -inf, and those below the bar drop out.
+            const int c = Piece<T>::column(e), slot = at + __popcll(hit & ((1ull << lane) - 1));
+            const uint64_t k = order_of(total_of_logit(base, p.v[e]));
+            sh.cand_key[slot] = c < columns ? k : 0;
+            sh.cand[slot] = c < columns && k >= bar ? (uint32_t)(b * a.vocab + piece * kPiece + c) : ~0u;
+          }
+          at += __popcll(hit);
         }
-        const int all = __shfl(before, 63, 64);
-        before -= mine;
-        int room = max(0, want_even - before);
-        while (bits != 0 && room > 0) {
-          keep |= (bits & -bits) << (k * VEC);
-          bits &= bits - 1;
-          --room;
-        }
-        want_even = max(0, want_even - all);
       }
-      even = keep;
     }
-    const uint32_t taken = over | even;
-    const int mine = __builtin_popcount(taken);
-    int before = mine;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int t = __shfl_up(before, d, 64);
-      if (lane >= d) before += t;
-    }
-    int at = 0;
-    if (lane == 63) at = atomicAdd(&counts[1], before);
-    at = __shfl(at, 63, 64) + before - mine;
-#pragma unroll
-    for (int i = 0; i < 32; ++i)
-      if ((taken >> i) & 1) {
-        cand[2 * at] = order_of(total(b, p.v[i]));
-        cand[2 * at + 1] = (uint64_t)((int64_t)b * a.vocab + (int64_t)piece * kPiece + Piece<T>::column(i));
-        ++at;
-      }
   }
   __syncthreads();
-  const int c = counts[1];
+  if (sh.count > kMaxCand) {
+    __syncthreads();
+    if (tid == 0) sh.count = 0;
+    __syncthreads();
+    pick_exact<T>(a, pieces, sh);
+    __syncthreads();
+  }
+
+  const int c = sh.count;
   const int64_t out0 = (int64_t)blockIdx.x * n;
   for (int e = tid; e < c; e += kPickThreads) {
-    const uint64_t k = cand[2 * e], flat = cand[2 * e + 1];
+    const uint64_t k = sh.cand_key[e];
+    const uint32_t flat = sh.cand[e];
+    if (flat == ~0u) continue;
     int rank = 0;
-    for (int o = 0; o < c; ++o) rank += cand[2 * o] > k || (cand[2 * o] == k && cand[2 * o + 1] < flat);
+    for (int o = 0; o < c; ++o) rank += sh.cand_key[o] > k || (sh.cand_key[o] == k && sh.cand[o] < flat);
     if (rank < n) {
-      const int64_t beam = (int64_t)(flat / (uint64_t)a.vocab);
+      const uint32_t beam = flat / (uint32_t)a.vocab;
       a.out_scores[out0 + rank] = (float)total_of(k);
       a.out_beams[out0 + rank] = beam;
-      a.out_tokens[out0 + rank] = (int64_t)flat - beam * a.vocab;
+      a.out_tokens[out0 + rank] = flat - beam * (uint32_t)a.vocab;
     }
   }
 }
