@@ -46,7 +46,7 @@ struct Piece {
     for (int k = 0; k < LOADS; ++k) {
       const int c = column(k * VEC);
       if (c + VEC <= left) {
-        raw[k] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(x + c));
+        raw[k] = *reinterpret_cast<const u32x4_any*>(x + c);
       } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -136,6 +136,7 @@ struct PickShared {
   uint64_t cand_key[kMaxCand];
   uint32_t cand[kMaxCand];        // b * vocab + v < 2^24 (at most 8192 pieces of 2048)
   double base[kBeamMaxBeams];
+  int better[64];
   int count;
 };
 
@@ -287,6 +288,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   const int64_t row0 = (int64_t)blockIdx.x * K;
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + row0 * pieces;
   if (tid == 0) sh.count = 0;
+  if (tid < 64) sh.better[tid] = 0;
 
   // A wave per beam: base_b = score_b - lse_b, in fp64 from the pieces' sums on, and the
   // keys of its pieces.
@@ -315,15 +317,18 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   if (M > n) {
     uint64_t best = 0;
     for (int i = lane; i < M; i += 64) best = max(best, sh.keys[i]);
+    // Each wave compares every lane's best with a few of them.
     int better = 0;
 #pragma unroll
-    for (int o = 0; o < 64; ++o) {
-      const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, o);
-      const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), o);
-      const uint64_t other = ((uint64_t)hi << 32) | lo;
+    for (int q = 0; q < 64 / kPickWaves; ++q) {
+      const int o = w * (64 / kPickWaves) + q;
+      const uint64_t other = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), o) << 32) |
+                             (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, o);
       better += other > best || (other == best && o < lane);
     }
-    const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(better == n - 1));
+    if (better != 0) atomicAdd(&sh.better[lane], better);
+    __syncthreads();
+    const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(sh.better[lane] == n - 1));
     bar = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), l) << 32) |
           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, l);
   }
