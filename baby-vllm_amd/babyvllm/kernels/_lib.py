@@ -125,7 +125,7 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32, _i32,  # m, n, k, gated, eager
         _p, _p,                     # workspace, stream
     ]),
-    "bvllm_tree_range_steps": (ctypes.c_int32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64]),
+    "bvllm_tree_split_tiles": (ctypes.c_int32, [_i32, _i32, _i32, _i32, _i32, _i32, _i32, _i64, _i64]),
     "bvllm_tree_workspace_bytes": (ctypes.c_int64, [_i32, _i32, _i32, _i32]),
     "bvllm_paged_tree_attention": (ctypes.c_int, [
         _p, _i64, _i64,             # q
@@ -137,7 +137,7 @@ SIGNATURES = {
         _p, _i64, _i64,             # out
         _i32, _i32, _i32,           # num_seqs, num_tokens, max_query_len
         _i32, _i32, _i32, _i32,     # H, Hkv, D, block_size
-        _p, _i32, _i32, _p,         # workspace, range_steps, num_ranges, stream
+        _p, _i32, _i32, _p,         # workspace, split_tiles, num_ranges, stream
     ]),
     "bvllm_commit_draft_tree": (ctypes.c_int, [
         _p, _p, _i32,               # k_caches, v_caches, num_layers

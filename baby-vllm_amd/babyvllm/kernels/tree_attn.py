@@ -10,11 +10,11 @@ own bit among them. ``ancestor_masks`` makes the words (and the depths, which gi
 rotary positions) from each node's parent.
 
 A row that sees no key gives zeros, and a key that a row does not see does not reach it,
-whatever it holds. Rows of ``q`` behind the last sequence are not computed. Few rows
-behind long contexts run in key ranges chosen from the step's host lists: the last bits of
-a row can depend on the other sequences of the step, within the rounding of fp32 sums in
-another order. They take fp32 scratch (at most 64 MiB); without the memory for it the
-launch that needs none runs.
+whatever it holds. Rows of ``q`` behind the last sequence are not computed. Long contexts
+run in key ranges chosen from the step's host lists: the last bits of a row can depend on
+the other sequences of the step, within the rounding of fp32 sums in another order. They
+take fp32 scratch (at most 64 MiB); without the memory for it the launch that needs none
+runs.
 """
 
 from __future__ import annotations
@@ -23,7 +23,7 @@ import torch
 
 from babyvllm.kernels import _lib
 
-_STEP = 32  # keys
+_TILE = 64  # keys
 
 
 def ancestor_masks(parents, words: int | None = None):
@@ -54,13 +54,13 @@ def ancestor_masks(parents, words: int | None = None):
             torch.tensor(depths, dtype=torch.int64))
 
 
-def _key_steps(md, num_seqs):
-    """(32-key steps of all sequences, of the longest) from the host list, -1 for each without it."""
+def _key_tiles(md, num_seqs):
+    """(64-key tiles of all sequences, of the longest) from the host list, -1 for each without it."""
     seq = getattr(md, "seq_lens_cpu", None)
     if seq is None or len(seq) != num_seqs:
         return -1, -1
-    steps = [(max(int(n), 0) + _STEP - 1) // _STEP for n in seq]
-    return sum(steps), max(steps, default=0)
+    tiles = [(max(int(n), 0) + _TILE - 1) // _TILE for n in seq]
+    return sum(tiles), max(tiles, default=0)
 
 
 def paged_tree_attention(q, kv_cache, md, scale):
@@ -114,17 +114,16 @@ def paged_tree_attention(q, kv_cache, md, scale):
     qsl, seq_lens, ctx_lens = md.query_start_loc.contiguous(), md.seq_lens.contiguous(), md.context_lens.contiguous()
     h = _lib.lib()
     with torch.cuda.device(q.device):
-        total, longest = _key_steps(md, num_seqs)
-        steps = h.bvllm_tree_range_steps(num_seqs, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
+        total, longest = _key_tiles(md, num_seqs)
+        split = h.bvllm_tree_split_tiles(num_seqs, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
                                          bt.shape[1], total, longest)
-        ranges, workspace = 1, None
-        if steps > 0:
-            widest = -(-bt.shape[1] // 2)
-            ranges = -(-(min(longest, widest) if longest >= 0 else widest) // steps)
-            nbytes = h.bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, ranges)
-            workspace = _lib.optional_scratch(nbytes, q.device) if nbytes > 0 else None
+        ranges, workspace = 0, None
+        if split > 0:
+            ranges = h.bvllm_prefill_ranges(bt.shape[1], split, longest)
+            workspace = _lib.optional_scratch(h.bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, ranges),
+                                              q.device)
             if workspace is None:
-                steps, ranges = 0, 1
+                split = 0
         rc = h.bvllm_paged_tree_attention(
             q.data_ptr(), q.stride(0), q.stride(1),
             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
@@ -134,6 +133,6 @@ def paged_tree_attention(q, kv_cache, md, scale):
             mask.data_ptr(), mask.stride(0), mask.shape[1], float(scale),
             out.data_ptr(), out.stride(0), out.stride(1),
             num_seqs, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim, page,
-            None if workspace is None else workspace.data_ptr(), steps, ranges, _lib.stream_handle(q.device))
+            None if workspace is None else workspace.data_ptr(), split, ranges, _lib.stream_handle(q.device))
     _lib.check(rc, "bvllm_paged_tree_attention")
     return out

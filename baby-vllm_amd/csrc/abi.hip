@@ -418,22 +418,22 @@ extern "C" int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t v
   return (int)embed_rows(a, (hipStream_t)stream);
 }
 
-extern "C" int32_t bvllm_tree_range_steps(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+extern "C" int32_t bvllm_tree_split_tiles(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                          int32_t max_blocks, int64_t key_steps, int64_t longest_steps) {
+                                          int32_t max_blocks, int64_t key_tiles, int64_t longest_tiles) {
   if (num_seqs < 1 || num_tokens < 1 || max_query_len < 1 || max_blocks < 1) return 0;
   if (!valid_heads(num_heads, num_kv_heads) || (head_dim != 64 && head_dim != 128)) return 0;
   TreeArgs a{};
   a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.max_query_len = max_query_len;
   a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
   a.max_blocks = max_blocks;
-  return tree_range_steps(a, key_steps, longest_steps);
+  return tree_split_tiles(a, key_tiles, longest_tiles);
 }
 
 extern "C" int64_t bvllm_tree_workspace_bytes(int32_t num_tokens, int32_t num_heads, int32_t head_dim,
                                               int32_t num_ranges) {
-  if (num_tokens < 1 || num_heads < 1 || head_dim < 1 || num_ranges < 2) return 0;
-  return tree_range_bytes(num_ranges, num_tokens, num_heads, head_dim);
+  if (num_tokens < 1 || num_heads < 1 || head_dim < 1 || num_ranges < 1) return 0;
+  return prefill_range_floats(num_ranges, num_tokens, num_heads, head_dim) * (int64_t)sizeof(float);
 }
 
 extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
@@ -448,7 +448,7 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
                                           void* out, int64_t out_stride_t, int64_t out_stride_h,
                                           int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                          int32_t block_size, void* workspace, int32_t range_steps,
+                                          int32_t block_size, void* workspace, int32_t split_tiles,
                                           int32_t num_ranges, void* stream) {
   if (num_seqs < 0 || num_tokens < 0 || max_query_len < 0) return kBad;
   if (!valid_heads(num_heads, num_kv_heads)) return kBad;
@@ -464,10 +464,10 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
   // Offsets inside one page are 32-bit, and so are (token, head) pairs.
   if ((int64_t)16 * cache_stride_tok > 0x3fffffff || (int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
   if (mask_words < 1 || (int64_t)mask_words * 64 < max_query_len || mask_stride < mask_words) return kBad;
-  if (range_steps < 0 || range_steps > (1 << 28)) return kBad;
-  if (range_steps > 0 && (num_ranges < 1 || num_ranges > tree_max_ranges(max_blocks, range_steps))) return kBad;
-  const int32_t ranges = range_steps > 0 ? num_ranges : 1;
-  if (ranges > 1 && (!workspace || !aligned16(workspace))) return kBad;
+  if (split_tiles < 0 || split_tiles > (1 << 20)) return kBad;
+  // (More ranges than the table's tiles make would stay empty.)
+  if (split_tiles > 0 && (num_ranges < 1 || num_ranges > prefill_ranges(max_blocks, split_tiles, -1))) return kBad;
+  if (split_tiles > 0 && (!workspace || !aligned16(workspace))) return kBad;
   TreeArgs a{};
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
   a.k_cache = k_cache; a.v_cache = v_cache;
@@ -480,11 +480,11 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
   a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
   a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.max_query_len = max_query_len;
   a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
-  a.range_steps = range_steps > 0 ? range_steps : 1 << 28;
-  a.num_ranges = ranges;
-  if (ranges > 1) {
+  if (split_tiles > 0) {
+    a.split_tiles = split_tiles;
+    a.num_ranges = num_ranges;
     a.part_out = reinterpret_cast<float*>(workspace);
-    a.part_ml = a.part_out + (int64_t)ranges * num_tokens * num_heads * head_dim;
+    a.part_ml = a.part_out + (int64_t)num_ranges * num_tokens * num_heads * head_dim;
   }
   return (int)paged_tree_attention(a, (hipStream_t)stream);
 }

@@ -148,23 +148,16 @@ struct TreeArgs {
   void* out;      int64_t o_st, o_sh;      // [T, H, D]
   int32_t num_seqs, num_tokens, max_query_len;
   int32_t num_heads, num_kv_heads, head_dim;
-  // Key ranges: 32-key steps per range, their number (the last one runs to the row's end)
-  // and, with more than one, their fp32 partials.
-  int32_t range_steps, num_ranges;
+  // The context on launches of its own (split_tiles > 0): 64-key tiles per range, the most
+  // ranges a sequence has, and their fp32 partials.
+  int32_t split_tiles, num_ranges;
   float* part_out;                         // [num_ranges, T, H, D], unnormalized
-  float* part_ml;                          // [num_ranges, T, H, 2]: maximum (log2 units), sum
+  float* part_ml;                          // [num_ranges, T, H, 2]: reference (log2 units), sum
 };
 hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
-// 32-key steps per range for the batch's shape, 0 for whole rows (key_steps: those of all
-// sequences, longest_steps: of the longest; < 0 if unknown).
-int32_t tree_range_steps(const TreeArgs& a, int64_t key_steps, int64_t longest_steps);
-inline int64_t tree_range_bytes(int32_t num_ranges, int32_t num_tokens, int32_t num_heads, int32_t head_dim) {
-  return (int64_t)num_ranges * num_tokens * num_heads * (head_dim + 2) * (int64_t)sizeof(float);
-}
-// Ranges of range_steps steps that a table of max_blocks pages can hold.
-inline int32_t tree_max_ranges(int32_t max_blocks, int32_t range_steps) {
-  return (int32_t)((((int64_t)max_blocks + 1) / 2 + range_steps - 1) / range_steps);
-}
+// 64-key tiles per range of the context's launch for the batch's shape, 0 without one
+// (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
+int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles);
 
 // The K and V caches of several layers, all of one shape.
 constexpr int kCacheSetLayers = 64;        // of one launch
@@ -288,6 +281,10 @@ enum TuneKnob {
 int tuning(int knob);
 int set_tuning(int knob, int value);
 hipError_t paged_prefill(const PrefillArgs& a, hipStream_t stream);
+// The context part of a draft tree step on the prefill kernel: every row over the whole
+// 64-key tiles below its sequence's context length, in at most num_ranges ranges of split_tiles
+// tiles whose partials (part_out, part_ml) the caller adds.
+hipError_t paged_prefill_context(const PrefillArgs& a, hipStream_t stream);
 // Key ranges of a prefill launch: tiles per range (0: no split) for the batch's shape
 // (key_tiles: 64-key tiles its 128-column blocks walk per KV head, longest_tiles: those of
 // its longest sequence of more than one query; < 0 if unknown).

@@ -42,7 +42,7 @@ struct Entry {
   decltype(&bvllm_silu_mul) silu = nullptr;
   decltype(&bvllm_linear_workspace_bytes) linear_bytes = nullptr;
   decltype(&bvllm_linear) linear = nullptr;
-  decltype(&bvllm_tree_range_steps) tree_steps = nullptr;
+  decltype(&bvllm_tree_split_tiles) tree_tiles = nullptr;
   decltype(&bvllm_tree_workspace_bytes) tree_bytes = nullptr;
   decltype(&bvllm_paged_tree_attention) tree = nullptr;
   decltype(&bvllm_commit_draft_tree) commit = nullptr;
@@ -71,7 +71,7 @@ const BindName kNames[] = {
     {"bvllm_silu_mul", (void**)&g.silu},
     {"bvllm_linear_workspace_bytes", (void**)&g.linear_bytes},
     {"bvllm_linear", (void**)&g.linear},
-    {"bvllm_tree_range_steps", (void**)&g.tree_steps},
+    {"bvllm_tree_split_tiles", (void**)&g.tree_tiles},
     {"bvllm_tree_workspace_bytes", (void**)&g.tree_bytes},
     {"bvllm_paged_tree_attention", (void**)&g.tree},
     {"bvllm_commit_draft_tree", (void**)&g.commit},
@@ -500,27 +500,25 @@ PyObject* fast_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!PyLong_CheckExact(l)) return none();
       const int64_t len = clamped(l);
       if (!small(len)) return none();
-      total += cdiv(len, 32);
-      longest = std::max(longest, cdiv(len, 32));
+      total += cdiv(len, 64);
+      longest = std::max(longest, cdiv(len, 64));
     }
   }
-  int32_t steps = g.tree_steps((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv, (int32_t)d,
+  int32_t split = g.tree_tiles((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv, (int32_t)d,
                                (int32_t)width, total, longest);
-  const int64_t widest = cdiv(width, 2);
-  int32_t ranges = steps > 0 ? (int32_t)cdiv(longest >= 0 ? std::min(longest, widest) : widest, steps) : 1;
+  const int32_t ranges = split > 0 ? g.ranges((int32_t)width, split, longest) : 0;
   at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16), ws;
-  if (ranges > 1) {
+  if (split > 0) {
     ws = optional_scratch(g.tree_bytes((int32_t)tokens, (int32_t)heads, (int32_t)d, ranges), *q);
-    if (!ws.defined()) ranges = 1;
+    if (!ws.defined()) split = 0;
   }
-  if (ranges <= 1) steps = 0;
   return launch(out, "bvllm_paged_tree_attention", [&] {
     return g.tree(ptr(*q), q->stride(0), q->stride(1), ptr(*c), v_half(*c), c->stride(1), c->stride(2), c->stride(3),
                   (int32_t)c->size(1), bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width,
                   qsl->const_data_ptr<int32_t>(), seq->const_data_ptr<int32_t>(), ctx->const_data_ptr<int32_t>(),
                   mask->const_data_ptr<int64_t>(), mask->stride(0), (int32_t)words, scale, ptr(out), out.stride(0),
                   out.stride(1), (int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv,
-                  (int32_t)d, (int32_t)kPage, ws.defined() ? ptr(ws) : nullptr, steps, ranges, stream);
+                  (int32_t)d, (int32_t)kPage, ws.defined() ? ptr(ws) : nullptr, split, ranges, stream);
   });
   END_HANDLE_TH_ERRORS
 }

@@ -36,6 +36,7 @@
 #include "bvllm_device.h"
 #include "bvllm_abi_internal.h"
 #include "paged_decode_wg.h"
+#include "tree_attn.h"
 
 #include <algorithm>
 #include <cmath>
@@ -107,7 +108,11 @@ constexpr int kDecodeDepth = 1;
 // keys. A range is a prefill of the sequence shifted by the range's start, so the
 // walk is unchanged; blocks of more than one range write unnormalized fp32
 // partials (with their reference max and row sum) that prefill_merge_kernel adds.
-template <int D, int NW, int QT, bool MB, int KS, bool SPL = false>
+// CTX: the context part of a draft tree step (tree_attn.hip): every row sees every key of the
+// whole 64-key tiles below its sequence's context length, so nothing is masked and no tile is
+// partial. A sequence's tiles are cut evenly into ranges of at most a.split_tiles, each a
+// work-group that always writes its partial.
+template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
                                                                   int xcd_group, int per_xcd, DecodeArgs dec,
                                                                   int n_dec_wgs, int bpw) {
@@ -134,7 +139,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // otherwise fills each CU's memory queue in front of them (mixed step
   // 1 x 512 + 63 decodes: 34.6 -> 29.5 us).
   const int n_pre_wgs = (int)gridDim.x - n_dec_wgs;
-  if ((int)blockIdx.x >= n_pre_wgs) {
+  if (!CTX && (int)blockIdx.x >= n_pre_wgs) {
     const int dw = (int)blockIdx.x - n_pre_wgs;
     if (dec.chunk_target > 0)  // uneven rows: cut into chunks (RowChunk)
       decode_work_group<D, kDecodeWaves, kDecodeDepth, true, true>(dec, dw, reinterpret_cast<float*>(lds));
@@ -145,7 +150,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
 
   const int G = a.num_heads / a.num_kv_heads;
   static_assert(KS == 1 || (KS == 2 && !MB && NW % 2 == 0), "key split: two halves, streaming path only");
-  static_assert(!SPL || (KS == 1 && !MB), "key ranges: single key walk only");
+  static_assert(!SPL || CTX || (KS == 1 && !MB), "key ranges: single key walk only");
+  static_assert(!CTX || (SPL && !MB), "context tiles come in ranges");
   constexpr int CB = NW / KS * QT * 16;  // columns of a work-group's block
 
   // Work-groups are dispatched round-robin over the 8 XCDs (XCD = id mod 8).
@@ -157,18 +163,28 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // boustrophedon order (0 1 | 1 0 | 0 1 ...): each L2 holds one KV head's
   // keys, and the heavy-to-light run of a sequence's blocks spreads evenly.
   // SPL: the ranges of a block are `bpw` whole grids apart, on the block's XCD.
+  // CTX (dense numbering, per_xcd = (sequence, KV head) pairs per XCD): the blocks of one (pair,
+  // range) follow each other on one XCD, and the ranges of a pair go to one XCD after
+  // another, so that a long sequence loads all of them (contiguous pairs per XCD: the step of
+  // 16 sequences of 1000 to 8000 had one XCD with 2.3 times the average's tiles).
   const int grid_wgs = SPL ? n_pre_wgs / bpw : n_pre_wgs;
-  const int range = SPL ? (int)blockIdx.x / grid_wgs : 0;
-  const int id = SPL ? (int)blockIdx.x - range * grid_wgs : (int)blockIdx.x;
-  const int tile0 = SPL ? range * a.split_tiles : 0;  // first key tile of the range
-  const int max_blocks = SPL ? a.max_blocks - 4 * tile0 : a.max_blocks;  // > 0: ranges start inside the table
+  const int range = CTX ? ((int)blockIdx.x >> 3) / (dense_qb * per_xcd) : SPL ? (int)blockIdx.x / grid_wgs : 0;
+  const int id = SPL && !CTX ? (int)blockIdx.x - range * grid_wgs : (int)blockIdx.x;
+  int tile0 = SPL && !CTX ? range * a.split_tiles : 0;  // first key tile of the range
+  int max_blocks = SPL ? a.max_blocks - 4 * tile0 : a.max_blocks;  // > 0: ranges start inside the table
   // The arguments that address the metadata and table loads below, read
   // with the mapping's own: otherwise their wait splits those loads' round trip.
   asm volatile("" ::"s"(a.block_tables), "s"(a.bt_stride), "s"(a.max_blocks), "s"(a.query_start_loc),
                "s"(a.seq_lens), "s"(a.context_lens), "s"(a.q), "s"(a.q_st), "s"(a.q_sh), "s"(a.k_cache),
                "s"(a.v_cache), "s"(a.c_st), "s"(a.c_sh), "s"(a.c_sb), "s"(a.num_pages));
   int kvh, r;
-  if (xcd_group < 0) {
+  if constexpr (CTX) {
+    const int at = (id >> 3) - range * (dense_qb * per_xcd);
+    const int pair = at / dense_qb * 8 + (((id & 7) - range) & 7);
+    if (pair >= a.num_seqs * a.num_kv_heads) return;
+    kvh = pair % a.num_kv_heads;
+    r = pair / a.num_kv_heads * dense_qb + at % dense_qb;
+  } else if (xcd_group < 0) {
     const int L = (id & 7) * per_xcd + (id >> 3);
     if (L >= n_blocks_bound * a.num_kv_heads) return;
     const int sk = L / dense_qb;
@@ -208,6 +224,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   int ctx = ((ConstI32)a.context_lens)[s];
   constexpr int PAGES_PER_TILE = KT / 16;
   static_assert(PAGES_PER_TILE == 4, "page_finish consumes four entries");
+  int ctx_tiles = 0;  // CTX: tiles of the range
+  if constexpr (CTX) {
+    const int tiles = context_tiles(ctx, seq_len, a.max_blocks);
+    const ContextRanges ranges(tiles, a.split_tiles, a.num_ranges);
+    if (range >= ranges.count) return;
+    tile0 = range * ranges.per;
+    ctx_tiles = min(ranges.per, tiles - tile0);
+    max_blocks = a.max_blocks - 4 * tile0;
+  }
   const ConstI32 bts = (ConstI32)(a.block_tables + (int64_t)s * a.bt_stride + (SPL ? 4 * tile0 : 0));
   const uint32_t page_bytes = (uint32_t)a.c_sb * 2u;  // c_sb < 2^31, checked on the host
   // (No branch between the fast and the clamped form: the waits that close
@@ -257,7 +282,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   }
   const int q_len = q_end - q_start;
   const int n_cols = q_len * G;
-  if constexpr (SPL) {  // the sequence as seen from the range's first key
+  if constexpr (SPL && !CTX) {  // the sequence as seen from the range's first key
     ctx -= KT * tile0;
     seq_len -= KT * tile0;
   }
@@ -284,10 +309,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   const int q_last = (min(n_cols, (blk + 1) * CB) - 1) / G;
   // (MB: the host checked that no sequence has more than two tiles' pages;
   // the clamp keeps an inconsistent seq_lens inside the staged tiles.)
-  const int hi_all = min(seq_len, ctx + q_last + 1);
+  const int hi_all = CTX ? KT * ctx_tiles : min(seq_len, ctx + q_last + 1);
   // (SPL: the last range takes the rest of the row, so a row longer than the host's
   // lists say is slower but no key of it is left out and no partial is out of range.)
-  const int hi = min(hi_all, MB ? 2 * KT : SPL && range < bpw - 1 ? KT * a.split_tiles : 0x7fffffff);
+  const int hi = min(hi_all, MB ? 2 * KT : SPL && !CTX && range < bpw - 1 ? KT * a.split_tiles : 0x7fffffff);
   if (SPL && range > 0 && hi <= 0) return;
   const int n_tiles = hi > 0 ? (hi + KT - 1) / KT : 0;
 
@@ -296,7 +321,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   const int wave_f0 = blk * CB + cw * QT * 16;
   const int wave_q0 = wave_f0 / G;  // first query index of this wave
   const bool wave_live = wave_f0 < n_cols;
-  const int wave_hi = ctx + min(q_len - 1, (wave_f0 + QT * 16 - 1) / G);  // last visible key position
+  const int wave_hi = CTX ? hi - 1 : ctx + min(q_len - 1, (wave_f0 + QT * 16 - 1) / G);  // last visible key position
 
   int qi[QT], hl[QT];
   int qpos[QT];
@@ -391,7 +416,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // zeros (unwritten slots may hold NaN, and 0·NaN would poison the PV
   // product). K rows there only reach scores that the mask replaces by -inf.
   auto zero_v_tail = [&](int kt, int buf) __attribute__((always_inline)) {
-    if (kt * KT + KT > hi) {  // uniform
+    if (!CTX && kt * KT + KT > hi) {  // uniform
 #pragma unroll
       for (int r = 0; r < PER_T; ++r) {
         const int row = (r * NW + w) * RPB + lane / CPR;
@@ -452,7 +477,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
     }
   };
   // Some key of the half at k0 may be invisible to some column of the wave.
-  auto needs_mask = [&](int k0) { return (k0 + 31 > ctx + wave_q0) || (k0 + 32 > hi); };
+  auto needs_mask = [&](int k0) { return !CTX && ((k0 + 31 > ctx + wave_q0) || (k0 + 32 > hi)); };
   // The scores' max of each column over a half, in log2 units (the scale is
   // > 0, so it commutes with the max): a chain of three-input maxima, then
   // across the four lane groups.
@@ -761,6 +786,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
         const float mm = fmax_prop(m[ct], m2);
         const float a1 = mm == kNegInf ? 0.f : fast_exp2(m[ct] - mm);
         const float a2 = mm == kNegInf ? 0.f : fast_exp2(m2 - mm);
+        m[ct] = mm;
         lsum[ct][0] = lsum[ct][0] * a1 + l2 * a2;
 #pragma unroll
         for (int c = 0; c < VD; ++c) {
@@ -788,11 +814,11 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   }
 
   if constexpr (SPL) {
-    if (range > 0 || hi_all > hi) {  // one of several ranges: fp32 partials
+    if (CTX || range > 0 || hi_all > hi) {  // one of several ranges: fp32 partials
       // Lane n + 16g holds dims 16c + 4g .. +3 of column n.
 #pragma unroll
       for (int ct = 0; ct < QT; ++ct) {
-        if (!valid[ct]) continue;
+        if (!valid[ct] || (KS == 2 && kh != 0)) continue;
         const int64_t row = ((int64_t)range * a.num_tokens + q_start + qi[ct]) * a.num_heads + kvh * G + hl[ct];
         float* po = a.part_out + row * D + 4 * g;
 #pragma unroll
@@ -1072,6 +1098,26 @@ int32_t prefill_split_tiles(const PrefillArgs& a, int64_t key_tiles, int64_t lon
     }
   }
   return tiles;
+}
+
+// The context part of a draft tree step, in blocks of 128 columns or, for at most 64 columns a
+// sequence, of 64 whose waves split the keys; the caller adds the ranges' partials.
+template <int D, int QT, int KS>
+static hipError_t launch_context(const PrefillArgs& a, hipStream_t stream) {
+  constexpr int CB = 4 / KS * QT * 16;
+  const int64_t blocks = ((int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads) + CB - 1) / CB;
+  const int64_t per_xcd = ((int64_t)a.num_seqs * a.num_kv_heads + 7) / 8;
+  const int64_t wgs = 8 * per_xcd * blocks * a.num_ranges;
+  if (wgs > 0x7ffffff0 || blocks * a.num_seqs > 0x7ffffff0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, true, true>), dim3((unsigned)wgs), dim3(4 * 64), 0,
+                     stream, a, (int)(blocks * a.num_seqs), (int)blocks, 0, (int)per_xcd, DecodeArgs{}, 0, a.num_ranges);
+  return hipGetLastError();
+}
+
+hipError_t paged_prefill_context(const PrefillArgs& a, hipStream_t stream) {
+  const bool narrow = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads) <= 64;
+  if (a.head_dim == 64) return narrow ? launch_context<64, 2, 2>(a, stream) : launch_context<64, 2, 1>(a, stream);
+  return narrow ? launch_context<128, 2, 2>(a, stream) : launch_context<128, 2, 1>(a, stream);
 }
 
 // Two column tiles per wave (128 columns per work-group) unless that grid

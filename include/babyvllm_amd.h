@@ -348,18 +348,19 @@ BVLLM_API int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t vo
  * row with no visible key outputs zeros; keys that a row does not see do not reach it,
  * whatever they hold. mask_words must be at least max_query_len / 64 rounded up; scale
  * must be positive and finite.
- * range_steps > 0 cuts every sequence's keys into ranges of range_steps 32-key steps, each
- * on work-groups of its own, with fp32 partials in workspace
- * (bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, num_ranges) bytes) that a
- * second launch adds; the last of the num_ranges ranges runs to the row's end. 0: one
- * launch, no workspace. bvllm_tree_range_steps returns the range_steps to use (0: none)
- * from host sizes alone: key_steps is ceil(seq_len / 32) summed over the sequences,
- * longest_steps the largest of them, each -1 if unknown. They steer the choice only;
- * results agree within the rounding of fp32 sums in another order.
+ * split_tiles > 0 gives the whole 64-key tiles below every context length to a launch of its
+ * own, cut into at most num_ranges ranges a sequence, of split_tiles tiles where that
+ * suffices, whose fp32 partials in workspace (bvllm_tree_workspace_bytes(num_tokens,
+ * num_heads, head_dim, num_ranges) bytes) a second launch adds to the other keys. 0: one
+ * launch over all keys, no workspace. bvllm_tree_split_tiles returns the split_tiles to use
+ * (0: none) from host sizes alone: key_tiles is ceil(seq_len / 64) summed over the
+ * sequences, longest_tiles the largest of them, each -1 if unknown; bvllm_prefill_ranges the
+ * num_ranges. They steer the choice only; results agree within the rounding of fp32 sums in
+ * another order.
  */
-BVLLM_API int32_t bvllm_tree_range_steps(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+BVLLM_API int32_t bvllm_tree_split_tiles(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks,
-                     int64_t key_steps, int64_t longest_steps);
+                     int64_t key_tiles, int64_t longest_tiles);
 BVLLM_API int64_t bvllm_tree_workspace_bytes(int32_t num_tokens, int32_t num_heads, int32_t head_dim,
                      int32_t num_ranges);
 BVLLM_API int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
@@ -373,7 +374,7 @@ BVLLM_API int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int6
                      void* out, int64_t out_stride_t, int64_t out_stride_h,
                      int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                     int32_t block_size, void* workspace, int32_t range_steps, int32_t num_ranges,
+                     int32_t block_size, void* workspace, int32_t split_tiles, int32_t num_ranges,
                      void* stream);
 
 /*

@@ -158,8 +158,8 @@ def test_python_path_gives_the_same_bits(monkeypatch, heads):
     check(paged_tree_attention(q, cache, md, q.shape[-1] ** -0.5), formula(q, cache, md, q.shape[-1] ** -0.5))
 
 
-def raw_call(q, cache, md, scale, steps, ranges):
-    """The C entry with a choice of key ranges."""
+def raw_call(q, cache, md, scale, split, ranges):
+    """The C entry with a choice of the context's ranges."""
     from babyvllm.kernels import _lib
     h = _lib.lib()
     t, heads, d = q.shape
@@ -170,21 +170,33 @@ def raw_call(q, cache, md, scale, steps, ranges):
         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), cache[1].data_ptr(), *k.stride()[:3], cache.shape[1],
         bt.data_ptr(), bt.stride(0), bt.shape[1], md.query_start_loc.data_ptr(), md.seq_lens.data_ptr(),
         md.context_lens.data_ptr(), m.data_ptr(), m.stride(0), m.shape[1], scale, out.data_ptr(), out.stride(0),
-        out.stride(1), md.seq_lens.shape[0], t, md.max_query_len, heads, cache.shape[3], d, 16, ws.data_ptr(), steps,
+        out.stride(1), md.seq_lens.shape[0], t, md.max_query_len, heads, cache.shape[3], d, 16, ws.data_ptr(), split,
         ranges, _lib.stream_handle(q.device))
     _lib.check(rc, "bvllm_paged_tree_attention")
     return out
 
 
-@pytest.mark.parametrize("heads", [(2, 7, 128), (2, 7, 64)], ids=str)
-@pytest.mark.parametrize("steps", [1, 2, 7, 8, 24, 1000])
-def test_key_ranges_of_any_length(heads, steps):
+@pytest.mark.parametrize("heads", [(2, 7, 128), (2, 7, 64), (1, 3, 128), (1, 2, 64)], ids=str)
+@pytest.mark.parametrize("split", [0, 1, 2, 3, 5, 12, 1000])
+def test_context_ranges_of_any_length(heads, split):
+    # Contexts of no whole tile, of one, of several; blocks of 64 and of 128 columns.
     rng = random.Random(1)
-    q, cache, md = build([(c, random_tree(rng, n)) for c, n in ((700, 9), (0, 3), (33, 40), (1500, 1))], *heads)
-    widest = cdiv(cdiv(md.block_tables.shape[1], 2), steps)
+    q, cache, md = build([(c, random_tree(rng, n)) for c, n in ((700, 9), (0, 3), (33, 40), (1500, 1), (64, 5), (127, 2))], *heads)
     want = formula(q, cache, md, 0.1)
+    widest = max(1, cdiv(cdiv(md.block_tables.shape[1], 4), max(1, split)))
     for ranges in sorted({1, 2, (widest + 1) // 2, widest} & set(range(1, widest + 1))):
-        check(raw_call(q, cache, md, 0.1, steps, ranges), want)
+        check(raw_call(q, cache, md, 0.1, split, ranges), want)
+
+
+@pytest.mark.parametrize("heads", [(2, 7, 128), (4, 7, 64)], ids=str)
+@pytest.mark.parametrize("seqs", [1, 3, 9, 20, 60])
+def test_every_number_of_waves_per_column(seqs, heads):
+    rng = random.Random(seqs)
+    specs = [(rng.choice([0, 5, 64, 100, 200]), random_tree(rng, rng.choice([1, 9, 30]))) for _ in range(seqs - 1)]
+    q, cache, md = build(specs + [(130, random_tree(rng, 33))], *heads)
+    want = formula(q, cache, md, 0.1)
+    check(raw_call(q, cache, md, 0.1, 0, 0), want)
+    check(raw_call(q, cache, md, 0.1, 1, 2), want)
 
 
 def test_masks_that_leave_rows_without_keys_or_without_themselves():
@@ -216,6 +228,7 @@ def test_what_a_row_does_not_see_does_not_reach_it(bad, heads):
     # Drafted tokens whose K and V are not finite spoil their own branch only.
     tree = [-1, 0, 0, 1, 2, 3, 4, 4, 6] + [0] * 30
     q, cache, md = build([(70, tree), (3, tree)], *heads)
+    calls = (lambda: paged_tree_attention(q, cache, md, 0.1), lambda: raw_call(q, cache, md, 0.1, 1, 1))
     for s, ctx in enumerate((70, 3)):
         for node in (2, 6, 20):
             p = ctx + node
@@ -223,23 +236,23 @@ def test_what_a_row_does_not_see_does_not_reach_it(bad, heads):
             cache[1, page, p % PAGE, :, node::3] = bad
             if node == 6:
                 cache[0, page, p % PAGE, :, 0] = bad
-    got = paged_tree_attention(q, cache, md, 0.1).cpu()
     clean = cache.clone()
     clean[~torch.isfinite(clean)] = 0
     want = formula(q, clean, md, 0.1)
     mask = md.tree_mask.cpu()
     untouched = [r for r in range(q.shape[0]) if not any((int(mask[r, 0]) >> n) & 1 for n in (2, 6, 20))]
     assert len(untouched) > 60
-    check(got[untouched], tuple(w[untouched] for w in want))
     touched = [r for r in range(q.shape[0]) if (int(mask[r, 0]) >> 20) & 1]
-    assert len(touched) == 2 and not torch.isfinite(got[touched][..., 20::3]).any()
     plain = torch.ones(heads[2], dtype=torch.bool)
     plain[20::3] = False  # the other dims of such a row are the formula's
-    out, tol, _ = (w[touched] for w in want)
     clean_v = cache.clone()
     clean_v[1][~torch.isfinite(clean_v[1])] = 0
     out, tol, _ = (w[touched] for w in formula(q, clean_v, md, 0.1))
-    assert ((got[touched].double() - out).abs()[..., plain] <= tol[..., plain]).all()
+    for call in calls:
+        got = call().cpu()
+        check(got[untouched], tuple(w[untouched] for w in want))
+        assert len(touched) == 2 and not torch.isfinite(got[touched][..., 20::3]).any()
+        assert ((got[touched].double() - out).abs()[..., plain] <= tol[..., plain]).all()
 
 
 def test_scores_that_grow_and_scores_far_below_zero():
@@ -361,7 +374,7 @@ def test_no_memory_for_the_scratch_takes_the_whole_rows(monkeypatch):
 
     q, cache, md = build([(4000, random_tree(random.Random(6), 16))], 2, 7, 64)
     python_path(monkeypatch)
-    assert _lib.lib().bvllm_tree_range_steps(1, 16, 16, 14, 2, 64, md.block_tables.shape[1], 126, 126) > 0
+    assert _lib.lib().bvllm_tree_split_tiles(1, 16, 16, 14, 2, 64, md.block_tables.shape[1], 63, 63) > 0
     monkeypatch.setattr(_lib, "optional_scratch", lambda n, dev: None)
     run(q, cache, md)
 
