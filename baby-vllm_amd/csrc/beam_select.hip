@@ -3,12 +3,18 @@
 //   total(b, v) = score_b + logit_bv - lse_b,  lse_b = log sum_v exp(logit_bv),
 // in descending order, equal totals by their flat index b·V + v.
 //
-// Bound by one pass over the logits (16 groups of 8 beams over 152,064 bf16 tokens are
-// 39 MB). Stage 1, one wave per piece of 2048 columns: the piece's maximum and its sum of
-// exponentials relative to it, nothing else. Stage 2, one work-group per group: the rows'
-// lse from the pieces; then a bar that n pieces' maxima reach, so that a token has to reach
-// it too. Only pieces that do are read again, some more than n of them, and few tokens in
-// them compete: each counts the better ones.
+// Stage 1, one wave per piece of 2048 columns: the piece's maximum and its sum of
+// exponentials relative to it, nothing else. It is one pass over the logits (16 groups of 8
+// beams over 152,064 bf16 tokens, 39 MB: 7.7-9.5 us, 4.1-5.1 TB/s). Stage 2, one work-group
+// per group: the rows' lse from the pieces; then a bar that n pieces' maxima reach, so that a
+// token has to reach it too. Only pieces that do are read again, some more than n of them, and
+// few tokens in them compete: each counts the better ones. It is bound by its chain of loads
+// and barriers (1 group of 4 beams, 8 candidates: 7.7 us; 16 groups of 8, 16 candidates: 12.6).
+// Choosing the n best of each piece in stage 1 instead took 24.4 us there, most of it in
+// counting that no later choice needed.
+//
+// Masked vocabularies, whose bar is -inf, and other crowds of equal totals take the exact
+// choice (the same two sizes with 20 tokens of a row left: 39 and 48 us in all, against 12 and 21).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -38,10 +44,10 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 struct Piece {
   static constexpr int VEC = 16 / sizeof(T), LOADS = 32 / VEC;
+  u32x4_any raw[LOADS];
   float v[32];
   static __device__ __forceinline__ int column(int e) { return ((e / VEC) * 64 + lane_id()) * VEC + e % VEC; }
-  __device__ __forceinline__ void load(const T* x, int left) {
-    u32x4_any raw[LOADS];
+  __device__ __forceinline__ void request(const T* x, int left) {
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int c = column(k * VEC);
@@ -59,6 +65,8 @@ struct Piece {
         for (int j = 0; j < 4; ++j) raw[k][j] = c + j < left ? __float_as_uint(x[c + j]) : 0xff800000u;
       }
     }
+  }
+  __device__ __forceinline__ void unpack() {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const uint32_t w = raw[e / VEC][sizeof(T) == 2 ? (e % VEC) / 2 : e % VEC];
@@ -90,8 +98,9 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamSelectAr
   const int piece = ((int)blockIdx.x - row * groups_per_row) * kScanWaves + wave_id();
   if (piece >= pieces) return;
   Piece<T> p;
-  p.load(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride + (int64_t)piece * kPiece,
-         a.vocab - piece * kPiece);
+  p.request(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride + (int64_t)piece * kPiece,
+            a.vocab - piece * kPiece);
+  p.unpack();
   float mx[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) mx[e] = fmax_prop(p.v[e], p.v[e + 16]);
@@ -127,18 +136,111 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 
 constexpr double kNegInf64 = -__builtin_huge_val();
 
-// Candidates of the fast path: more than this many send the group to the exact one.
+// Candidates: more than this many send the group to the exact choice.
 constexpr int kMaxCand = kMaxPick * kMaxPick;
-static_assert(kMaxCand >= kMaxPick * kMaxPick, "the exact path: n tokens of n pieces");
+static_assert(kMaxCand >= kMaxPick * kMaxPick, "the exact choice: n tokens of n pieces");
+static_assert(kBeamMaxPieces >= 64 * kMaxPick, "a key for each lane's share of up to n pieces");
+constexpr int kSets = 128;
+constexpr int kRankDirect = 128;  // items that count the better ones among all of them
 
 struct PickShared {
-  uint64_t keys[kBeamMaxPieces];  // the pieces' maxima as totals
+  uint64_t keys[kBeamMaxPieces];  // maxima as totals: of the pieces, or of the lanes' shares of few pieces
   uint64_t cand_key[kMaxCand];
   uint32_t cand[kMaxCand];        // b * vocab + v < 2^24 (at most 8192 pieces of 2048)
+  uint64_t part_key[kPickThreads], set_key[kSets];
+  uint32_t part_index[kPickThreads], set_index[kSets];
   double base[kBeamMaxBeams];
-  int better[64];
-  int count;
+  int rank[kSets];
+  uint64_t bar_key;
+  uint32_t bar_index;
+  uint16_t near[kMaxCand];        // items that reach the threshold
+  uint16_t best[kMaxPick];        // the n best, in order
+  int count, n_near;
 };
+
+// (key, index) pairs: larger keys first, equal ones by index.
+__device__ __forceinline__ bool ahead(uint64_t k, uint32_t i, uint64_t l, uint32_t j) {
+  return k > l || (k == l && i < j);
+}
+
+// A pair that at least n of the items reach and few others, into bar_key and bar_index (0 and
+// ~0, reached by all, with fewer): the items are dealt to 128 sets, and it is the n-th best of the
+// sets' best. With n at most half the sets, about 1.4 n items reach it.
+template <typename Key, typename Index>
+__device__ __forceinline__ void near_best(PickShared& sh, int n_items, int n, Key key, Index index) {
+  const int tid = (int)threadIdx.x, set = tid & (kSets - 1), slice = tid / kSets;
+  uint64_t k = 0;
+  uint32_t x = ~0u;
+  for (int i = tid; i < n_items; i += kPickThreads)
+    if (ahead(key(i), index(i), k, x)) {
+      k = key(i);
+      x = index(i);
+    }
+  sh.part_key[tid] = k;
+  sh.part_index[tid] = x;
+  if (tid < kSets) sh.rank[tid] = 0;
+  if (tid == 0) {
+    sh.bar_key = 0;
+    sh.bar_index = ~0u;
+    sh.n_near = 0;
+  }
+  __syncthreads();
+  if (tid < kSets) {
+#pragma unroll
+    for (int q = 1; q < kPickThreads / kSets; ++q)
+      if (ahead(sh.part_key[tid + q * kSets], sh.part_index[tid + q * kSets], k, x)) {
+        k = sh.part_key[tid + q * kSets];
+        x = sh.part_index[tid + q * kSets];
+      }
+    sh.set_key[tid] = k;
+    sh.set_index[tid] = x;
+  }
+  __syncthreads();
+  k = sh.set_key[set];
+  x = sh.set_index[set];
+  int better = 0;
+  constexpr int kEach = kSets * kSets / kPickThreads;
+#pragma unroll
+  for (int q = 0; q < kEach; ++q) {
+    const int o = slice * kEach + q;
+    better += ahead(sh.set_key[o], sh.set_index[o], k, x);
+  }
+  if (better != 0) atomicAdd(&sh.rank[set], better);
+  __syncthreads();
+  // (An empty set's pair ranks behind every item's, as all empty sets do together.)
+  if (tid < kSets && sh.rank[tid] == n - 1 && k != 0) {
+    sh.bar_key = k;
+    sh.bar_index = x;
+  }
+  __syncthreads();
+}
+
+// The n best items in order, into sh.best (there are at least n with a key).
+template <typename Key, typename Index>
+__device__ __forceinline__ void best_items(PickShared& sh, int n_items, int n, Key key, Index index) {
+  const int tid = (int)threadIdx.x;
+  int m = n_items;
+  const bool all = n_items <= kRankDirect;
+  if (!all) {
+    near_best(sh, n_items, n, key, index);
+    for (int i = tid; i < n_items; i += kPickThreads)
+      if (!ahead(sh.bar_key, sh.bar_index, key(i), index(i))) sh.near[atomicAdd(&sh.n_near, 1)] = (uint16_t)i;
+    __syncthreads();
+    m = sh.n_near;
+  }
+  for (int e = tid; e < m; e += kPickThreads) {
+    const int i = all ? e : sh.near[e];
+    const uint64_t k = key(i);
+    const uint32_t x = index(i);
+    int rank = 0;
+    for (int f = 0; f < m; ++f) {
+      const int o = all ? f : sh.near[f];
+      rank += ahead(key(o), index(o), k, x);
+    }
+    if (rank < n && k != 0) sh.best[rank] = (uint16_t)i;
+  }
+  __syncthreads();
+}
 
 // Totals of beam b; -inf for a beam without a distribution (base -inf), whatever its logits.
 __device__ __forceinline__ double total_of_logit(double base, float x) {
@@ -146,12 +248,23 @@ __device__ __forceinline__ double total_of_logit(double base, float x) {
 }
 
 template <typename T>
-__device__ __forceinline__ void load_piece(const BeamSelectArgs& a, int64_t row, int piece, bool live, Piece<T>& p) {
-  p.load(reinterpret_cast<const T*>(a.logits) + row * a.row_stride + (int64_t)piece * kPiece, a.vocab - piece * kPiece);
+__device__ __forceinline__ void request_piece(const BeamSelectArgs& a, int64_t row, int piece, Piece<T>& p) {
+  p.request(reinterpret_cast<const T*>(a.logits) + row * a.row_stride + (int64_t)piece * kPiece, a.vocab - piece * kPiece);
+}
+// A beam without a distribution holds nothing but -inf.
+template <typename T>
+__device__ __forceinline__ void unpack_piece(bool live, Piece<T>& p) {
+  p.unpack();
   if (!live) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) p.v[i] = kNegInf;
   }
+}
+
+template <typename T>
+__device__ __forceinline__ void load_piece(const BeamSelectArgs& a, int64_t row, int piece, bool live, Piece<T>& p) {
+  request_piece(a, row, piece, p);
+  unpack_piece(live, p);
 }
 
 // Wave-wide: exclusive prefix sum, and the sum in `all`.
@@ -184,8 +297,8 @@ __device__ __forceinline__ uint32_t best_of_piece(const Piece<T>& p, double base
   };
   int n_over = wave_count(over);
   if (n_over > n) {
-    // The piece alone holds more than n above the bar: its own bar is its n-th logit, found
-    // bit by bit from the top (the largest value that at least n reach).
+    // The piece alone holds more than n above the bar: its own bar is the total of its n-th logit,
+    // which is found bit by bit from the top (the largest value that at least n reach).
     const uint32_t open = over;
     uint32_t nth = 0;
     for (int bit = 31; bit >= 0; --bit) {
@@ -197,11 +310,18 @@ __device__ __forceinline__ uint32_t best_of_piece(const Piece<T>& p, double base
       if (reach >= n) nth = probe;
       if (reach == n) break;
     }
+    uint32_t least = ~0u;  // (the search ends early at a value between two logits)
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      if (((open >> i) & 1) && order_of(p.v[i]) >= nth) least = min(least, order_of(p.v[i]));
+    least = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+    const uint64_t own = order_of(total_of_logit(base, __uint_as_float(least >> 31 ? least & ~(1u << 31) : ~least)));
     over = even = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      over |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) > nth) << i;
-      even |= (uint32_t)(((open >> i) & 1) && order_of(p.v[i]) == nth) << i;
+      const uint64_t k = order_of(total_of_logit(base, p.v[i]));
+      over |= (uint32_t)(((open >> i) & 1) && k > own) << i;
+      even |= (uint32_t)(((open >> i) & 1) && k == own) << i;
     }
     n_over = wave_count(over);
   }
@@ -227,57 +347,37 @@ __device__ __forceinline__ uint32_t best_of_piece(const Piece<T>& p, double base
   return over | even;
 }
 
-// The exact choice of pieces and tokens, for groups whose candidates overflow: many equal
-// totals at the bar (masked vocabularies, few distinct logits), or many good tokens in one piece.
+// The exact choice of pieces and tokens, for groups with too many candidates: many equal
+// totals at the bar (masked vocabularies, few distinct logits), or many good tokens in one
+// piece. The n best pieces by maximum and index (all of fewer), and of each its n best tokens.
 template <typename T>
 __device__ __forceinline__ void pick_exact(const BeamSelectArgs& a, int pieces, PickShared& sh) {
   const int lane = lane_id(), w = wave_id();
   const int n = a.num_candidates, M = a.num_beams * pieces;
   const int64_t row0 = (int64_t)blockIdx.x * a.num_beams;
-  // The n-th best piece's key (0 with fewer pieces), bit by bit; then pieces above it, and the
-  // first ones at it. Every wave finds the same.
   uint64_t bar = 0;
-  int above = M;
   if (M > n) {
-    auto reach = [&](uint64_t k) {
-      int c = 0;
-      for (int i0 = 0; i0 < M; i0 += 64)
-        c += __popcll(__builtin_amdgcn_ballot_w64(i0 + lane < M && sh.keys[min(i0 + lane, M - 1)] >= k));
-      return c;
-    };
-    for (int bit = 63; bit >= 0; --bit) {
-      const uint64_t probe = bar | (1ull << bit);
-      if (reach(probe) >= n) bar = probe;
-    }
-    above = bar == ~0ull ? 0 : reach(bar + 1);
+    best_items(sh, M, n, [&](int i) { return sh.keys[i]; }, [&](int i) { return (uint32_t)i; });
+    bar = sh.keys[sh.best[n - 1]];
   }
-  int found = 0, found_even = 0;
-  for (int i0 = 0; i0 < M; i0 += 64) {
-    const uint64_t key = i0 + lane < M ? sh.keys[i0 + lane] : 0;
-    const bool in = i0 + lane < M;
-    uint64_t over = __builtin_amdgcn_ballot_w64(in && (M <= n || key > bar));
-    const uint64_t even = M <= n ? 0 : __builtin_amdgcn_ballot_w64(in && key == bar);
-    for (uint64_t left = over | even; left != 0; left &= left - 1) {
-      const int l = (int)__builtin_ctzll(left);
-      if (((even >> l) & 1) && found_even++ >= n - above) continue;
-      if ((found++ & (kPickWaves - 1)) != w) continue;
-      const int i = i0 + l, b = i / pieces, piece = i - b * pieces;
-      Piece<T> p;
-      load_piece(a, row0 + b, piece, sh.base[b] != kNegInf64, p);
-      const uint32_t taken = best_of_piece(p, sh.base[b], bar, a.vocab - piece * kPiece, n);
-      int all;
-      int at = wave_prefix(__builtin_popcount(taken), all);
-      int start = 0;
-      if (lane == 0) start = atomicAdd(&sh.count, all);
-      at += __shfl(start, 0, 64);
+  for (int e = w; e < min(n, M); e += kPickWaves) {
+    const int i = M > n ? sh.best[e] : e, b = i / pieces, piece = i - b * pieces;
+    Piece<T> p;
+    load_piece(a, row0 + b, piece, sh.base[b] != kNegInf64, p);
+    const uint32_t taken = best_of_piece(p, sh.base[b], bar, a.vocab - piece * kPiece, n);
+    int all;
+    int at = wave_prefix(__builtin_popcount(taken), all);
+    int start = 0;
+    if (lane == 0) start = atomicAdd(&sh.count, all);
+    at += __shfl(start, 0, 64);
 #pragma unroll
-      for (int e = 0; e < 32; ++e)
-        if ((taken >> e) & 1) {
-          sh.cand_key[at] = order_of(total_of_logit(sh.base[b], p.v[e]));
-          sh.cand[at++] = (uint32_t)(b * a.vocab + piece * kPiece + Piece<T>::column(e));
-        }
-    }
+    for (int q = 0; q < 32; ++q)
+      if ((taken >> q) & 1) {
+        sh.cand_key[at] = order_of(total_of_logit(sh.base[b], p.v[q]));
+        sh.cand[at++] = (uint32_t)(b * a.vocab + piece * kPiece + Piece<T>::column(q));
+      }
   }
+  __syncthreads();
 }
 
 template <typename T>
@@ -288,10 +388,12 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   const int64_t row0 = (int64_t)blockIdx.x * K;
   const float2* stats = reinterpret_cast<const float2*>(a.stats) + row0 * pieces;
   if (tid == 0) sh.count = 0;
-  if (tid < 64) sh.better[tid] = 0;
+  if (tid < 64) sh.rank[tid] = 0;
 
-  // A wave per beam: base_b = score_b - lse_b, in fp64 from the pieces' sums on, and the
-  // keys of its pieces.
+  // A wave per beam: base_b = score_b - lse_b, in fp64 from the pieces' sums on, and the keys
+  // of its pieces, or of the lanes' shares of them where the pieces alone are too few for a bar.
+  const bool shares = M <= n;
+  const int share_lanes = min(64, (a.vocab + Piece<T>::VEC - 1) / Piece<T>::VEC);  // that hold a token of some piece
   for (int b = w; b < K; b += kPickWaves) {
     const float score = a.scores[row0 + b];
     float m = kNegInf;
@@ -307,14 +409,32 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     const bool live = fabsf(m) < __builtin_huge_valf() && fabsf(score) < __builtin_huge_valf();
     const double base = live ? (double)score - ((double)m + log(sum)) : kNegInf64;
     if (lane == 0) sh.base[b] = base;
-    for (int i = lane; i < pieces; i += 64) sh.keys[b * pieces + i] = order_of(total_of_logit(base, stats[b * pieces + i].x));
+    if (!shares) {
+      for (int i = lane; i < pieces; i += 64)
+        sh.keys[b * pieces + i] = order_of(total_of_logit(base, stats[b * pieces + i].x));
+    } else {
+      for (int piece = 0; piece < pieces; ++piece) {
+        Piece<T> p;
+        load_piece(a, row0 + b, piece, live, p);
+        float x = kNegInf;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) x = fmax_prop(x, p.v[e]);
+        // (A share behind the row's end holds no token: key 0.)
+        const bool any = Piece<T>::column(0) < a.vocab - piece * kPiece;
+        if (lane < share_lanes)
+          sh.keys[(b * pieces + piece) * share_lanes + lane] = any ? order_of(total_of_logit(base, x)) : 0;
+      }
+    }
   }
   __syncthreads();
 
-  // The bar: a total that at least n pieces reach, and few others. Lane l takes the best of
-  // pieces l, l + 64, ...; the bar is the n-th best of those 64. Every wave finds the same.
+  // The bar: a total that at least n tokens reach, and few others. Few candidates among many
+  // pieces: lane l takes the best of pieces l, l + 64, ...; the bar is the n-th best of those
+  // 64 (1 group of 4 beams, 8 candidates: 1.0 us less than with the sets). Else, with more
+  // candidates to tell apart, 128 sets of all the work-group's threads (4 groups of 32 beams over
+  // 50,257 tokens, 64 candidates, in all: 34 us; with the bar of 64 lanes 49).
   uint64_t bar = 0;
-  if (M > n) {
+  if (!shares && n <= 24 && M >= 4 * n) {
     uint64_t best = 0;
     for (int i = lane; i < M; i += 64) best = max(best, sh.keys[i]);
     // Each wave compares every lane's best with a few of them.
@@ -326,74 +446,93 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
                              (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, o);
       better += other > best || (other == best && o < lane);
     }
-    if (better != 0) atomicAdd(&sh.better[lane], better);
+    if (better != 0) atomicAdd(&sh.rank[lane], better);
     __syncthreads();
-    const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(sh.better[lane] == n - 1));
+    const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(sh.rank[lane] == n - 1));
     bar = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(best >> 32), l) << 32) |
           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)best, l);
+  } else {
+    near_best(sh, shares ? share_lanes * M : M, n, [&](int i) { return sh.keys[i]; }, [&](int i) { return (uint32_t)i; });
+    bar = sh.bar_key;
   }
 
-  // The pieces that reach it, dealt to the waves; their tokens that do are candidates. A
-  // conservative fp32 threshold sorts out nearly all others.
+  // The pieces that reach it (all, if the bar comes from shares), dealt to the waves.
+  if (tid == 0) sh.n_near = 0;
+  __syncthreads();
+  for (int i = tid; i < M; i += kPickThreads)
+    if (shares || sh.keys[i] >= bar) {
+      const int at = atomicAdd(&sh.n_near, 1);
+      if (at < kMaxCand) sh.near[at] = (uint16_t)i;
+    }
+  __syncthreads();
+  const int n_reach = sh.n_near;
+  // (Far more pieces than candidates: equal maxima at the bar, and not worth reading.)
+  const bool too_many = n_reach > 4 * n + 64;
+  // Their tokens that reach it are candidates: a conservative fp32 threshold sorts out nearly
+  // all others. A wave's next piece is on its way while it looks at one.
   const double bar_total = bar == 0 ? kNegInf64 : total_of(bar);
-  int found = 0;
-  for (int i0 = 0; i0 < M; i0 += 64) {
-    const bool in = i0 + lane < M && sh.keys[min(i0 + lane, M - 1)] >= bar;
-    for (uint64_t left = __builtin_amdgcn_ballot_w64(in); left != 0; left &= left - 1) {
-      if ((found++ & (kPickWaves - 1)) != w) continue;
-      const int i = i0 + (int)__builtin_ctzll(left), b = i / pieces, piece = i - b * pieces;
-      const int columns = a.vocab - piece * kPiece;
-      const double base = sh.base[b];
-      Piece<T> p;
-      load_piece(a, row0 + b, piece, base != kNegInf64, p);
-      const float at_bar = base == kNegInf64 ? kNegInf : (float)(bar_total - base);
-      const float threshold = at_bar - fabsf(at_bar) * 0x1p-22f - 0x1p-126f;
-      int all = 0;
+  Piece<T> p, next;
+  int i = 0, i_next = 0;
+  auto request_next = [&](int e) __attribute__((always_inline)) {
+    i_next = uniform((int)sh.near[e]);
+    const int b = i_next / pieces;
+    request_piece(a, row0 + b, i_next - b * pieces, next);
+  };
+  if (!too_many && w < n_reach) request_next(w);
+  for (int e = w; e < n_reach && !too_many; e += kPickWaves) {
+    p = next;
+    i = i_next;
+    if (e + kPickWaves < n_reach) request_next(e + kPickWaves);
+    const int b = i / pieces, piece = i - b * pieces, columns = a.vocab - piece * kPiece;
+    const double base = sh.base[b];
+    unpack_piece(base != kNegInf64, p);
+    const float at_bar = base == kNegInf64 ? kNegInf : (float)(bar_total - base);
+    // (The second term: scores so large that a total's own rounding hides logits.)
+    const float threshold =
+        at_bar - fabsf(at_bar) * 0x1p-22f - (base == kNegInf64 ? 0.f : (float)(fabs(base) * 0x1p-51)) - 0x1p-126f;
+    if (threshold == kNegInf && columns < kPiece) {  // columns behind the row's end, which read as -inf, are none
 #pragma unroll
-      for (int e = 0; e < 32; ++e) all += __popcll(__builtin_amdgcn_ballot_w64(p.v[e] >= threshold));
-      int at = 0;
-      if (lane == 0) at = atomicAdd(&sh.count, all);
-      at = uniform(at);
-      if (at + all > kMaxCand) continue;  // (the count tells everybody)
+      for (int q = 0; q < 32; ++q)
+        if (Piece<T>::column(q) >= columns) p.v[q] = __builtin_nanf("");
+    }
+    int all = 0;
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(p.v[e] >= threshold);
-        if (hit != 0) {
-          if ((hit >> lane) & 1) {
-            // Columns behind the row's end, which read as -inf, and those below the bar drop out.
-            const int c = Piece<T>::column(e), slot = at + __popcll(hit & ((1ull << lane) - 1));
-            const uint64_t k = order_of(total_of_logit(base, p.v[e]));
-            sh.cand_key[slot] = c < columns ? k : 0;
-            sh.cand[slot] = c < columns && k >= bar ? (uint32_t)(b * a.vocab + piece * kPiece + c) : ~0u;
-          }
-          at += __popcll(hit);
+    for (int q = 0; q < 32; ++q) all += __popcll(__builtin_amdgcn_ballot_w64(p.v[q] >= threshold));
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh.count, all);
+    at = uniform(at);
+    if (at + all > kMaxCand) continue;  // (the count tells everybody)
+#pragma unroll
+    for (int q = 0; q < 32; ++q) {
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(p.v[q] >= threshold);
+      if (hit != 0) {
+        if ((hit >> lane) & 1) {
+          const int slot = at + __popcll(hit & ((1ull << lane) - 1));
+          const uint64_t k = order_of(total_of_logit(base, p.v[q]));
+          sh.cand_key[slot] = k >= bar ? k : 0;  // (just below the bar: no candidate)
+          sh.cand[slot] = (uint32_t)(b * a.vocab + piece * kPiece + Piece<T>::column(q));
         }
+        at += __popcll(hit);
       }
     }
   }
   __syncthreads();
-  if (sh.count > kMaxCand) {
+  if (too_many || sh.count > kMaxCand) {
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();
     pick_exact<T>(a, pieces, sh);
-    __syncthreads();
   }
 
-  const int c = sh.count;
-  const int64_t out0 = (int64_t)blockIdx.x * n;
-  for (int e = tid; e < c; e += kPickThreads) {
-    const uint64_t k = sh.cand_key[e];
-    const uint32_t flat = sh.cand[e];
-    if (flat == ~0u) continue;
-    int rank = 0;
-    for (int o = 0; o < c; ++o) rank += sh.cand_key[o] > k || (sh.cand_key[o] == k && sh.cand[o] < flat);
-    if (rank < n) {
-      const uint32_t beam = flat / (uint32_t)a.vocab;
-      a.out_scores[out0 + rank] = (float)total_of(k);
-      a.out_beams[out0 + rank] = beam;
-      a.out_tokens[out0 + rank] = flat - beam * (uint32_t)a.vocab;
-    }
+  // The n best candidates by key, equal ones by index.
+  best_items(sh, sh.count, n, [&](int i) { return sh.cand_key[i]; }, [&](int i) { return sh.cand[i]; });
+  if (tid < n) {
+    const int e = sh.best[tid];
+    const int64_t at = (int64_t)blockIdx.x * n + tid;
+    const uint32_t flat = sh.cand[e], beam = flat / (uint32_t)a.vocab;
+    a.out_scores[at] = (float)total_of(sh.cand_key[e]);
+    a.out_beams[at] = beam;
+    a.out_tokens[at] = flat - beam * (uint32_t)a.vocab;
   }
 }
 

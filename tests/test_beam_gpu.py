@@ -127,6 +127,54 @@ def test_extreme_values():
     check(z, torch.tensor([-1.0, -1.0], device="cuda"), 2, 9)
 
 
+@pytest.mark.parametrize("k,n,vocab", [(1, 2, 5000), (4, 8, 70000), (32, 64, 100), (32, 64, 4099), (32, 64, 50257), (2, 64, 30000)])
+def test_scores_that_hide_logits(k, n, vocab):
+    # At 1e20 a total's 64 bits step by 16384: all totals of equal scores are equal, and the
+    # first tokens of the first beam lead.
+    x, s = inputs(2 * k, vocab, seed=n)
+    s.fill_(-1e20)
+    scores, beams, tokens = beam_select(x, s, k, n)
+    flat = torch.arange(n, device="cuda").expand(2, n)
+    assert torch.equal(beams, flat // vocab) and torch.equal(tokens, flat % vocab)
+    assert (scores == -1e20).all()
+    # One beam far above the rest.
+    s[k // 2] = 0.0
+    s[k + k // 2] = 3e38
+    check(x[:k].float(), s[:k], k, n)
+    if vocab >= n:
+        got = beam_select(x, s, k, n)
+        assert (got[1] == k // 2).all() and (got[0][1] == 3e38).all()
+        assert torch.equal(got[2][1], torch.arange(n, device="cuda"))
+
+
+@pytest.mark.parametrize("groups,k,n,vocab,dtype", [(2, 32, 64, 100, torch.float32), (2, 32, 64, 4096, torch.bfloat16),
+                                                    (1, 19, 38, 3000, torch.bfloat16), (2, 3, 64, 2500, torch.float32),
+                                                    (2, 32, 64, 50257, torch.bfloat16), (3, 1, 64, 152064, torch.bfloat16)])
+@pytest.mark.parametrize("kept", [None, 1, 40])
+def test_many_candidates_among_equal_and_masked_ones(groups, k, n, vocab, dtype, kept):
+    x, s = inputs(groups * k, vocab, torch.float32, seed=n + vocab)
+    x = x.round().to(dtype)  # a few dozen distinct values
+    if kept is not None:
+        x[:, kept:] = -float("inf")
+    s = s.round()
+    scores, beams, tokens = beam_select(x, s, k, n)
+    # Equal rows have equal bits; what is equal by the definition is equal here only within a beam:
+    # the totals are the definition's, and no token is chosen twice or before an equal one.
+    totals, _, _ = definition(x, s, k, n)
+    got = scores.cpu().numpy().astype(np.float64)
+    fin = np.isfinite(totals)
+    assert np.array_equal(np.isinf(got), ~fin)
+    assert (np.abs(got - totals)[fin] <= np.abs(totals[fin]) * 2 ** -24 + 2 ** -18).all()
+    for g in range(groups):
+        taken = list(zip(beams[g].tolist(), tokens[g].tolist()))
+        assert len(set(taken)) == n
+        for b in range(k):
+            of_b = [t for beam, t in taken if beam == b]
+            row = x[g * k + b].float()
+            order = torch.argsort(-row.double(), stable=True)[:len(of_b)].tolist()
+            assert of_b == order
+
+
 def test_strided_rows_and_scores_of_any_shape():
     x, s = inputs(6, 4000, seed=8)
     want = check(x, s, 3, 6)
