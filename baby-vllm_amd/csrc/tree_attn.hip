@@ -480,14 +480,17 @@ constexpr int64_t kMaxTreeBytes = 64ll << 20;
 
 // Whether the context gets a launch of its own, and its range. Times in us as measured here,
 // 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
-//   one launch: 4.3 + 1.45 (0.86 at D = 64) per 32-key step of a wave on the longest row, but at
-//     least 2.7 per thousand steps of all waves (half of that at D = 64);
-//   two: 10.8 + 0.5 per tile of a range (0.8 with more than one work-group per CU), + 0.19
+//   one launch: 4.3 + 1.87 (1.29 at D = 64) per 32-key step of a wave on the longest row, but at
+//     least 3.1 per thousand steps of all waves (2.0 at D = 64);
+//   two: 11.8 + 0.8 per tile of a range (1.0 with more than one work-group per CU), + 0.15
 //     per partial that a 16-column tile's waves add one after the other (of 16 waves).
-// The range is as short as about 1.5 work-groups per CU allow (sequences end ranges early: half
-// of one each), and not so short that adding partials outweighs the walk (0.35 times the
-// longest row's tiles, as a root). Over 70 random steps the choice was 1.3% above the best
-// of one launch and twelve ranges on average, 14% at most.
+// The range is as short as about 1.55 work-groups per CU allow (sequences end ranges early: half
+// of one each), and not so short that adding partials outweighs the walk (0.29 times the
+// longest row's tiles, as a root). Where that is more than 24 tiles, and more than a 6.4th of
+// the longest row, it is cut shorter: long ranges leave CUs idle behind the last ones (26
+// sequences of 2100 to 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 70 random
+// steps that the figures were not taken from the choice was 1.7% above the best of one launch
+// and up to 12 ranges on average, 14% at most.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
   const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);
   const int64_t cb = cols <= 64 ? 64 : 128;
@@ -498,20 +501,21 @@ int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_t
   const double max_ranges =
       (double)(kMaxTreeBytes / (prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4));
   if (max_ranges < 1 || longest < 2) return 0;
-  const double work = total * blocks, units = a.num_seqs * blocks, target = 1.5 * device_cus();
+  const double work = total * blocks, units = a.num_seqs * blocks, target = 1.55 * device_cus();
   const double rounds = 1.0 + std::floor(units / target);
-  double range = std::max({work / (rounds * target - units / 2), std::sqrt(0.35 * longest), longest / max_ranges, 3.0});
+  double range = std::max({work / (rounds * target - units / 2), std::sqrt(0.29 * longest), 3.0});
+  range = std::max(std::min(range, std::max(24.0, longest / 6.4)), longest / max_ranges);
   range = std::min({std::ceil(range), longest, (double)(1 << 20)});
 
-  const double small = a.head_dim == 64 ? 0.59 : 1.0, half = a.head_dim == 64 ? 0.5 : 1.0;
+  const double small = a.head_dim == 64 ? 0.69 : 1.0, half = a.head_dim == 64 ? 0.66 : 1.0;
   const double waves = (double)waves_per_column_tile(a), key_waves = waves >= 8 ? waves / 2 : waves;
   const double col_tiles = (double)((cols + 15) / 16) * a.num_kv_heads;
-  const double one = 4.3 + std::max(1.45 * small * std::ceil(2 * longest / key_waves),
-                                    1.35 * half * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
+  const double one = 4.3 + std::max(1.87 * small * std::ceil(2 * longest / key_waves),
+                                    1.53 * half * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
   const double wgs = work / range + units / 2;
-  const double two = 10.8 * (a.head_dim == 64 ? 0.88 : 1.0) +
-                     (wgs < device_cus() ? 0.5 : 0.8) * std::sqrt(half) * range * std::max(1.0, wgs / (2 * device_cus())) +
-                     0.19 * longest / range * (16 / waves) + 2.3 * half * a.num_seqs * col_tiles * 3.5 / 1000;
+  const double two = 11.8 * (a.head_dim == 64 ? 0.88 : 1.0) +
+                     (wgs < device_cus() ? 0.8 : 1.0) * std::sqrt(half) * range * std::max(1.0, wgs / (2 * device_cus())) +
+                     0.15 * longest / range * (16 / waves) + 2.44 * half * a.num_seqs * col_tiles * 3.5 / 1000;
   return one <= two ? 0 : (int32_t)range;
 }
 
