@@ -118,8 +118,8 @@ def paged_tree_attention(q, kv_cache, md, scale):
         split = h.bvllm_tree_split_tiles(num_seqs, num_tokens, max_query_len, num_heads, num_kv_heads, head_dim,
                                          bt.shape[1], total, longest)
         ranges, workspace = 0, None
-        if split > 0:
-            ranges = h.bvllm_prefill_ranges(bt.shape[1], split, longest)
+        if split != 0:
+            ranges = h.bvllm_prefill_ranges(bt.shape[1], abs(split), longest)
             workspace = _lib.optional_scratch(h.bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, ranges),
                                               q.device)
             if workspace is None:

@@ -464,7 +464,9 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
   // Offsets inside one page are 32-bit, and so are (token, head) pairs.
   if ((int64_t)16 * cache_stride_tok > 0x3fffffff || (int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
   if (mask_words < 1 || (int64_t)mask_words * 64 < max_query_len || mask_stride < mask_words) return kBad;
-  if (split_tiles < 0 || split_tiles > (1 << 20)) return kBad;
+  if (split_tiles < -(1 << 20) || split_tiles > (1 << 20)) return kBad;
+  const bool narrow = split_tiles < 0;
+  split_tiles = narrow ? -split_tiles : split_tiles;
   // (More ranges than the table's tiles make would stay empty.)
   if (split_tiles > 0 && (num_ranges < 1 || num_ranges > prefill_ranges(max_blocks, split_tiles, -1))) return kBad;
   if (split_tiles > 0 && (!workspace || !aligned16(workspace))) return kBad;
@@ -483,6 +485,7 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
   if (split_tiles > 0) {
     a.split_tiles = split_tiles;
     a.num_ranges = num_ranges;
+    a.narrow = narrow;
     a.part_out = reinterpret_cast<float*>(workspace);
     a.part_ml = a.part_out + (int64_t)num_ranges * num_tokens * num_heads * head_dim;
   }

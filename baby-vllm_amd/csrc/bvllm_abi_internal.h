@@ -149,14 +149,15 @@ struct TreeArgs {
   int32_t num_seqs, num_tokens, max_query_len;
   int32_t num_heads, num_kv_heads, head_dim;
   // The context on launches of its own (split_tiles > 0): 64-key tiles per range, the most
-  // ranges a sequence has, and their fp32 partials.
+  // ranges a sequence has, whether its blocks have 64 columns (else 128), and the fp32 partials.
   int32_t split_tiles, num_ranges;
+  bool narrow;
   float* part_out;                         // [num_ranges, T, H, D], unnormalized
   float* part_ml;                          // [num_ranges, T, H, 2]: reference (log2 units), sum
 };
 hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
-// 64-key tiles per range of the context's launch for the batch's shape, 0 without one
-// (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
+// 64-key tiles per range of the context's launch for the batch's shape, negative with blocks of
+// 64 columns, 0 without one (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles);
 
 // The K and V caches of several layers, all of one shape.
@@ -283,8 +284,8 @@ int set_tuning(int knob, int value);
 hipError_t paged_prefill(const PrefillArgs& a, hipStream_t stream);
 // The context part of a draft tree step on the prefill kernel: every row over the whole
 // 64-key tiles below its sequence's context length, in at most num_ranges ranges of split_tiles
-// tiles whose partials (part_out, part_ml) the caller adds.
-hipError_t paged_prefill_context(const PrefillArgs& a, hipStream_t stream);
+// tiles whose partials (part_out, part_ml) the caller adds. Blocks of 64 columns (narrow) or 128.
+hipError_t paged_prefill_context(const PrefillArgs& a, bool narrow, hipStream_t stream);
 // Key ranges of a prefill launch: tiles per range (0: no split) for the batch's shape
 // (key_tiles: 64-key tiles its 128-column blocks walk per KV head, longest_tiles: those of
 // its longest sequence of more than one query; < 0 if unknown).

@@ -506,9 +506,9 @@ PyObject* fast_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   int32_t split = g.tree_tiles((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)heads, (int32_t)hkv, (int32_t)d,
                                (int32_t)width, total, longest);
-  const int32_t ranges = split > 0 ? g.ranges((int32_t)width, split, longest) : 0;
+  const int32_t ranges = split != 0 ? g.ranges((int32_t)width, std::abs(split), longest) : 0;
   at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16), ws;
-  if (split > 0) {
+  if (split != 0) {
     ws = optional_scratch(g.tree_bytes((int32_t)tokens, (int32_t)heads, (int32_t)d, ranges), *q);
     if (!ws.defined()) split = 0;
   }

@@ -1100,8 +1100,8 @@ int32_t prefill_split_tiles(const PrefillArgs& a, int64_t key_tiles, int64_t lon
   return tiles;
 }
 
-// The context part of a draft tree step, in blocks of 128 columns or, for at most 64 columns a
-// sequence, of 64 whose waves split the keys; the caller adds the ranges' partials.
+// The context part of a draft tree step, in blocks of 128 columns or (narrow) of 64 whose waves
+// split the keys; the caller adds the ranges' partials.
 template <int D, int QT, int KS>
 static hipError_t launch_context(const PrefillArgs& a, hipStream_t stream) {
   constexpr int CB = 4 / KS * QT * 16;
@@ -1114,8 +1114,7 @@ static hipError_t launch_context(const PrefillArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-hipError_t paged_prefill_context(const PrefillArgs& a, hipStream_t stream) {
-  const bool narrow = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads) <= 64;
+hipError_t paged_prefill_context(const PrefillArgs& a, bool narrow, hipStream_t stream) {
   if (a.head_dim == 64) return narrow ? launch_context<64, 2, 2>(a, stream) : launch_context<64, 2, 1>(a, stream);
   return narrow ? launch_context<128, 2, 2>(a, stream) : launch_context<128, 2, 1>(a, stream);
 }

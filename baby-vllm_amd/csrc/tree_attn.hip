@@ -445,7 +445,7 @@ hipError_t launch_context_part(const TreeArgs& a, hipStream_t stream) {
   p.num_heads = a.num_heads; p.num_kv_heads = a.num_kv_heads; p.head_dim = a.head_dim;
   p.split_tiles = a.split_tiles; p.num_ranges = a.num_ranges;
   p.part_out = a.part_out; p.part_ml = a.part_ml;
-  return paged_prefill_context(p, stream);
+  return paged_prefill_context(p, a.narrow, stream);
 }
 
 // Waves (slices times key waves) that each 16-column tile gets: what fills the card at two
@@ -478,45 +478,53 @@ hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream) {
 // Partials hold every token of the step for every range: at most this many bytes.
 constexpr int64_t kMaxTreeBytes = 64ll << 20;
 
-// Whether the context gets a launch of its own, and its range. Times in us as measured here,
-// 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
-//   one launch: 4.3 + 1.87 (1.29 at D = 64) per 32-key step of a wave on the longest row, but at
-//     least 3.1 per thousand steps of all waves (2.0 at D = 64);
-//   two: 11.8 + 0.8 per tile of a range (1.0 with more than one work-group per CU), + 0.15
-//     per partial that a 16-column tile's waves add one after the other (of 16 waves).
-// The range is as short as about 1.55 work-groups per CU allow (sequences end ranges early: half
-// of one each), and not so short that adding partials outweighs the walk (0.29 times the
-// longest row's tiles, as a root). Where that is more than 24 tiles, and more than a 6.4th of
-// the longest row, it is cut shorter: long ranges leave CUs idle behind the last ones (26
-// sequences of 2100 to 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 70 random
-// steps that the figures were not taken from the choice was 1.7% above the best of one launch
-// and up to 12 ranges on average, 14% at most.
+// Whether the context gets a launch of its own, its range and its blocks (negative: of 64 columns).
+// Times in us as measured here, 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
+//   one launch: 4.3 + 2.0 (1.3 at D = 64) per 32-key step of a wave on the longest row, but at
+//     least 2.4 per thousand steps of all waves;
+//   two: 13.2 (11.6 at D = 64) + 0.5 per tile of a range in blocks of 64 columns, 0.8 to 1.2
+//     of 128 (with more than one work-group per CU), + 0.15 per partial that a 16-column
+//     tile's waves add one after the other (of 16 waves).
+// Blocks of 64 columns, whose waves share a tile's keys, walk a tile in half the time where
+// work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 34.4 us, with 128
+// columns 38.9; 8 trees of 11 to 45: 29.3 and 32.6); they read the keys twice as often, which
+// counts once there are more than 18 128-column tiles per CU (57 at D = 64): 21 trees of 5 to 18
+// behind 4858: 71 and 61.
+// The range is as short as about 1.5 work-groups per CU allow (sequences end ranges early: half
+// of one each), and not so short that adding partials outweighs the walk (a third of the
+// longest row's tiles, as a root). Where that is more than 20 tiles, and more than a 6th or 12th
+// of the longest row, it is cut shorter: long ranges leave CUs idle behind the last ones (26
+// sequences of 2100 to 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random
+// steps the choice was 2.4% above the best of one launch and up to 22 ranges of either
+// block on average, 35% at most.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
+  const bool d64 = a.head_dim == 64;
   const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);
-  const int64_t cb = cols <= 64 ? 64 : 128;
-  const double blocks = (double)((cols + cb - 1) / cb * a.num_kv_heads);
   const int64_t table_tiles = ((int64_t)a.max_blocks + 3) / 4;
   const double longest = (double)(longest_tiles >= 0 ? std::min(table_tiles, longest_tiles) : table_tiles);
   const double total = key_tiles >= 0 ? (double)key_tiles : longest * a.num_seqs;
   const double max_ranges =
       (double)(kMaxTreeBytes / (prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4));
   if (max_ranges < 1 || longest < 2) return 0;
-  const double work = total * blocks, units = a.num_seqs * blocks, target = 1.55 * device_cus();
+  const double cus = device_cus();
+  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 57 : 18) * cus;
+  const int64_t cb = narrow ? 64 : 128;
+  const double blocks = (double)((cols + cb - 1) / cb * a.num_kv_heads);
+  const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.45 : 1.6) * cus;
   const double rounds = 1.0 + std::floor(units / target);
-  double range = std::max({work / (rounds * target - units / 2), std::sqrt(0.29 * longest), 3.0});
-  range = std::max(std::min(range, std::max(24.0, longest / 6.4)), longest / max_ranges);
-  range = std::min({std::ceil(range), longest, (double)(1 << 20)});
+  double range = std::max({work / (rounds * target - units / 2), std::sqrt((narrow ? 0.27 : 0.33) * longest), 3.0});
+  range = std::min(range, narrow ? std::max(20.0, longest / 12) : std::max(23.0, longest / 5.7));
+  range = std::min({std::ceil(std::max(range, longest / max_ranges)), longest, (double)(1 << 20)});
 
-  const double small = a.head_dim == 64 ? 0.69 : 1.0, half = a.head_dim == 64 ? 0.66 : 1.0;
   const double waves = (double)waves_per_column_tile(a), key_waves = waves >= 8 ? waves / 2 : waves;
   const double col_tiles = (double)((cols + 15) / 16) * a.num_kv_heads;
-  const double one = 4.3 + std::max(1.87 * small * std::ceil(2 * longest / key_waves),
-                                    1.53 * half * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
+  const double one = 4.3 + std::max((d64 ? 1.3 : 2.0) * std::ceil(2 * longest / key_waves),
+                                    1.2 * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
   const double wgs = work / range + units / 2;
-  const double two = 11.8 * (a.head_dim == 64 ? 0.88 : 1.0) +
-                     (wgs < device_cus() ? 0.8 : 1.0) * std::sqrt(half) * range * std::max(1.0, wgs / (2 * device_cus())) +
-                     0.15 * longest / range * (16 / waves) + 2.44 * half * a.num_seqs * col_tiles * 3.5 / 1000;
-  return one <= two ? 0 : (int32_t)range;
+  const double two = (d64 ? 11.6 : 13.2) +
+                     (narrow ? 0.5 : wgs < cus ? 0.8 : 1.2) * range * std::max(1.0, wgs / (2 * cus)) +
+                     0.15 * longest / range * (16 / waves) + 2.55 * a.num_seqs * col_tiles * 3.5 / 1000;
+  return one <= two ? 0 : narrow ? -(int32_t)range : (int32_t)range;
 }
 
 }  // namespace bvllm

@@ -351,12 +351,13 @@ BVLLM_API int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t vo
  * split_tiles > 0 gives the whole 64-key tiles below every context length to a launch of its
  * own, cut into at most num_ranges ranges a sequence, of split_tiles tiles where that
  * suffices, whose fp32 partials in workspace (bvllm_tree_workspace_bytes(num_tokens,
- * num_heads, head_dim, num_ranges) bytes) a second launch adds to the other keys. 0: one
+ * num_heads, head_dim, num_ranges) bytes) a second launch adds to the other keys. < 0: the
+ * same with ranges of -split_tiles tiles and narrower blocks (64 columns instead of 128). 0: one
  * launch over all keys, no workspace. bvllm_tree_split_tiles returns the split_tiles to use
- * (0: none) from host sizes alone: key_tiles is ceil(seq_len / 64) summed over the
- * sequences, longest_tiles the largest of them, each -1 if unknown; bvllm_prefill_ranges the
- * num_ranges. They steer the choice only; results agree within the rounding of fp32 sums in
- * another order.
+ * from host sizes alone: key_tiles is ceil(seq_len / 64) summed over the sequences,
+ * longest_tiles the largest of them, each -1 if unknown; bvllm_prefill_ranges the num_ranges
+ * (of split_tiles without its sign). They steer the choice only; results agree within the
+ * rounding of fp32 sums in another order.
  */
 BVLLM_API int32_t bvllm_tree_split_tiles(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks,

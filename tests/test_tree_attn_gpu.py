@@ -177,13 +177,13 @@ def raw_call(q, cache, md, scale, split, ranges):
 
 
 @pytest.mark.parametrize("heads", [(2, 7, 128), (2, 7, 64), (1, 3, 128), (1, 2, 64)], ids=str)
-@pytest.mark.parametrize("split", [0, 1, 2, 3, 5, 12, 1000])
+@pytest.mark.parametrize("split", [0, 1, 2, 3, 5, 12, 1000, -1, -2, -3, -5, -12, -1000])
 def test_context_ranges_of_any_length(heads, split):
     # Contexts of no whole tile, of one, of several; blocks of 64 and of 128 columns.
     rng = random.Random(1)
     q, cache, md = build([(c, random_tree(rng, n)) for c, n in ((700, 9), (0, 3), (33, 40), (1500, 1), (64, 5), (127, 2))], *heads)
     want = formula(q, cache, md, 0.1)
-    widest = max(1, cdiv(cdiv(md.block_tables.shape[1], 4), max(1, split)))
+    widest = max(1, cdiv(cdiv(md.block_tables.shape[1], 4), max(1, abs(split))))
     for ranges in sorted({1, 2, (widest + 1) // 2, widest} & set(range(1, widest + 1))):
         check(raw_call(q, cache, md, 0.1, split, ranges), want)
 
@@ -197,6 +197,7 @@ def test_every_number_of_waves_per_column(seqs, heads):
     want = formula(q, cache, md, 0.1)
     check(raw_call(q, cache, md, 0.1, 0, 0), want)
     check(raw_call(q, cache, md, 0.1, 1, 2), want)
+    check(raw_call(q, cache, md, 0.1, -1, 2), want)
 
 
 def test_masks_that_leave_rows_without_keys_or_without_themselves():
@@ -374,7 +375,7 @@ def test_no_memory_for_the_scratch_takes_the_whole_rows(monkeypatch):
 
     q, cache, md = build([(4000, random_tree(random.Random(6), 16))], 2, 7, 64)
     python_path(monkeypatch)
-    assert _lib.lib().bvllm_tree_split_tiles(1, 16, 16, 14, 2, 64, md.block_tables.shape[1], 63, 63) > 0
+    assert _lib.lib().bvllm_tree_split_tiles(1, 16, 16, 14, 2, 64, md.block_tables.shape[1], 63, 63) != 0
     monkeypatch.setattr(_lib, "optional_scratch", lambda n, dev: None)
     run(q, cache, md)
 
