@@ -433,7 +433,7 @@ extern "C" int32_t bvllm_tree_split_tiles(int32_t num_seqs, int32_t num_tokens, 
 extern "C" int64_t bvllm_tree_workspace_bytes(int32_t num_tokens, int32_t num_heads, int32_t head_dim,
                                               int32_t num_ranges) {
   if (num_tokens < 1 || num_heads < 1 || head_dim < 1 || num_ranges < 1) return 0;
-  return prefill_range_floats(num_ranges, num_tokens, num_heads, head_dim) * (int64_t)sizeof(float);
+  return prefill_range_floats(num_ranges + 1, num_tokens, num_heads, head_dim) * (int64_t)sizeof(float);
 }
 
 extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
@@ -487,7 +487,7 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
     a.num_ranges = num_ranges;
     a.narrow = narrow;
     a.part_out = reinterpret_cast<float*>(workspace);
-    a.part_ml = a.part_out + (int64_t)num_ranges * num_tokens * num_heads * head_dim;
+    a.part_ml = a.part_out + ((int64_t)num_ranges + 1) * num_tokens * num_heads * head_dim;
   }
   return (int)paged_tree_attention(a, (hipStream_t)stream);
 }

@@ -152,8 +152,9 @@ struct TreeArgs {
   // ranges a sequence has, whether its blocks have 64 columns (else 128), and the fp32 partials.
   int32_t split_tiles, num_ranges;
   bool narrow;
-  float* part_out;                         // [num_ranges, T, H, D], unnormalized
-  float* part_ml;                          // [num_ranges, T, H, 2]: reference (log2 units), sum
+  FastDiv by_kv_heads, by_group, by_heads;  // by num_kv_heads, num_heads / num_kv_heads, num_heads (of the launches)
+  float* part_out;                         // [num_ranges + 1, T, H, D], unnormalized
+  float* part_ml;                          // [num_ranges + 1, T, H, 2]: reference (log2 units), sum
 };
 hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
 // 64-key tiles per range of the context's launch for the batch's shape, negative with blocks of
@@ -282,10 +283,10 @@ enum TuneKnob {
 int tuning(int knob);
 int set_tuning(int knob, int value);
 hipError_t paged_prefill(const PrefillArgs& a, hipStream_t stream);
-// The context part of a draft tree step on the prefill kernel: every row over the whole
-// 64-key tiles below its sequence's context length, in at most num_ranges ranges of split_tiles
-// tiles whose partials (part_out, part_ml) the caller adds. Blocks of 64 columns (narrow) or 128.
-hipError_t paged_prefill_context(const PrefillArgs& a, bool narrow, hipStream_t stream);
+// The keys of a draft tree step on the prefill kernel: every row over the whole 64-key tiles below
+// its sequence's context length, in at most num_ranges ranges of split_tiles tiles, and beside
+// them over the keys behind, whose partials (part_out, part_ml) the caller adds.
+hipError_t paged_prefill_context(const PrefillArgs& a, const TreeArgs& tree, hipStream_t stream);
 // Key ranges of a prefill launch: tiles per range (0: no split) for the batch's shape
 // (key_tiles: 64-key tiles its 128-column blocks walk per KV head, longest_tiles: those of
 // its longest sequence of more than one query; < 0 if unknown).

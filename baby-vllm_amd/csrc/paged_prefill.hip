@@ -40,6 +40,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace bvllm {
 
@@ -114,7 +115,8 @@ constexpr int kDecodeDepth = 1;
 // work-group that always writes its partial.
 template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
-                                                                  int xcd_group, int per_xcd, DecodeArgs dec,
+                                                                  int xcd_group, int per_xcd,
+                                                                  std::conditional_t<CTX, TreeArgs, DecodeArgs> dec,
                                                                   int n_dec_wgs, int bpw) {
   constexpr int KT = 64;
   constexpr int RB = 2 * D;   // bytes of one key row of K or V (no padding)
@@ -139,7 +141,20 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // otherwise fills each CU's memory queue in front of them (mixed step
   // 1 x 512 + 63 decodes: 34.6 -> 29.5 us).
   const int n_pre_wgs = (int)gridDim.x - n_dec_wgs;
-  if (!CTX && (int)blockIdx.x >= n_pre_wgs) {
+  if constexpr (CTX) {
+    // The last n_dec_wgs work-groups take the keys behind the whole tiles, a wave 16 columns; those
+    // of one (sequence, KV head) follow each other on one XCD.
+    static_assert(NW * 4 * kTreeStep * D <= sizeof(lds), "the waves' V buffers");
+    if ((int)blockIdx.x >= n_pre_wgs) {
+      const int t = (int)blockIdx.x - n_pre_wgs;
+      const int groups = (dec.max_query_len * (dec.num_heads / dec.num_kv_heads) + 16 * NW - 1) / (16 * NW);
+      const int pair = (t >> 3) / groups * 8 + (t & 7), s = pair / dec.num_kv_heads;
+      if (pair < dec.num_seqs * dec.num_kv_heads)
+        tree_columns<D, 1, 1, true>(dec, lds + wave_id() * 4 * kTreeStep * D, 0, s, pair - s * dec.num_kv_heads,
+                                    ((t >> 3) % groups * NW + wave_id()) * 16, 0);
+      return;
+    }
+  } else if ((int)blockIdx.x >= n_pre_wgs) {
     const int dw = (int)blockIdx.x - n_pre_wgs;
     if (dec.chunk_target > 0)  // uneven rows: cut into chunks (RowChunk)
       decode_work_group<D, kDecodeWaves, kDecodeDepth, true, true>(dec, dw, reinterpret_cast<float*>(lds));
@@ -1100,23 +1115,25 @@ int32_t prefill_split_tiles(const PrefillArgs& a, int64_t key_tiles, int64_t lon
   return tiles;
 }
 
-// The context part of a draft tree step, in blocks of 128 columns or (narrow) of 64 whose waves
-// split the keys; the caller adds the ranges' partials.
+// The context part of a draft tree step, in blocks of 128 columns or (tree.narrow) of 64 whose
+// waves split the keys, and its tail; the caller adds the partials.
 template <int D, int QT, int KS>
-static hipError_t launch_context(const PrefillArgs& a, hipStream_t stream) {
+static hipError_t launch_context(const PrefillArgs& a, const TreeArgs& tree, hipStream_t stream) {
   constexpr int CB = 4 / KS * QT * 16;
-  const int64_t blocks = ((int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads) + CB - 1) / CB;
+  const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);
+  const int64_t blocks = (cols + CB - 1) / CB;
   const int64_t per_xcd = ((int64_t)a.num_seqs * a.num_kv_heads + 7) / 8;
-  const int64_t wgs = 8 * per_xcd * blocks * a.num_ranges;
-  if (wgs > 0x7ffffff0 || blocks * a.num_seqs > 0x7ffffff0) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, true, true>), dim3((unsigned)wgs), dim3(4 * 64), 0,
-                     stream, a, (int)(blocks * a.num_seqs), (int)blocks, 0, (int)per_xcd, DecodeArgs{}, 0, a.num_ranges);
+  const int64_t wgs = 8 * per_xcd * blocks * a.num_ranges, tails = 8 * per_xcd * ((cols + 63) / 64);
+  if (wgs + tails > 0x7ffffff0 || blocks * a.num_seqs > 0x7ffffff0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, true, true>), dim3((unsigned)(wgs + tails)), dim3(4 * 64),
+                     0, stream, a, (int)(blocks * a.num_seqs), (int)blocks, 0, (int)per_xcd, tree, (int)tails,
+                     a.num_ranges);
   return hipGetLastError();
 }
 
-hipError_t paged_prefill_context(const PrefillArgs& a, bool narrow, hipStream_t stream) {
-  if (a.head_dim == 64) return narrow ? launch_context<64, 2, 2>(a, stream) : launch_context<64, 2, 1>(a, stream);
-  return narrow ? launch_context<128, 2, 2>(a, stream) : launch_context<128, 2, 1>(a, stream);
+hipError_t paged_prefill_context(const PrefillArgs& a, const TreeArgs& tree, hipStream_t stream) {
+  if (a.head_dim == 64) return tree.narrow ? launch_context<64, 2, 2>(a, tree, stream) : launch_context<64, 2, 1>(a, tree, stream);
+  return tree.narrow ? launch_context<128, 2, 2>(a, tree, stream) : launch_context<128, 2, 1>(a, tree, stream);
 }
 
 // Two column tiles per wave (128 columns per work-group) unless that grid

@@ -78,7 +78,7 @@ def test_context_ranges_fit_the_table_and_the_scratch():
             taken[split > 0] += 1
             ranges = h.bvllm_prefill_ranges(width, abs(split), longest)
             assert 1 <= ranges <= h.bvllm_prefill_ranges(width, abs(split), -1)
-            assert h.bvllm_tree_workspace_bytes(seqs * n, heads, d, ranges) == ranges * seqs * n * heads * (d + 2) * 4 <= 64 << 20
+            assert h.bvllm_tree_workspace_bytes(seqs * n, heads, d, ranges) == (ranges + 1) * seqs * n * heads * (d + 2) * 4 <= 64 << 20
     assert min(taken) > 200
     assert h.bvllm_tree_workspace_bytes(8, 28, 128, 0) == 0
     # One short chat stays on one launch; a long document does not.
