@@ -112,7 +112,8 @@ constexpr int kDecodeDepth = 1;
 // CTX: the context part of a draft tree step (tree_attn.hip): every row sees every key of the
 // whole 64-key tiles below its sequence's context length, so nothing is masked and no tile is
 // partial. A sequence's tiles are cut evenly into ranges of at most a.split_tiles, each a
-// work-group that always writes its partial.
+// work-group that always writes its partial. The last n_dec_wgs work-groups take the keys behind
+// them, with masks (tree_columns).
 template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
                                                                   int xcd_group, int per_xcd,

@@ -1,5 +1,6 @@
-// What the two launches of a draft tree step share (tree_attn.hip, and the context part in
-// paged_prefill.hip): how a sequence's keys are divided between them, and what a row sees.
+// The waves that walk a draft tree step's keys with masks (of tree_attn.hip, where the whole is
+// described, and beside the context's work-groups in paged_prefill.hip), how a sequence's keys are
+// divided between the two, and what a row sees.
 #pragma once
 
 #include "bvllm_abi_internal.h"

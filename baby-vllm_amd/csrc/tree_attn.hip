@@ -8,22 +8,32 @@
 // over the keys that row i sees: every position below ctx, and ctx + j where bit j of
 // the row's mask words is set. A row that sees no key gives zeros.
 //
-// Long contexts run on a launch of their own (paged_prefill.hip, CTX): there every row sees
-// every key, so it walks whole 64-key tiles without a mask, in ranges, and leaves fp32
-// partials. The kernel here takes the rest, at most 63 context keys and the drafted ones, with
-// the masks, adds the partials and writes the output; short contexts it takes whole.
+// Short contexts take one launch over all keys (tree_attn_kernel). Long ones are cut: below the
+// context length every row sees every key, so work-groups of the prefill kernel walk
+// whole 64-key tiles without a mask, in ranges (paged_prefill.hip, CTX); on the same launch waves
+// of their own take the rest, at most 63 context keys and the drafted ones, with the
+// masks (the tail); all leave fp32 partials that a second launch adds. (The tail on the second
+// launch, which then added the partials to its own walk: 16 trees of 64 tokens 109 us, now 91; 8
+// trees of 11 to 45 30 and 26.)
 //
-// Work-group = (sequence, KV head, 16 columns, DS-th of the head's dims). A column is one of
-// the sequence's (drafted token, query head) pairs of the KV head, numbered token first, so
-// the GQA group shares every key. The NW waves of a work-group hold the same columns and take
-// 32-key steps (and partials) in turn, each with a running maximum and sum of its own; their
-// states meet once, through LDS. No wave waits for another inside the walk: a wave's K step
-// goes from the cache straight into MFMA operand registers (a key's row is a lane's operand),
-// its V step into a private double buffer in LDS by direct global->LDS loads, from where
-// transpose reads form the operand.
-//   Sᵀ[32 keys × 16 cols] = K · Qᵀ,  Oᵀ[D/DS × 16 cols] += Vᵀ · Pᵀ   (mfma 16x16x32)
+// What bounds it: 48 chains of 2 to 7 tokens behind 200 to 4000 read 125 MB of keys in 35 us
+// (3.6 TB/s) and 4 more on the second launch; 16 trees of 64 behind 1000 to 8000 multiply at 0.6
+// PFLOP/s in 82 us (their 448 columns fill 3.5 of 4 blocks, and ranges are uneven); a few trees
+// are bound by the chain of a range's round trips and tiles, and by the second launch (4.4 us).
+//
+// The walk with masks (tree_attn.h, tree_columns): a column is one of the sequence's (drafted token,
+// query head) pairs of the KV head, numbered token first, so the GQA group shares every key.
+// A wave holds 16 columns and takes 32-key steps. On the launch over all keys a work-group is
+// (sequence, KV head, 16 columns, DS-th of the head's dims); its NW waves hold the same columns and
+// take steps in turn, each with a running maximum and sum of its own, and their states
+// meet once, through LDS. No wave waits for another inside the walk: a wave's K step goes from the
+// cache straight into MFMA operand registers (a key's row is a lane's operand), its V step
+// into a private double buffer in LDS by direct global->LDS loads, from where transpose reads
+// form the operand.
+//   S^T[32 keys x 16 cols] = K Q^T,  O^T[D/DS x 16 cols] += V^T P^T   (mfma 16x16x32)
 // A walk of a few steps is a chain of round trips (metadata, table, keys, states), so waves
-// are spent until the card is full (tree_for_dim).
+// are spent until the card is full (tree_for_dim): one tree of 8 behind 300 takes 5.3 us on 8 waves
+// per 16 columns.
 // Sums, maxima and outputs are fp32 up to the final rounding. P is rounded to bf16 for its
 // MFMA, and the row sum adds the rounded values, so a weight's rounding error (at most 2^-8)
 // cancels where one key dominates and averages out where many do.
@@ -174,25 +184,25 @@ hipError_t paged_tree_attention(const TreeArgs& args, hipStream_t stream) {
 // Partials hold every token of the step for every range: at most this many bytes.
 constexpr int64_t kMaxTreeBytes = 64ll << 20;
 
-// Whether the context gets a launch of its own, its range and its blocks (negative: of 64 columns).
-// Times in us as measured here, 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
-//   one launch: 4.3 + 2.0 (1.3 at D = 64) per 32-key step of a wave on the longest row, but at
+// Whether the context runs in ranges, their length and their blocks (negative: of 64 columns). Times in
+// us as measured here, 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
+//   one launch: 4.3 + 1.8 (1.15 at D = 64) per 32-key step of a wave on the longest row, but at
 //     least 2.4 per thousand steps of all waves;
-//   two: 13.2 (11.6 at D = 64) + 0.5 per tile of a range in blocks of 64 columns, 0.8 to 1.2
-//     of 128 (with more than one work-group per CU), + 0.15 per partial that a 16-column
-//     tile's waves add one after the other (of 16 waves).
+//   two: 8.7 (10.3 at D = 64) + 0.4 per tile of a range in blocks of 64 columns (0.57 with more
+//     than one work-group per CU), 0.9 and 1.6 of 128, + 0.17 per range of the longest row, less
+//     where waves are few, + 7.7 per thousand 16-column tiles, the tail's.
 // Blocks of 64 columns, whose waves share a tile's keys, walk a tile in half the time where
 // work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 34.4 us, with 128
 // columns 38.9; 8 trees of 11 to 45: 29.3 and 32.6); they read the keys twice as often, which
-// counts once there are more than 18 128-column tiles per CU (57 at D = 64): 21 trees of 5 to 18
+// counts once there are more than 18.7 128-column tiles per CU (57 at D = 64): 21 trees of 5 to 18
 // behind 4858: 71 and 61.
 // The range is as short as about 1.5 work-groups per CU allow (sequences end ranges early: half
-// of one each), and not so short that adding partials outweighs the walk (a third of the
-// longest row's tiles, as a root). Where that is more than 20 tiles, and more than a 6th or 12th
-// of the longest row, it is cut shorter: long ranges leave CUs idle behind the last ones (26
-// sequences of 2100 to 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random
-// steps the choice was 2.4% above the best of one launch and up to 22 ranges of either
-// block on average, 35% at most.
+// of one each), and not so short that adding partials outweighs the walk (a root of the longest
+// row's tiles). Where that is more than 20 tiles, and more than a 6th or 15th of the longest row,
+// it is cut shorter: long ranges leave CUs idle behind the last ones (26 sequences of 2100 to
+// 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random steps the choice
+// was 2.7% above the best of one launch and up to 22 ranges of either block on average, 35%
+// at most.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
   const bool d64 = a.head_dim == 64;
   const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);
@@ -203,23 +213,23 @@ int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_t
       (double)(kMaxTreeBytes / (prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4) - 1);
   if (max_ranges < 1 || longest < 2) return 0;
   const double cus = device_cus();
-  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 57 : 18) * cus;
+  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 57 : 18.7) * cus;
   const int64_t cb = narrow ? 64 : 128;
   const double blocks = (double)((cols + cb - 1) / cb * a.num_kv_heads);
-  const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.45 : 1.6) * cus;
+  const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.45 : 1.7) * cus;
   const double rounds = 1.0 + std::floor(units / target);
-  double range = std::max({work / (rounds * target - units / 2), std::sqrt((narrow ? 0.27 : 0.33) * longest), 3.0});
-  range = std::min(range, narrow ? std::max(20.0, longest / 12) : std::max(23.0, longest / 5.7));
+  double range = std::max(work / (rounds * target - units / 2), std::sqrt((narrow ? 0.43 : 0.16) * longest));
+  range = std::max(range, narrow ? 4.0 : 3.0);
+  range = std::min(range, narrow ? std::max(20.0, longest / 15) : std::max(23.0, longest / 6.3));
   range = std::min({std::ceil(std::max(range, longest / max_ranges)), longest, (double)(1 << 20)});
 
   const double waves = (double)waves_per_column_tile(a), key_waves = waves >= 8 ? waves / 2 : waves;
   const double col_tiles = (double)((cols + 15) / 16) * a.num_kv_heads;
-  const double one = 4.3 + std::max((d64 ? 1.3 : 2.0) * std::ceil(2 * longest / key_waves),
+  const double one = 4.3 + std::max((d64 ? 1.15 : 1.8) * std::ceil(2 * longest / key_waves),
                                     1.2 * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
-  const double wgs = work / range + units / 2;
-  const double two = (d64 ? 11.6 : 13.2) +
-                     (narrow ? 0.5 : wgs < cus ? 0.8 : 1.2) * range * std::max(1.0, wgs / (2 * cus)) +
-                     0.15 * longest / range * (16 / waves) + 2.55 * a.num_seqs * col_tiles * 3.5 / 1000;
+  const double wgs = work / range + units / 2, alone = narrow ? 0.39 : 0.9, shared = narrow ? 0.57 : 1.6;
+  const double two = (d64 ? 10.3 : 8.7) + (wgs < cus ? alone : shared) * range * std::max(1.0, wgs / (2 * cus)) +
+                     0.17 * longest / range * (16 / waves) + 7.7 * a.num_seqs * col_tiles / 1000;
   return one <= two ? 0 : narrow ? -(int32_t)range : (int32_t)range;
 }
 
