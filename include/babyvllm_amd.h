@@ -1,7 +1,7 @@
 /*
  * babyvllm_amd — C ABI of the MI355X (gfx950) paged-KV hot path.
  *
- * Three operations, each a drop-in for one Python entry point of the
+ * The attention path's three operations are drop-ins for Python entry points of the
  * reference's babyvllm/kernels package:
  *
  *   bvllm_rope_kv_append  <- fused_rope_and_cache      (babyvllm/kernels/rope.py:101-153)
