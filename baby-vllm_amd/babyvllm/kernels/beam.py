@@ -21,7 +21,7 @@ MAX_CANDIDATES = 64
 def beam_select(logits, scores, num_beams: int, num_candidates: int | None = None):
     """The best continuations of every group of ``num_beams`` rows: ``(scores, beams, tokens)``.
 
-    ``logits`` ``[G * K, vocab]`` bf16 or fp32 with unit column stride, ``scores`` fp32 (one
+    ``logits`` ``[G * K, vocab]`` bf16 or fp32 with unit column stride (rows may be one, expanded), ``scores`` fp32 (one
     per row, in any shape): the beams' summed log-probabilities. A continuation's total is
     ``score + logit - logsumexp(logits of the beam)``. Returned are the ``num_candidates``
     (default ``2 * K``, at most 64) best of each group, fp32 totals, int64 beam numbers within
@@ -30,7 +30,9 @@ def beam_select(logits, scores, num_beams: int, num_candidates: int | None = Non
     finite (an unused one: -inf), or whose logits hold a NaN, a +inf or no finite value,
     has totals of -inf.
     """
-    if logits.is_cuda and num_candidates is not None:
+    if num_candidates is None and logits.dim() == 2:
+        num_candidates = min(2 * num_beams, num_beams * logits.shape[1])
+    if logits.is_cuda:
         done = _lib.fast().beam(logits, scores, num_beams, num_candidates, MAX_BEAMS, MAX_CANDIDATES, *_lib.current())
         if done is not None:
             return done
@@ -49,7 +51,7 @@ def beam_select(logits, scores, num_beams: int, num_candidates: int | None = Non
         raise ValueError(f"num_beams must be 1 to {MAX_BEAMS} and divide the {rows} rows, got {num_beams}")
     if scores.numel() != rows:
         raise ValueError(f"scores has {scores.numel()} values for {rows} rows")
-    n = min(2 * num_beams, num_beams * vocab) if num_candidates is None else int(num_candidates)
+    n = int(num_candidates)
     if not 1 <= n <= min(MAX_CANDIDATES, num_beams * vocab):
         raise ValueError(f"num_candidates must be 1 to {min(MAX_CANDIDATES, num_beams * vocab)}, got {n}")
     groups = rows // num_beams

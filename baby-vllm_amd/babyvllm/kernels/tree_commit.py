@@ -33,6 +33,8 @@ def layer_caches(kv_caches, device):
             raise ValueError(f"kv_caches[{i}] must be [2, NB, BS, Hkv, D] with a unit last stride, got {tuple(c.shape)}")
         if c.shape != caches[0].shape or c.stride() != caches[0].stride():
             raise ValueError(f"kv_caches[{i}] has another shape or layout than kv_caches[0]")
+    if len({c.data_ptr() for c in caches}) < len(caches):
+        raise ValueError("a cache is in kv_caches twice")
     k = (ctypes.c_void_p * max(1, len(caches)))(*[c.data_ptr() for c in caches])
     v = (ctypes.c_void_p * max(1, len(caches)))(*[c[1].data_ptr() for c in caches])
     return caches, k, v
@@ -49,7 +51,7 @@ def cache_shape(caches):
 def commit_draft_tree(kv_caches, md, draft_tokens, target_tokens, parents, max_path: int | None = None):
     """Moves the verified paths' K/V behind the contexts; returns ``(path, accepted, following)``.
 
-    ``kv_caches`` are the layers' caches (all of one shape; none: only the walk).
+    ``kv_caches`` are the layers' caches (all of one shape, each once; none: only the walk).
     ``draft_tokens`` and ``target_tokens`` int64 ``[T]`` and ``parents`` int32 ``[T]`` (node
     numbers within the sequence, before their children; -1 for the root) follow ``md.query_start_loc``.
     ``max_path`` bounds the accepted nodes (default ``md.max_query_len``).

@@ -480,7 +480,8 @@ extern "C" int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int
   a.tree_mask = tree_mask; a.mask_stride = mask_stride; a.mask_words = mask_words;
   a.scale_log2 = scale * kLog2e;
   a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
-  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.max_query_len = max_query_len;
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens;
+  a.max_query_len = max_query_len < num_tokens ? max_query_len : num_tokens;  // (columns are numbered in 32 bits)
   a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
   if (split_tiles > 0) {
     a.split_tiles = split_tiles;
@@ -497,8 +498,11 @@ static bool cache_set_ok(void* const* k, void* const* v, int32_t layers, int64_t
                          int32_t nb, int32_t hkv, int32_t d, int32_t block_size) {
   if (layers < 0 || hkv < 1 || d < 8 || d % 8 || block_size != 16 || (layers > 0 && (!k || !v))) return false;
   if ((int64_t)hkv * d > 1 << 20) return false;  // chunks of 64 layers' rows are numbered in 32 bits
-  for (int32_t i = 0; i < layers; ++i)
+  for (int32_t i = 0; i < layers; ++i) {
     if (!cache_ok(k[i], v[i], sb, st, sh, nb)) return false;
+    for (int32_t j = 0; j < i; ++j)  // (a cache named twice would be moved twice at once)
+      if (k[j] == k[i]) return false;
+  }
   return true;
 }
 
@@ -544,7 +548,7 @@ extern "C" int bvllm_beam_select(const void* logits, int64_t row_stride, int32_t
   if (((int64_t)vocab + kBeamPiece - 1) / kBeamPiece * num_beams > kBeamMaxPieces) return kBad;
   if (num_groups == 0) return 0;
   if ((int64_t)num_groups * num_beams > 0x7fffffff) return kBad;
-  if (!logits || !scores || !workspace || !out_scores || !out_beams || !out_tokens || row_stride < vocab) return kBad;
+  if (!logits || !scores || !workspace || !out_scores || !out_beams || !out_tokens || row_stride < 0) return kBad;
   if (((uintptr_t)workspace & 7u) != 0 || ((uintptr_t)logits & (logits_fp32 ? 3u : 1u)) != 0) return kBad;
   BeamSelectArgs a{};
   a.logits = logits; a.row_stride = row_stride; a.fp32 = logits_fp32;

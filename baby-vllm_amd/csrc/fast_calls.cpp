@@ -549,6 +549,9 @@ bool plain_layers(PyObject* o, int64_t dev, Layers& l) {
     if (!plain_cache(c)) return false;
     if (i == 0) l.one = c;
     else if (c->sizes() != l.one->sizes() || c->strides() != l.one->strides()) return false;
+    l.k[i] = ptr(*c);
+    for (Py_ssize_t j = 0; j < i; ++j)
+      if (l.k[j] == l.k[i]) return false;
   }
   return l.one->size(2) == kPage && small(l.one->size(4));
 }

@@ -157,7 +157,7 @@ template <int D>
 hipError_t tree_for_dim(const TreeArgs& a, hipStream_t stream) {
   if (a.split_tiles > 0) {
     const int64_t chunks = ((int64_t)a.max_query_len * a.num_heads * (D / 4) + 255) / 256;
-    if (chunks * a.num_seqs > 0x7fffffff) return hipErrorInvalidValue;
+    if (chunks * a.num_seqs > 0x7fffffff || chunks * 256 > 0x7fffffff) return hipErrorInvalidValue;
     const hipError_t err = launch_context_part(a, stream);
     if (err != hipSuccess) return err;
     hipLaunchKernelGGL((tree_merge_kernel<D>), dim3((unsigned)(chunks * a.num_seqs)), dim3(256), 0, stream, a, (int)chunks);

@@ -388,7 +388,7 @@ BVLLM_API int bvllm_paged_tree_attention(const void* q, int64_t q_stride_t, int6
  * its last node. In every layer the K/V rows at positions context_lens[s] + path[s][i]
  * then move to context_lens[s] + i. A sequence without rows gets 0 and -1.
  * k_caches and v_caches are host arrays of num_layers device pointers, read during the
- * call; all layers share the strides and num_blocks. Rows outside the table or the pool are
+ * call; all layers share the strides and num_blocks, and no cache is named twice. Rows outside the table or the pool are
  * not moved. max_path at most 4096.
  */
 BVLLM_API int bvllm_commit_draft_tree(void* const* k_caches, void* const* v_caches, int32_t num_layers,
@@ -405,7 +405,7 @@ BVLLM_API int bvllm_commit_draft_tree(void* const* k_caches, void* const* v_cach
  * scores[b] + logits[b][v] - logsumexp(logits[b]) over the num_beams rows of each group and
  * the vocabulary, in descending order, equal ones by b * vocab + v. logits
  * [num_groups * num_beams, vocab] bf16 (logits_fp32 = 0) or fp32 (1) with unit column
- * stride, scores fp32. Totals are formed and compared in fp64. out_scores fp32, out_beams
+ * stride and any row stride (0: one row for all), scores fp32. Totals are formed and compared in fp64. out_scores fp32, out_beams
  * (within the group) and out_tokens int64, each [num_groups, num_candidates]. A beam whose
  * score is not finite, or whose logits hold a NaN, a +inf or no finite value, gives totals
  * of -inf. num_beams at most 32, num_candidates at most 64 and num_beams * vocab,

@@ -187,6 +187,42 @@ def test_strided_rows_and_scores_of_any_shape():
     assert all(torch.equal(a, b) for a, b in zip(beam_select(x, many[:, 0], 3, 6), want))
 
 
+@pytest.mark.parametrize("k,vocab,n", [(32, 524288, 64), (32, 524288, 9), (1, 3_000_001, 2), (1, 64, 64)])
+def test_largest_and_smallest_sets_of_pieces(k, vocab, n):
+    x, s = inputs(k, vocab, torch.float32 if vocab % 2 else torch.bfloat16, seed=n)
+    x = x.float() + torch.rand_like(x, dtype=torch.float32) * 2 ** -9  # no ties
+    totals = (s[:, None].double() + torch.log_softmax(x.double(), -1)).view(-1)
+    want = totals.topk(n)
+    got = beam_select(x, s, k, n)
+    flat = got[1][0] * vocab + got[2][0]
+    # (Equal fp32 logits are few among 16 million, but there: their order is by index.)
+    assert torch.equal(totals[flat], want.values) and len(set(flat.tolist())) == n
+    # Masked but for three tokens of every other beam: those, then the first masked ones.
+    keep = torch.zeros_like(x, dtype=torch.bool)
+    keep[::2, [3, vocab // 2, vocab - 1]] = True
+    x[~keep] = -float("inf")
+    x[1::2] = -float("inf")
+    got = beam_select(x, s, k, n)
+    flat = (got[1][0] * vocab + got[2][0]).tolist()
+    live = min(n, 3 * ((k + 1) // 2))
+    totals = torch.where(keep, s[:, None].double() + torch.log_softmax(x.double(), -1), -float("inf")).view(-1)
+    order = totals.topk(live)
+    assert torch.equal(totals[flat[:live]], order.values)
+    rest = [i for i in range(min(n + 3, vocab)) if not keep.view(-1)[i]][:n - live]
+    assert flat[live:] == rest and torch.isinf(got[0][0, live:]).all()
+
+
+def test_one_row_for_all_beams(monkeypatch):
+    # A search's first step: the prompt's logits for every beam, one of them live.
+    x, s = inputs(4, 5000)
+    s[1:] = -float("inf")
+    want = check(x[:1].expand(4, -1), s, 4)
+    for got in (beam_select(x[:1].repeat(4, 1), s, 4), beam_select(x[:1].expand(4, -1), s, 4, 8)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    python_path(monkeypatch)
+    assert all(torch.equal(a, b) for a, b in zip(beam_select(x[:1].expand(4, -1), s, 4), want))
+
+
 def test_defaults_the_python_path_and_no_rows(monkeypatch):
     x, s = inputs(6, 4000)
     want = beam_select(x, s, 3, 6)
@@ -362,4 +398,5 @@ def test_reorder_refusals():
     refused(ValueError, tables=tables[:1].expand(6, -1))
     refused(ValueError, seq=seq[:5])
     refused(ValueError, caches=[caches[0], caches[1][:, :2]])
+    refused(ValueError, caches=[caches[1], caches[0], caches[1]])
     refused(RuntimeError, caches=[c[:, :, :8].contiguous() for c in caches])

@@ -93,7 +93,7 @@ def layers(*pointers):
 
 
 def commit(**k):
-    a = dict(k=layers(P, P), v=layers(P, P), n=2, sb=8192, st=512, sh=128, nb=10, hkv=4, d=128, bs=16, bt=P, bts=8, mb=8,
+    a = dict(k=layers(P, 2 * P), v=layers(P, P), n=2, sb=8192, st=512, sh=128, nb=10, hkv=4, d=128, bs=16, bt=P, bts=8, mb=8,
              qsl=P, ctx=P, draft=P, target=P, parents=P, path=P, acc=P, fol=P, s=0, mp=8, stream=None)
     assert set(k) <= set(a)
     return _lib.lib().bvllm_commit_draft_tree(*{**a, **k}.values())
@@ -101,7 +101,7 @@ def commit(**k):
 
 def test_commit_refuses_on_the_host():
     assert commit() == 0 and commit(n=0, k=None, v=None) == 0
-    bad = [dict(n=-1), dict(n=2, k=None), dict(k=layers(P, None)), dict(v=layers(P, P + 2)), dict(bs=8), dict(d=12), dict(hkv=0),
+    bad = [dict(n=-1), dict(n=2, k=None), dict(k=layers(P, None)), dict(k=layers(P, P)), dict(v=layers(P, P + 2)), dict(bs=8), dict(d=12), dict(hkv=0),
            dict(mp=0), dict(mp=4097), dict(s=-1), dict(s=65536), dict(sb=0), dict(hkv=1 << 18)]
     assert [k for k in bad if commit(**k) != BAD] == []
     bad = [dict(bt=None), dict(mb=0), dict(bts=7), dict(qsl=None), dict(ctx=None), dict(draft=None), dict(target=None),
@@ -121,7 +121,7 @@ def test_select_refuses_on_the_host():
            dict(k=32, v=524289)]
     assert [k for k in bad if select(**k) != BAD] == []
     assert select(k=32, v=524288, st=524288) == 0
-    bad = [dict(x=None), dict(scores=None), dict(ws=None), dict(os=None), dict(ob=None), dict(ot=None), dict(st=999),
+    bad = [dict(x=None), dict(scores=None), dict(ws=None), dict(os=None), dict(ob=None), dict(ot=None), dict(st=-1),
            dict(ws=P + 4), dict(x=P + 1), dict(x=P + 2, fp32=1)]
     assert [k for k in bad if select(**{"g": 1, **k}) != BAD] == []
     assert _lib.lib().bvllm_beam_workspace_bytes(8, 2049) == 8 * 2 * 8

@@ -189,6 +189,7 @@ def test_refusals():
     refused(ValueError, block_tables=md.block_tables[:0])
     refused(ValueError, caches=[caches[0], caches[1][:, :1]])
     refused(ValueError, caches=[caches[0][0]])
+    refused(ValueError, caches=caches + caches[:1])  # moved twice at once
     refused(TypeError, caches=[caches[0].float()])
     refused(RuntimeError, caches=[caches[0].cpu()])
     refused(RuntimeError, draft=draft.cpu())
