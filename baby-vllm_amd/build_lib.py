@@ -45,7 +45,6 @@ FLAGS = [
 # Per-file additions: paged_decode_pair.hip keeps its MFMA accumulators in
 # VGPRs (see the file's header for the measurements).
 FILE_FLAGS = {
-    "tree_attn.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "paged_decode_pair.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

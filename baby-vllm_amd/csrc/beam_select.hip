@@ -9,12 +9,12 @@
 // per group: the rows' lse from the pieces; then a bar that n pieces' maxima reach, so that a
 // token has to reach it too. Only pieces that do are read again, some more than n of them, and
 // few tokens in them compete: each counts the better ones. It is bound by its chain of loads
-// and barriers (1 group of 4 beams, 8 candidates: 7.7 us; 16 groups of 8, 16 candidates: 12.6).
+// and barriers (1 group of 4 beams, 8 candidates: 7.3 us; 16 groups of 8, 16 candidates: 11.9).
 // Choosing the n best of each piece in stage 1 instead took 24.4 us there, most of it in
 // counting that no later choice needed.
 //
 // Masked vocabularies, whose bar is -inf, and other crowds of equal totals take the exact
-// choice (the same two sizes with 20 tokens of a row left: 39 and 48 us in all, against 12 and 21).
+// choice (the same two sizes with 20 tokens of a row left: 40 and 49 us in all, against 11.5 and 20).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -396,21 +396,32 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   const int share_lanes = min(64, (a.vocab + Piece<T>::VEC - 1) / Piece<T>::VEC);  // that hold a token of some piece
   for (int b = w; b < K; b += kPickWaves) {
     const float score = a.scores[row0 + b];
-    float m = kNegInf;
-    for (int i = lane; i < pieces; i += 64) m = fmax_prop(m, stats[b * pieces + i].x);
+    // (Up to 256 pieces are read once: 4 beams of 75 pieces 0.3 us less.)
+    constexpr int kHeld = 4;
+    float2 held[kHeld];
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q)
+      held[q] = lane + 64 * q < pieces ? stats[b * pieces + lane + 64 * q] : make_float2(kNegInf, 0.f);
+    float m = fmax_prop(fmax_prop(held[0].x, held[1].x), fmax_prop(held[2].x, held[3].x));
+    for (int i = lane + 64 * kHeld; i < pieces; i += 64) m = fmax_prop(m, stats[b * pieces + i].x);
     m = wave_max(m);
     double sum = 0.0;
-    for (int i = lane; i < pieces; i += 64) {
-      const float2 x = stats[b * pieces + i];
+    auto add = [&](float2 x) __attribute__((always_inline)) {
       if (x.x != kNegInf) sum += (double)(x.y * fast_exp2((x.x - m) * kLog2e));
-    }
+    };
+#pragma unroll
+    for (int q = 0; q < kHeld; ++q) add(held[q]);
+    for (int i = lane + 64 * kHeld; i < pieces; i += 64) add(stats[b * pieces + i]);
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d, 64);
     const bool live = fabsf(m) < __builtin_huge_valf() && fabsf(score) < __builtin_huge_valf();
     const double base = live ? (double)score - ((double)m + log(sum)) : kNegInf64;
     if (lane == 0) sh.base[b] = base;
     if (!shares) {
-      for (int i = lane; i < pieces; i += 64)
+#pragma unroll
+      for (int q = 0; q < kHeld; ++q)
+        if (lane + 64 * q < pieces) sh.keys[b * pieces + lane + 64 * q] = order_of(total_of_logit(base, held[q].x));
+      for (int i = lane + 64 * kHeld; i < pieces; i += 64)
         sh.keys[b * pieces + i] = order_of(total_of_logit(base, stats[b * pieces + i].x));
     } else {
       for (int piece = 0; piece < pieces; ++piece) {
