@@ -112,8 +112,8 @@ constexpr int kDecodeDepth = 1;
 // CTX: the context part of a draft tree step (tree_attn.hip): every row sees every key of the
 // whole 64-key tiles below its sequence's context length, so nothing is masked and no tile is
 // partial. A sequence's tiles are cut evenly into ranges of at most a.split_tiles, each a
-// work-group that always writes its partial. The last n_dec_wgs work-groups take the keys behind
-// them, with masks (tree_columns).
+// work-group that always writes its partial. The work-groups behind them take the other keys,
+// with masks (tree_columns).
 template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
                                                                   int xcd_group, int per_xcd,
@@ -142,26 +142,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // otherwise fills each CU's memory queue in front of them (mixed step
   // 1 x 512 + 63 decodes: 34.6 -> 29.5 us).
   const int n_pre_wgs = (int)gridDim.x - n_dec_wgs;
-  if constexpr (CTX) {
-    // The last n_dec_wgs work-groups take the keys behind the whole tiles, a wave 16 columns; those
-    // of one (sequence, KV head) follow each other on one XCD.
-    static_assert(NW * 4 * kTreeStep * D <= sizeof(lds), "the waves' V buffers");
+  if constexpr (!CTX) {
     if ((int)blockIdx.x >= n_pre_wgs) {
-      const int t = (int)blockIdx.x - n_pre_wgs;
-      const int groups = (dec.max_query_len * (dec.num_heads / dec.num_kv_heads) + 16 * NW - 1) / (16 * NW);
-      const int pair = (t >> 3) / groups * 8 + (t & 7), s = pair / dec.num_kv_heads;
-      if (pair < dec.num_seqs * dec.num_kv_heads)
-        tree_columns<D, 1, 1, true>(dec, lds + wave_id() * 4 * kTreeStep * D, 0, s, pair - s * dec.num_kv_heads,
-                                    ((t >> 3) % groups * NW + wave_id()) * 16, 0);
+      const int dw = (int)blockIdx.x - n_pre_wgs;
+      if (dec.chunk_target > 0)  // uneven rows: cut into chunks (RowChunk)
+        decode_work_group<D, kDecodeWaves, kDecodeDepth, true, true>(dec, dw, reinterpret_cast<float*>(lds));
+      else if (dw < dec.batch * dec.num_kv_heads * col_groups_per_kv(dec.num_heads / dec.num_kv_heads))
+        decode_work_group<D, kDecodeWaves, kDecodeDepth, true>(dec, dw, reinterpret_cast<float*>(lds));
       return;
     }
-  } else if ((int)blockIdx.x >= n_pre_wgs) {
-    const int dw = (int)blockIdx.x - n_pre_wgs;
-    if (dec.chunk_target > 0)  // uneven rows: cut into chunks (RowChunk)
-      decode_work_group<D, kDecodeWaves, kDecodeDepth, true, true>(dec, dw, reinterpret_cast<float*>(lds));
-    else if (dw < dec.batch * dec.num_kv_heads * col_groups_per_kv(dec.num_heads / dec.num_kv_heads))
-      decode_work_group<D, kDecodeWaves, kDecodeDepth, true>(dec, dw, reinterpret_cast<float*>(lds));
-    return;
   }
 
   const int G = a.num_heads / a.num_kv_heads;
@@ -179,12 +168,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // boustrophedon order (0 1 | 1 0 | 0 1 ...): each L2 holds one KV head's
   // keys, and the heavy-to-light run of a sequence's blocks spreads evenly.
   // SPL: the ranges of a block are `bpw` whole grids apart, on the block's XCD.
-  // CTX (dense numbering, per_xcd = (sequence, KV head) pairs per XCD): the blocks of one (pair,
-  // range) follow each other on one XCD, and the ranges of a pair go to one XCD after
-  // another, so that a long sequence loads all of them (contiguous pairs per XCD: the step of
-  // 16 sequences of 1000 to 8000 had one XCD with 2.3 times the average's tiles).
+  // CTX: ContextUnit (tree_attn.h).
   const int grid_wgs = SPL ? n_pre_wgs / bpw : n_pre_wgs;
-  const int range = CTX ? ((int)blockIdx.x >> 3) / (dense_qb * per_xcd) : SPL ? (int)blockIdx.x / grid_wgs : 0;
+  int range = SPL && !CTX ? (int)blockIdx.x / grid_wgs : 0;
   const int id = SPL && !CTX ? (int)blockIdx.x - range * grid_wgs : (int)blockIdx.x;
   int tile0 = SPL && !CTX ? range * a.split_tiles : 0;  // first key tile of the range
   int max_blocks = SPL ? a.max_blocks - 4 * tile0 : a.max_blocks;  // > 0: ranges start inside the table
@@ -193,13 +179,25 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   asm volatile("" ::"s"(a.block_tables), "s"(a.bt_stride), "s"(a.max_blocks), "s"(a.query_start_loc),
                "s"(a.seq_lens), "s"(a.context_lens), "s"(a.q), "s"(a.q_st), "s"(a.q_sh), "s"(a.k_cache),
                "s"(a.v_cache), "s"(a.c_st), "s"(a.c_sh), "s"(a.c_sb), "s"(a.num_pages));
-  int kvh, r;
+  int kvh, r, s, qb;
+  int ctx_tiles = 0;  // CTX: tiles of the range
+  int ctx_meta[4];    // CTX: the sequence's metadata
   if constexpr (CTX) {
-    const int at = (id >> 3) - range * (dense_qb * per_xcd);
-    const int pair = at / dense_qb * 8 + (((id & 7) - range) & 7);
-    if (pair >= a.num_seqs * a.num_kv_heads) return;
-    kvh = pair % a.num_kv_heads;
-    r = pair / a.num_kv_heads * dense_qb + at % dense_qb;
+    static_assert(NW * 4 * kTreeStep * D <= sizeof(lds), "the waves' V buffers");
+    int j = id >> 3;
+    const ContextUnit u(dec, CB, id & 7, j);
+    if (u.seq < 0) {
+      const TailUnit t(dec, 16 * NW, id & 7, j);
+      if (t.seq >= 0)
+        tree_columns<D, 1, 1, true>(dec, lds + wave_id() * 4 * kTreeStep * D, 0, t.seq, t.kv_head,
+                                    (t.group * NW + wave_id()) * 16, 0);
+      return;
+    }
+    s = u.seq; kvh = u.kv_head; qb = u.block; range = u.range;
+    tile0 = u.first_tile;
+    ctx_tiles = u.tiles;
+    max_blocks = a.max_blocks - 4 * tile0;
+    ctx_meta[0] = u.q_start; ctx_meta[1] = u.q_end; ctx_meta[2] = u.seq_len; ctx_meta[3] = u.ctx;
   } else if (xcd_group < 0) {
     const int L = (id & 7) * per_xcd + (id >> 3);
     if (L >= n_blocks_bound * a.num_kv_heads) return;
@@ -216,14 +214,15 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
     kvh = id % a.num_kv_heads;
     r = id / a.num_kv_heads;
   }
-  if (r >= n_blocks_bound) return;
-  int s, qb;
-  if (dense_qb > 0) {
-    // Dense numbering: every sequence owns dense_qb block numbers.
-    s = r / dense_qb;
-    qb = dense_qb - 1 - (r - s * dense_qb);
-  } else if (!find_query_block(a, CB * (MB ? bpw : 1), r, s, qb)) {
-    return;
+  if constexpr (!CTX) {
+    if (r >= n_blocks_bound) return;
+    if (dense_qb > 0) {
+      // Dense numbering: every sequence owns dense_qb block numbers.
+      s = r / dense_qb;
+      qb = dense_qb - 1 - (r - s * dense_qb);
+    } else if (!find_query_block(a, CB * (MB ? bpw : 1), r, s, qb)) {
+      return;
+    }
   }
 
   // The sequence's metadata and the page numbers of its first two 64-key
@@ -234,21 +233,12 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // entries (entries past the row's last are clamped to it: only the last
   // tiles reach there); page_finish waits for them and forms byte offsets.
   typedef const int32_t __attribute__((address_space(4)))* ConstI32;
-  int q_start = ((ConstI32)a.query_start_loc)[s];
-  int q_end = ((ConstI32)a.query_start_loc)[s + 1];
-  int seq_len = ((ConstI32)a.seq_lens)[s];
-  int ctx = ((ConstI32)a.context_lens)[s];
+  int q_start = CTX ? ctx_meta[0] : ((ConstI32)a.query_start_loc)[s];
+  int q_end = CTX ? ctx_meta[1] : ((ConstI32)a.query_start_loc)[s + 1];
+  int seq_len = CTX ? ctx_meta[2] : ((ConstI32)a.seq_lens)[s];
+  int ctx = CTX ? ctx_meta[3] : ((ConstI32)a.context_lens)[s];
   constexpr int PAGES_PER_TILE = KT / 16;
   static_assert(PAGES_PER_TILE == 4, "page_finish consumes four entries");
-  int ctx_tiles = 0;  // CTX: tiles of the range
-  if constexpr (CTX) {
-    const int tiles = context_tiles(ctx, seq_len, a.max_blocks);
-    const ContextRanges ranges(tiles, a.split_tiles, a.num_ranges);
-    if (range >= ranges.count) return;
-    tile0 = range * ranges.per;
-    ctx_tiles = min(ranges.per, tiles - tile0);
-    max_blocks = a.max_blocks - 4 * tile0;
-  }
   const ConstI32 bts = (ConstI32)(a.block_tables + (int64_t)s * a.bt_stride + (SPL ? 4 * tile0 : 0));
   const uint32_t page_bytes = (uint32_t)a.c_sb * 2u;  // c_sb < 2^31, checked on the host
   // (No branch between the fast and the clamped form: the waits that close
@@ -1121,14 +1111,17 @@ int32_t prefill_split_tiles(const PrefillArgs& a, int64_t key_tiles, int64_t lon
 template <int D, int QT, int KS>
 static hipError_t launch_context(const PrefillArgs& a, const TreeArgs& tree, hipStream_t stream) {
   constexpr int CB = 4 / KS * QT * 16;
-  const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);
-  const int64_t blocks = (cols + CB - 1) / CB;
-  const int64_t per_xcd = ((int64_t)a.num_seqs * a.num_kv_heads + 7) / 8;
-  const int64_t wgs = 8 * per_xcd * blocks * a.num_ranges, tails = 8 * per_xcd * ((cols + 63) / 64);
-  if (wgs + tails > 0x7ffffff0 || blocks * a.num_seqs > 0x7ffffff0) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, true, true>), dim3((unsigned)(wgs + tails)), dim3(4 * 64),
-                     0, stream, a, (int)(blocks * a.num_seqs), (int)blocks, 0, (int)per_xcd, tree, (int)tails,
-                     a.num_ranges);
+  // Work-groups per XCD that suffice: of the blocks of all sequences, each XCD has at most the
+  // eighth, rounded up, of the (range, KV head) pairs; of the tails the eighth of the KV heads.
+  const int64_t group = a.num_heads / a.num_kv_heads, cols = a.max_query_len * group;
+  auto blocks = [&](int64_t width) {
+    return std::min((cols + width - 1) / width * a.num_seqs, a.num_tokens * group / width + a.num_seqs);
+  };
+  const int64_t per_xcd = blocks(CB) * (((int64_t)a.num_ranges * a.num_kv_heads + 7) / 8) +
+                          blocks(64) * ((a.num_kv_heads + 7) / 8);
+  if (8 * per_xcd > 0x7ffffff0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, true, true>), dim3((unsigned)(8 * per_xcd)), dim3(4 * 64),
+                     0, stream, a, 0, 0, 0, 0, tree, 0, 1);
   return hipGetLastError();
 }
 

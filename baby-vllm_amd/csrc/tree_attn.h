@@ -24,6 +24,99 @@ struct ContextRanges {
   }
 };
 
+// Wave-wide: exclusive prefix sum, and the sum in `all`. Within the rows of 16 lanes, then the last
+// lane of a row into the next, and of the first two rows into the others (ds_permutes instead took the
+// first launch of a tree behind 32,000 0.4 us more).
+__device__ __forceinline__ int row_prefix(int mine, int& all) {
+  int upto = mine;
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, false);
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+  upto += __builtin_amdgcn_update_dpp(0, upto, 0x143, 0xc, 0xf, false);
+  all = __builtin_amdgcn_readlane(upto, 63);
+  return upto - mine;
+}
+
+// Numbers below n that are x modulo 8.
+__device__ __forceinline__ int congruent_below(int n, int x) { return (n + 7 - x) >> 3; }
+
+// What the slot-th work-group of an XCD takes of the context. Teams are the work-groups of one
+// (sequence, range, KV head), one per block of columns: numbered in that order, team t runs on
+// XCD t mod 8, so that its blocks read their keys from one L2 and every sequence loads all XCDs.
+// Only work there is has a number: the grid is larger, and work-groups without any, between the
+// others, would hold them up, since each takes its LDS and two round trips before it ends (35
+// sequences of 500 to 5000 with up to 64 tokens, 416 work-groups with work among 2304: 94 us, now
+// NOW35). seq < 0: the slot lies behind them, and slot is its number there. Sequences are looked at
+// 64 at a time, a lane each.
+struct ContextUnit {
+  int seq = -1, kv_head, block, range, first_tile, tiles;
+  int q_start, q_end, seq_len, ctx;
+  __device__ __forceinline__ ContextUnit(const TreeArgs& a, int width, int xcd, int& slot) {
+    const int group = a.num_heads / a.num_kv_heads;
+    int teams = 0;
+    for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+      const int i = min(s0 + lane_id(), a.num_seqs - 1);
+      const int q0 = a.query_start_loc[i], q1 = a.query_start_loc[i + 1];
+      const int c = a.context_lens[i], len = a.seq_lens[i];
+      const int n_blocks = s0 + lane_id() < a.num_seqs ? max(0, ((q1 - q0) * group + width - 1) / width) : 0;
+      const int all_tiles = context_tiles(c, len, a.max_blocks);
+      const ContextRanges ranges(all_tiles, a.split_tiles, a.num_ranges);
+      const int t = n_blocks > 0 && all_tiles > 0 ? ranges.count * a.num_kv_heads : 0;
+      int all, all_slots;
+      const int before = teams + row_prefix(t, all);
+      const int slots = (congruent_below(before + t, xcd) - congruent_below(before, xcd)) * n_blocks;
+      const int first = row_prefix(slots, all_slots);
+      if (slot < all_slots) {
+        const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(slot >= first && slot < first + slots));
+        seq = s0 + l;
+        const int b = __builtin_amdgcn_readlane(n_blocks, l), at = slot - __builtin_amdgcn_readlane(first, l);
+        const int team0 = __builtin_amdgcn_readlane(before, l), k = at / b;
+        block = at - k * b;
+        const int in_seq = ((xcd - team0) & 7) + 8 * k;
+        range = in_seq / a.num_kv_heads;
+        kv_head = in_seq - range * a.num_kv_heads;
+        first_tile = range * __builtin_amdgcn_readlane(ranges.per, l);
+        tiles = min(__builtin_amdgcn_readlane(ranges.per, l), __builtin_amdgcn_readlane(all_tiles, l) - first_tile);
+        q_start = __builtin_amdgcn_readlane(q0, l);
+        q_end = __builtin_amdgcn_readlane(q1, l);
+        seq_len = __builtin_amdgcn_readlane(len, l);
+        ctx = __builtin_amdgcn_readlane(c, l);
+        return;
+      }
+      slot -= all_slots;
+      teams += all;
+    }
+  }
+};
+
+// The same for the tails, behind them: teams are the work-groups of one (sequence, KV head), each of
+// `width` columns.
+struct TailUnit {
+  int seq = -1, kv_head, group;
+  __device__ __forceinline__ TailUnit(const TreeArgs& a, int width, int xcd, int& slot) {
+    for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+      const int i = min(s0 + lane_id(), a.num_seqs - 1);
+      const int cols = (a.query_start_loc[i + 1] - a.query_start_loc[i]) * (a.num_heads / a.num_kv_heads);
+      const int groups = s0 + lane_id() < a.num_seqs ? max(0, (cols + width - 1) / width) : 0;
+      const int before = i * a.num_kv_heads;
+      const int slots = (congruent_below(before + a.num_kv_heads, xcd) - congruent_below(before, xcd)) * groups;
+      int all_slots;
+      const int first = row_prefix(slots, all_slots);
+      if (slot < all_slots) {
+        const int l = (int)__builtin_ctzll(__builtin_amdgcn_ballot_w64(slot >= first && slot < first + slots));
+        seq = s0 + l;
+        const int g = __builtin_amdgcn_readlane(groups, l), at = slot - __builtin_amdgcn_readlane(first, l), k = at / g;
+        group = at - k * g;
+        kv_head = ((xcd - seq * a.num_kv_heads) & 7) + 8 * k;
+        return;
+      }
+      slot -= all_slots;
+    }
+  }
+};
+
 // Keys that a sequence's rows can see at all: written ones (seq_len), up to its last
 // drafted token, inside its table.
 __device__ __forceinline__ int tree_keys(int seq_len, int ctx, int q_len, int max_blocks) {
