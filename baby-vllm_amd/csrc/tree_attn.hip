@@ -186,22 +186,21 @@ constexpr int64_t kMaxTreeBytes = 64ll << 20;
 
 // Whether the context runs in ranges, their length and their blocks (negative: of 64 columns). Times in
 // us as measured here, 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
-//   one launch: 4.3 + 1.8 (1.15 at D = 64) per 32-key step of a wave on the longest row, but at
+//   one launch: 4.3 + 1.7 (1.15 at D = 64) per 32-key step of a wave on the longest row, but at
 //     least 2.4 per thousand steps of all waves;
-//   two: 8.7 (10.3 at D = 64) + 0.4 per tile of a range in blocks of 64 columns (0.57 with more
-//     than one work-group per CU), 0.9 and 1.6 of 128, + 0.17 per range of the longest row, less
-//     where waves are few, + 7.7 per thousand 16-column tiles, the tail's.
+//   two: 8.7 (10.3 at D = 64) + 0.38 per tile of a range in blocks of 64 columns (0.53 with more
+//     than one work-group per CU), 1.0 and 2.5 of 128, + 0.17 per range of the longest row, less
+//     where waves are few, + 7.8 per thousand 16-column tiles, the tail's.
 // Blocks of 64 columns, whose waves share a tile's keys, walk a tile in half the time where
-// work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 34.4 us, with 128
-// columns 38.9; 8 trees of 11 to 45: 29.3 and 32.6); they read the keys twice as often, which
-// counts once there are more than 18.7 128-column tiles per CU (57 at D = 64): 21 trees of 5 to 18
-// behind 4858: 71 and 61.
-// The range is as short as about 1.5 work-groups per CU allow (sequences end ranges early: half
-// of one each), and not so short that adding partials outweighs the walk (a root of the longest
-// row's tiles). Where that is more than 20 tiles, and more than a 6th or 15th of the longest row,
-// it is cut shorter: long ranges leave CUs idle behind the last ones (26 sequences of 2100 to
+// work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 32.7 us, with 128
+// columns 37.0); they read the keys twice as often, which counts once there are more than 21
+// 128-column tiles per CU (56 at D = 64): 26 trees of up to 53 behind 2100 to 6400 take 73.8 and 64.5.
+// The range is as short as 1.63 work-groups per CU allow (1.8 of 128 columns; sequences end ranges
+// early: half of one each), and not so short that adding partials outweighs the walk (a root of the
+// longest row's tiles). Where that is more than 16 tiles (20), and more than a 14th (6th) of the longest
+// row, it is cut shorter: long ranges leave CUs idle behind the last ones (26 sequences of 2100 to
 // 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random steps the choice
-// was 2.7% above the best of one launch and up to 22 ranges of either block on average, 35%
+// was 1.9% above the best of one launch and up to 22 ranges of either block on average, 14%
 // at most.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
   const bool d64 = a.head_dim == 64;
@@ -213,23 +212,23 @@ int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_t
       (double)(kMaxTreeBytes / (prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4) - 1);
   if (max_ranges < 1 || longest < 2) return 0;
   const double cus = device_cus();
-  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 57 : 18.7) * cus;
+  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 56 : 21) * cus;
   const int64_t cb = narrow ? 64 : 128;
   const double blocks = (double)((cols + cb - 1) / cb * a.num_kv_heads);
-  const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.45 : 1.7) * cus;
+  const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.63 : 1.8) * cus;
   const double rounds = 1.0 + std::floor(units / target);
-  double range = std::max(work / (rounds * target - units / 2), std::sqrt((narrow ? 0.43 : 0.16) * longest));
+  double range = std::max(work / (rounds * target - units / 2), std::sqrt((narrow ? 0.43 : 0.19) * longest));
   range = std::max(range, narrow ? 4.0 : 3.0);
-  range = std::min(range, narrow ? std::max(20.0, longest / 15) : std::max(23.0, longest / 6.3));
+  range = std::min(range, narrow ? std::max(16.0, longest / 14) : std::max(20.0, longest / 6.3));
   range = std::min({std::ceil(std::max(range, longest / max_ranges)), longest, (double)(1 << 20)});
 
   const double waves = (double)waves_per_column_tile(a), key_waves = waves >= 8 ? waves / 2 : waves;
   const double col_tiles = (double)((cols + 15) / 16) * a.num_kv_heads;
-  const double one = 4.3 + std::max((d64 ? 1.15 : 1.8) * std::ceil(2 * longest / key_waves),
+  const double one = 4.3 + std::max((d64 ? 1.15 : 1.7) * std::ceil(2 * longest / key_waves),
                                     1.2 * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
-  const double wgs = work / range + units / 2, alone = narrow ? 0.39 : 0.9, shared = narrow ? 0.57 : 1.6;
+  const double wgs = work / range + units / 2, alone = narrow ? 0.38 : 1.0, shared = narrow ? 0.53 : 2.5;
   const double two = (d64 ? 10.3 : 8.7) + (wgs < cus ? alone : shared) * range * std::max(1.0, wgs / (2 * cus)) +
-                     0.17 * longest / range * (16 / waves) + 7.7 * a.num_seqs * col_tiles / 1000;
+                     0.17 * longest / range * (16 / waves) + 7.8 * a.num_seqs * col_tiles / 1000;
   return one <= two ? 0 : narrow ? -(int32_t)range : (int32_t)range;
 }
 
