@@ -18,7 +18,7 @@
 //
 // What bounds it: 48 chains of 2 to 7 tokens behind 200 to 4000 read 125 MB of keys in 35 us
 // (3.6 TB/s) and 4 more on the second launch; 16 trees of 64 behind 1000 to 8000 multiply at 0.6
-// PFLOP/s in 82 us (their 448 columns fill 3.5 of 4 blocks, and ranges are uneven); a few trees
+// PFLOP/s in 80 us (their 448 columns fill 3.5 of 4 blocks, and ranges are uneven); a few trees
 // are bound by the chain of a range's round trips and tiles, and by the second launch (4.4 us).
 //
 // The walk with masks (tree_attn.h, tree_columns): a column is one of the sequence's (drafted token,
