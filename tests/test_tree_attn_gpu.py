@@ -176,7 +176,7 @@ def raw_call(q, cache, md, scale, split, ranges):
     return out
 
 
-@pytest.mark.parametrize("heads", [(2, 7, 128), (2, 7, 64), (1, 3, 128), (1, 2, 64)], ids=str)
+@pytest.mark.parametrize("heads", [(2, 7, 128), (2, 7, 64), (1, 3, 128), (1, 2, 64), (3, 2, 64), (12, 5, 128)], ids=str)
 @pytest.mark.parametrize("split", [0, 1, 2, 3, 5, 12, 1000, -1, -2, -3, -5, -12, -1000])
 def test_context_ranges_of_any_length(heads, split):
     # Contexts of no whole tile, of one, of several; blocks of 64 and of 128 columns.
@@ -189,7 +189,7 @@ def test_context_ranges_of_any_length(heads, split):
 
 
 @pytest.mark.parametrize("heads", [(2, 7, 128), (4, 7, 64)], ids=str)
-@pytest.mark.parametrize("seqs", [1, 3, 9, 20, 60])
+@pytest.mark.parametrize("seqs", [1, 3, 9, 20, 60, 64, 65, 140])
 def test_every_number_of_waves_per_column(seqs, heads):
     rng = random.Random(seqs)
     specs = [(rng.choice([0, 5, 64, 100, 200]), random_tree(rng, rng.choice([1, 9, 30]))) for _ in range(seqs - 1)]
