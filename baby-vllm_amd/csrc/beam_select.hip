@@ -9,12 +9,12 @@
 // per group: the rows' lse from the pieces; then a bar that n pieces' maxima reach, so that a
 // token has to reach it too. Only pieces that do are read again, some more than n of them, and
 // few tokens in them compete: each counts the better ones. It is bound by its chain of loads
-// and barriers (1 group of 4 beams, 8 candidates: 7.3 us; 16 groups of 8, 16 candidates: 11.9).
+// and barriers (1 group of 4 beams, 8 candidates: 7.1 us; 16 groups of 8, 16 candidates: 10.2).
 // Choosing the n best of each piece in stage 1 instead took 24.4 us there, most of it in
 // counting that no later choice needed.
 //
 // Masked vocabularies, whose bar is -inf, and other crowds of equal totals take the exact
-// choice (the same two sizes with 20 tokens of a row left: 40 and 49 us in all, against 11.5 and 20).
+// choice (the same two sizes with 20 tokens of a row left: 40 and 49 us in all, against 11 and 19).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -443,7 +443,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   // pieces: lane l takes the best of pieces l, l + 64, ...; the bar is the n-th best of those
   // 64 (1 group of 4 beams, 8 candidates: 1.0 us less than with the sets). Else, with more
   // candidates to tell apart, 128 sets of all the work-group's threads (4 groups of 32 beams over
-  // 50,257 tokens, 64 candidates, in all: 34 us; with the bar of 64 lanes 49).
+  // 50,257 tokens, 64 candidates, in all: 32 us; with the bar of 64 lanes 15 more).
   uint64_t bar = 0;
   if (!shares && n <= 24 && M >= 4 * n) {
     uint64_t best = 0;
@@ -506,26 +506,33 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
       for (int q = 0; q < 32; ++q)
         if (Piece<T>::column(q) >= columns) p.v[q] = __builtin_nanf("");
     }
-    int all = 0;
+    // Few do: only groups of 8 elements whose maximum reaches it are looked into (4 groups of 32
+    // beams, 83 pieces, element by element: 2.7 us more).
+    bool full = false;
 #pragma unroll
-    for (int q = 0; q < 32; ++q) all += __popcll(__builtin_amdgcn_ballot_w64(p.v[q] >= threshold));
-    int at = 0;
-    if (lane == 0) at = atomicAdd(&sh.count, all);
-    at = uniform(at);
-    if (at + all > kMaxCand) continue;  // (the count tells everybody)
+    for (int h = 0; h < 32; h += 8) {
+      float top = p.v[h];
 #pragma unroll
-    for (int q = 0; q < 32; ++q) {
-      const uint64_t hit = __builtin_amdgcn_ballot_w64(p.v[q] >= threshold);
-      if (hit != 0) {
-        if ((hit >> lane) & 1) {
-          const int slot = at + __popcll(hit & ((1ull << lane) - 1));
-          const uint64_t k = order_of(total_of_logit(base, p.v[q]));
-          sh.cand_key[slot] = k >= bar ? k : 0;  // (just below the bar: no candidate)
-          sh.cand[slot] = (uint32_t)(b * a.vocab + piece * kPiece + Piece<T>::column(q));
+      for (int q = 1; q < 8; ++q) top = __builtin_fmaxf(top, p.v[h + q]);  // (of a NaN: the other)
+      if (full || __builtin_amdgcn_ballot_w64(top >= threshold) == 0) continue;
+#pragma unroll
+      for (int q = h; q < h + 8; ++q) {
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(p.v[q] >= threshold);
+        if (hit == 0 || full) continue;
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&sh.count, (int)__popcll(hit));
+        at = uniform(at);
+        full = at + (int)__popcll(hit) > kMaxCand;  // (the count tells everybody)
+        if (!full && ((hit >> lane) & 1)) {
+          int l = lane;
+          asm volatile("" : "+v"(l));  // (formed here, not for all 32 elements ahead)
+          const int slot = at + __popcll(hit & ((1ull << l) - 1));
+          sh.cand_key[slot] = (uint64_t)b << 32 | __float_as_uint(p.v[q]);
+          sh.cand[slot] = (uint32_t)(b * a.vocab + piece * kPiece + (q / Piece<T>::VEC * 64 + l) * Piece<T>::VEC + q % Piece<T>::VEC);
         }
-        at += __popcll(hit);
       }
     }
+    if (full) break;
   }
   __syncthreads();
   if (too_many || sh.count > kMaxCand) {
@@ -533,6 +540,13 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     if (tid == 0) sh.count = 0;
     __syncthreads();
     pick_exact<T>(a, pieces, sh);
+  } else {
+    for (int c = tid; c < sh.count; c += kPickThreads) {
+      const uint64_t x = sh.cand_key[c];
+      const uint64_t k = order_of(total_of_logit(sh.base[x >> 32], __uint_as_float((uint32_t)x)));
+      sh.cand_key[c] = k >= bar ? k : 0;  // (just below the bar: no candidate)
+    }
+    __syncthreads();
   }
 
   // The n best candidates by key, equal ones by index.
