@@ -32,7 +32,7 @@
 // form the operand.
 //   S^T[32 keys x 16 cols] = K Q^T,  O^T[D/DS x 16 cols] += V^T P^T   (mfma 16x16x32)
 // A walk of a few steps is a chain of round trips (metadata, table, keys, states), so waves
-// are spent until the card is full (tree_for_dim): one tree of 8 behind 300 takes 5.3 us on 8 waves
+// are spent until the card is full (tree_shape): one tree of 8 behind 300 takes 5.1 us on 16 waves
 // per 16 columns.
 // Sums, maxima and outputs are fp32 up to the final rounding. P is rounded to bf16 for its
 // MFMA, and the row sum adds the rounded values, so a weight's rounding error (at most 2^-8)
@@ -146,11 +146,24 @@ hipError_t launch_context_part(const TreeArgs& a, hipStream_t stream) {
   return paged_prefill_context(p, a, stream);
 }
 
-// Waves (slices times key waves) that each 16-column tile gets: what fills the card at two
-// waves per SIMD.
-int64_t waves_per_column_tile(const TreeArgs& a) {
+// Slices and key waves of a 16-column tile on the launch over all keys, by the waves that each could
+// have at two per SIMD of the whole card. Measured, us, 9 tokens a tree (7 / 2 heads of 64 and 28 / 4
+// of 128), n trees behind c:
+//   D = 128, 64 to 21 waves (2 to 6 trees, c = 600): <2,8> 10.3-10.6, <2,4> 10.3-10.5, <1,4> 11.1-11.3
+//   14 to 9 (9, 14 trees): <2,4> 16.3, 17.3, <1,4> 12.0, 13.1, <1,2> 13.4, 15.4
+//   6.4 to 4.3 (20, 30): <1,4> 19.9, 20.5, <1,2> 18.4, 19.0, <1,1> 23.9, 24.9
+//   2.7, 0.7 (48 of 9, 36, c = 250): <1,2> 15.5, 46.3, <1,1> 17.2, 44.4
+//   D = 64, 128 (c = 600): <2,8> 7.0, <2,4> 7.2, <1,4> 7.6; 5.3 (48 trees): <1,4> 11.1, <1,2> 11.9
+struct TreeShape {
+  int slices, key_waves;
+};
+TreeShape tree_shape(const TreeArgs& a) {
   const int64_t tiles = ((int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads) + 15) / 16;
-  return std::min<int64_t>(16, std::max<int64_t>(1, 8 * (int64_t)device_cus() / (a.num_seqs * tiles * a.num_kv_heads)));
+  const int64_t waves = 8 * (int64_t)device_cus() / (a.num_seqs * tiles * a.num_kv_heads);
+  const bool d64 = a.head_dim == 64;
+  if (waves >= 16) return {2, d64 ? 8 : 4};
+  if (waves >= (d64 ? 4 : 8)) return {1, 4};
+  return {1, waves >= 2 ? 2 : 1};
 }
 
 template <int D>
@@ -163,11 +176,10 @@ hipError_t tree_for_dim(const TreeArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((tree_merge_kernel<D>), dim3((unsigned)(chunks * a.num_seqs)), dim3(256), 0, stream, a, (int)chunks);
     return hipGetLastError();
   }
-  const int64_t waves = waves_per_column_tile(a);
-  if (waves >= 16) return launch_tree<D, 2, 8>(a, stream);
-  if (waves >= 8) return launch_tree<D, 2, 4>(a, stream);
-  if (waves >= 4) return launch_tree<D, 1, 4>(a, stream);
-  if (waves >= 2) return launch_tree<D, 1, 2>(a, stream);
+  const TreeShape shape = tree_shape(a);
+  if (shape.slices == 2) return launch_tree<D, 2, D == 64 ? 8 : 4>(a, stream);
+  if (shape.key_waves == 4) return launch_tree<D, 1, 4>(a, stream);
+  if (shape.key_waves == 2) return launch_tree<D, 1, 2>(a, stream);
   return launch_tree<D, 1, 1>(a, stream);
 }
 
@@ -186,21 +198,21 @@ constexpr int64_t kMaxTreeBytes = 64ll << 20;
 
 // Whether the context runs in ranges, their length and their blocks (negative: of 64 columns). Times in
 // us as measured here, 1 to 48 sequences of up to 32 thousand tokens and 160 drafted ones:
-//   one launch: 4.3 + 1.7 (1.15 at D = 64) per 32-key step of a wave on the longest row, but at
-//     least 2.4 per thousand steps of all waves;
-//   two: 8.7 (10.3 at D = 64) + 0.38 per tile of a range in blocks of 64 columns (0.53 with more
-//     than one work-group per CU), 1.0 and 2.5 of 128, + 0.17 per range of the longest row, less
-//     where waves are few, + 7.8 per thousand 16-column tiles, the tail's.
+//   one launch: 4.3 + 1.35 per 32-key step of a wave on the longest row, but at least 2.3 per
+//     thousand steps of all waves;
+//   two: 10.7 (11.8 at D = 64) + 0.4 per tile of a range in blocks of 64 columns (0.69 with more
+//     than one work-group per CU), 0.7 and 1.9 of 128, + 0.17 per range of the longest row, + 7.1
+//     per thousand 16-column tiles, the tail's.
 // Blocks of 64 columns, whose waves share a tile's keys, walk a tile in half the time where
 // work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 32.7 us, with 128
-// columns 37.0); they read the keys twice as often, which counts once there are more than 21
+// columns 37.0); they read the keys twice as often, which counts once there are more than 20
 // 128-column tiles per CU (56 at D = 64): 26 trees of up to 53 behind 2100 to 6400 take 73.8 and 64.5.
 // The range is as short as 1.63 work-groups per CU allow (1.8 of 128 columns; sequences end ranges
 // early: half of one each), and not so short that adding partials outweighs the walk (a root of the
-// longest row's tiles). Where that is more than 16 tiles (20), and more than a 14th (6th) of the longest
+// longest row's tiles). Where that is more than 16 tiles (20), and more than a 10th (6th) of the longest
 // row, it is cut shorter: long ranges leave CUs idle behind the last ones (26 sequences of 2100 to
 // 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random steps the choice
-// was 1.9% above the best of one launch and up to 22 ranges of either block on average, 14%
+// was 2.0% above the best of one launch and up to 22 ranges of either block on average, 15%
 // at most.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
   const bool d64 = a.head_dim == 64;
@@ -212,23 +224,23 @@ int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_t
       (double)(kMaxTreeBytes / (prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4) - 1);
   if (max_ranges < 1 || longest < 2) return 0;
   const double cus = device_cus();
-  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 56 : 21) * cus;
+  const bool narrow = cols <= 64 || total * (double)((cols + 127) / 128 * a.num_kv_heads) <= (d64 ? 56 : 20) * cus;
   const int64_t cb = narrow ? 64 : 128;
   const double blocks = (double)((cols + cb - 1) / cb * a.num_kv_heads);
   const double work = total * blocks, units = a.num_seqs * blocks, target = (narrow ? 1.63 : 1.8) * cus;
   const double rounds = 1.0 + std::floor(units / target);
-  double range = std::max(work / (rounds * target - units / 2), std::sqrt((narrow ? 0.43 : 0.19) * longest));
+  double range = std::max(work / (rounds * target - units / 2), std::sqrt((narrow ? 0.43 : 0.26) * longest));
   range = std::max(range, narrow ? 4.0 : 3.0);
-  range = std::min(range, narrow ? std::max(16.0, longest / 14) : std::max(20.0, longest / 6.3));
+  range = std::min(range, narrow ? std::max(16.0, longest / 10) : std::max(20.0, longest / 6.4));
   range = std::min({std::ceil(std::max(range, longest / max_ranges)), longest, (double)(1 << 20)});
 
-  const double waves = (double)waves_per_column_tile(a), key_waves = waves >= 8 ? waves / 2 : waves;
+  const TreeShape shape = tree_shape(a);
   const double col_tiles = (double)((cols + 15) / 16) * a.num_kv_heads;
-  const double one = 4.3 + std::max((d64 ? 1.15 : 1.7) * std::ceil(2 * longest / key_waves),
-                                    1.2 * col_tiles * (waves >= 8 ? 2 : 1) * 2 * total / 1000);
-  const double wgs = work / range + units / 2, alone = narrow ? 0.38 : 1.0, shared = narrow ? 0.53 : 2.5;
-  const double two = (d64 ? 10.3 : 8.7) + (wgs < cus ? alone : shared) * range * std::max(1.0, wgs / (2 * cus)) +
-                     0.17 * longest / range * (16 / waves) + 7.8 * a.num_seqs * col_tiles / 1000;
+  const double one = 4.3 + std::max(1.35 * std::ceil(2 * longest / shape.key_waves),
+                                    1.13 * col_tiles * shape.slices * 2 * total / 1000);
+  const double wgs = work / range + units / 2, alone = narrow ? 0.4 : 0.7, shared = narrow ? 0.69 : 1.9;
+  const double two = (d64 ? 11.8 : 10.7) + (wgs < cus ? alone : shared) * range * std::max(1.0, wgs / (2 * cus)) +
+                     0.17 * longest / range + 7.1 * a.num_seqs * col_tiles / 1000;
   return one <= two ? 0 : narrow ? -(int32_t)range : (int32_t)range;
 }
 
