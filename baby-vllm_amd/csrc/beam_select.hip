@@ -9,12 +9,12 @@
 // per group: the rows' lse from the pieces; then a bar that n pieces' maxima reach, so that a
 // token has to reach it too. Only pieces that do are read again, some more than n of them, and
 // few tokens in them compete: each counts the better ones. It is bound by its chain of loads
-// and barriers (1 group of 4 beams, 8 candidates: 7.1 us; 16 groups of 8, 16 candidates: 10.2).
+// and barriers (1 group of 4 beams, 8 candidates: 6.8 us; 16 groups of 8, 16 candidates: 9).
 // Choosing the n best of each piece in stage 1 instead took 24.4 us there, most of it in
 // counting that no later choice needed.
 //
 // Masked vocabularies, whose bar is -inf, and other crowds of equal totals take the exact
-// choice (the same two sizes with 20 tokens of a row left: 40 and 49 us in all, against 11 and 19).
+// choice (the same two sizes with 20 tokens of a row left: 37 and 48 us in all, against 10.6 and 18.6).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -44,10 +44,10 @@ typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 struct Piece {
   static constexpr int VEC = 16 / sizeof(T), LOADS = 32 / VEC;
-  u32x4_any raw[LOADS];
   float v[32];
   static __device__ __forceinline__ int column(int e) { return ((e / VEC) * 64 + lane_id()) * VEC + e % VEC; }
-  __device__ __forceinline__ void request(const T* x, int left) {
+  __device__ __forceinline__ void load(const T* x, int left) {
+    u32x4_any raw[LOADS];
 #pragma unroll
     for (int k = 0; k < LOADS; ++k) {
       const int c = column(k * VEC);
@@ -65,8 +65,6 @@ struct Piece {
         for (int j = 0; j < 4; ++j) raw[k][j] = c + j < left ? __float_as_uint(x[c + j]) : 0xff800000u;
       }
     }
-  }
-  __device__ __forceinline__ void unpack() {
 #pragma unroll
     for (int e = 0; e < 32; ++e) {
       const uint32_t w = raw[e / VEC][sizeof(T) == 2 ? (e % VEC) / 2 : e % VEC];
@@ -98,9 +96,8 @@ __global__ __launch_bounds__(64 * kScanWaves) void beam_scan_kernel(BeamSelectAr
   const int piece = ((int)blockIdx.x - row * groups_per_row) * kScanWaves + wave_id();
   if (piece >= pieces) return;
   Piece<T> p;
-  p.request(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride + (int64_t)piece * kPiece,
-            a.vocab - piece * kPiece);
-  p.unpack();
+  p.load(reinterpret_cast<const T*>(a.logits) + (int64_t)row * a.row_stride + (int64_t)piece * kPiece,
+         a.vocab - piece * kPiece);
   float mx[16];
 #pragma unroll
   for (int e = 0; e < 16; ++e) mx[e] = fmax_prop(p.v[e], p.v[e + 16]);
@@ -228,16 +225,22 @@ __device__ __forceinline__ void best_items(PickShared& sh, int n_items, int n, K
     __syncthreads();
     m = sh.n_near;
   }
-  for (int e = tid; e < m; e += kPickThreads) {
+  // Eight lanes per item count the better ones among an eighth of them each (107 items: 6.4 us
+  // with one).
+  for (int e = tid >> 3; e < m; e += kPickThreads / 8) {
     const int i = all ? e : sh.near[e];
     const uint64_t k = key(i);
     const uint32_t x = index(i);
     int rank = 0;
-    for (int f = 0; f < m; ++f) {
+#pragma unroll 2
+    for (int f = tid & 7; f < m; f += 8) {
       const int o = all ? f : sh.near[f];
       rank += ahead(key(o), index(o), k, x);
     }
-    if (rank < n && k != 0) sh.best[rank] = (uint16_t)i;
+    rank += (int)dpp<kQuadSwap1>((uint32_t)rank);
+    rank += (int)dpp<kQuadSwap2>((uint32_t)rank);
+    rank += (int)dpp<kRowHalfMirror>((uint32_t)rank);
+    if ((tid & 7) == 0 && rank < n && k != 0) sh.best[rank] = (uint16_t)i;
   }
   __syncthreads();
 }
@@ -247,24 +250,14 @@ __device__ __forceinline__ double total_of_logit(double base, float x) {
   return base == kNegInf64 ? kNegInf64 : (double)x + base;
 }
 
-template <typename T>
-__device__ __forceinline__ void request_piece(const BeamSelectArgs& a, int64_t row, int piece, Piece<T>& p) {
-  p.request(reinterpret_cast<const T*>(a.logits) + row * a.row_stride + (int64_t)piece * kPiece, a.vocab - piece * kPiece);
-}
 // A beam without a distribution holds nothing but -inf.
 template <typename T>
-__device__ __forceinline__ void unpack_piece(bool live, Piece<T>& p) {
-  p.unpack();
+__device__ __forceinline__ void load_piece(const BeamSelectArgs& a, int64_t row, int piece, bool live, Piece<T>& p) {
+  p.load(reinterpret_cast<const T*>(a.logits) + row * a.row_stride + (int64_t)piece * kPiece, a.vocab - piece * kPiece);
   if (!live) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) p.v[i] = kNegInf;
   }
-}
-
-template <typename T>
-__device__ __forceinline__ void load_piece(const BeamSelectArgs& a, int64_t row, int piece, bool live, Piece<T>& p) {
-  request_piece(a, row, piece, p);
-  unpack_piece(live, p);
 }
 
 // Wave-wide: exclusive prefix sum, and the sum in `all`.
@@ -315,11 +308,13 @@ __device__ __forceinline__ uint32_t best_of_piece(const Piece<T>& p, double base
     for (int i = 0; i < 32; ++i)
       if (((open >> i) & 1) && order_of(p.v[i]) >= nth) least = min(least, order_of(p.v[i]));
     least = wave_reduce(least, [](uint32_t x, uint32_t y) { return min(x, y); });
+    double again = base;
+    asm volatile("" : "+v"(again));  // (the totals are formed again, not kept in registers meanwhile)
     const uint64_t own = order_of(total_of_logit(base, __uint_as_float(least >> 31 ? least & ~(1u << 31) : ~least)));
     over = even = 0;
 #pragma unroll
     for (int i = 0; i < 32; ++i) {
-      const uint64_t k = order_of(total_of_logit(base, p.v[i]));
+      const uint64_t k = order_of(total_of_logit(again, p.v[i]));
       over |= (uint32_t)(((open >> i) & 1) && k > own) << i;
       even |= (uint32_t)(((open >> i) & 1) && k == own) << i;
     }
@@ -443,7 +438,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   // pieces: lane l takes the best of pieces l, l + 64, ...; the bar is the n-th best of those
   // 64 (1 group of 4 beams, 8 candidates: 1.0 us less than with the sets). Else, with more
   // candidates to tell apart, 128 sets of all the work-group's threads (4 groups of 32 beams over
-  // 50,257 tokens, 64 candidates, in all: 32 us; with the bar of 64 lanes 15 more).
+  // 50,257 tokens, 64 candidates, in all: 27 us; with the bar of 64 lanes 15 more).
   uint64_t bar = 0;
   if (!shares && n <= 24 && M >= 4 * n) {
     uint64_t best = 0;
@@ -480,23 +475,14 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   // (Far more pieces than candidates: equal maxima at the bar, and not worth reading.)
   const bool too_many = n_reach > 4 * n + 64;
   // Their tokens that reach it are candidates: a conservative fp32 threshold sorts out nearly
-  // all others. A wave's next piece is on its way while it looks at one.
+  // all others. (A wave's next piece on its way meanwhile took registers that spilled: 1 group of
+  // 23 fp32 beams, 46 candidates 31.4 us in all, now 20.6; 16 groups of 8 bf16 beams 19.9 and 18.6.)
   const double bar_total = bar == 0 ? kNegInf64 : total_of(bar);
-  Piece<T> p, next;
-  int i = 0, i_next = 0;
-  auto request_next = [&](int e) __attribute__((always_inline)) {
-    i_next = uniform((int)sh.near[e]);
-    const int b = i_next / pieces;
-    request_piece(a, row0 + b, i_next - b * pieces, next);
-  };
-  if (!too_many && w < n_reach) request_next(w);
   for (int e = w; e < n_reach && !too_many; e += kPickWaves) {
-    p = next;
-    i = i_next;
-    if (e + kPickWaves < n_reach) request_next(e + kPickWaves);
-    const int b = i / pieces, piece = i - b * pieces, columns = a.vocab - piece * kPiece;
+    const int i = uniform((int)sh.near[e]), b = i / pieces, piece = i - b * pieces, columns = a.vocab - piece * kPiece;
     const double base = sh.base[b];
-    unpack_piece(base != kNegInf64, p);
+    Piece<T> p;
+    load_piece(a, row0 + b, piece, base != kNegInf64, p);
     const float at_bar = base == kNegInf64 ? kNegInf : (float)(bar_total - base);
     // (The second term: scores so large that a total's own rounding hides logits.)
     const float threshold =
