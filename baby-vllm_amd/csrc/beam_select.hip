@@ -13,8 +13,9 @@
 // Choosing the n best of each piece in stage 1 instead took 24.4 us there, most of it in
 // counting that no later choice needed.
 //
-// Masked vocabularies, whose bar is -inf, and other crowds of equal totals take the exact
-// choice (the same two sizes with 20 tokens of a row left: 37 and 48 us in all, against 10.6 and 18.6).
+// Crowds of equal totals, of masks that leave fewer tokens than candidates among them, take the
+// exact choice (the same two sizes with one token of a row left: 20 and 32 us in all, with 20
+// tokens 12 and 20, with all 10.6 and 18.5).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
@@ -461,6 +462,9 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     near_best(sh, shares ? share_lanes * M : M, n, [&](int i) { return sh.keys[i]; }, [&](int i) { return (uint32_t)i; });
     bar = sh.bar_key;
   }
+  // Totals of -inf (masked tokens) are no candidates: where fewer than n others are found, the
+  // exact choice is taken.
+  bar = max(bar, order_of(kNegInf64) + 1);
 
   // The pieces that reach it (all, if the bar comes from shares), dealt to the waves.
   if (tid == 0) sh.n_near = 0;
@@ -477,21 +481,17 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   // Their tokens that reach it are candidates: a conservative fp32 threshold sorts out nearly
   // all others. (A wave's next piece on its way meanwhile took registers that spilled: 1 group of
   // 23 fp32 beams, 46 candidates 31.4 us in all, now 20.6; 16 groups of 8 bf16 beams 19.9 and 18.6.)
-  const double bar_total = bar == 0 ? kNegInf64 : total_of(bar);
+  const double bar_total = total_of(bar);
   for (int e = w; e < n_reach && !too_many; e += kPickWaves) {
-    const int i = uniform((int)sh.near[e]), b = i / pieces, piece = i - b * pieces, columns = a.vocab - piece * kPiece;
+    const int i = uniform((int)sh.near[e]), b = i / pieces, piece = i - b * pieces;
     const double base = sh.base[b];
     Piece<T> p;
     load_piece(a, row0 + b, piece, base != kNegInf64, p);
     const float at_bar = base == kNegInf64 ? kNegInf : (float)(bar_total - base);
     // (The second term: scores so large that a total's own rounding hides logits.)
-    const float threshold =
+    float threshold =
         at_bar - fabsf(at_bar) * 0x1p-22f - (base == kNegInf64 ? 0.f : (float)(fabs(base) * 0x1p-51)) - 0x1p-126f;
-    if (threshold == kNegInf && columns < kPiece) {  // columns behind the row's end, which read as -inf, are none
-#pragma unroll
-      for (int q = 0; q < 32; ++q)
-        if (Piece<T>::column(q) >= columns) p.v[q] = __builtin_nanf("");
-    }
+    if (!(threshold >= -3.402823466e38f)) threshold = at_bar > 0.f ? at_bar : -3.402823466e38f;  // (nothing; all but -inf)
     // Few do: only groups of 8 elements whose maximum reaches it are looked into (4 groups of 32
     // beams, 83 pieces, element by element: 2.7 us more).
     bool full = false;
@@ -499,7 +499,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     for (int h = 0; h < 32; h += 8) {
       float top = p.v[h];
 #pragma unroll
-      for (int q = 1; q < 8; ++q) top = __builtin_fmaxf(top, p.v[h + q]);  // (of a NaN: the other)
+      for (int q = 1; q < 8; ++q) top = fmaxf(top, p.v[h + q]);
       if (full || __builtin_amdgcn_ballot_w64(top >= threshold) == 0) continue;
 #pragma unroll
       for (int q = h; q < h + 8; ++q) {
@@ -521,7 +521,7 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     if (full) break;
   }
   __syncthreads();
-  if (too_many || sh.count > kMaxCand) {
+  if (too_many || sh.count > kMaxCand || sh.count < n) {
     __syncthreads();
     if (tid == 0) sh.count = 0;
     __syncthreads();

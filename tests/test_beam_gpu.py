@@ -111,6 +111,21 @@ def test_masked_vocabularies_and_beams_without_a_distribution():
     assert (check(x, s, 5, 10)[1] == 0).all()
 
 
+@pytest.mark.parametrize("fill", [-float("inf"), torch.finfo(torch.bfloat16).min], ids=str)
+@pytest.mark.parametrize("k,n,vocab,kept", [(4, 8, 151936, 20), (4, 8, 151936, 2), (4, 8, 151936, 1), (1, 64, 40000, 64),
+                                            (1, 64, 40000, 63), (8, 9, 1000, 2), (3, 64, 70, 30)])
+def test_masks_that_leave_more_or_fewer_tokens_than_candidates(k, n, vocab, kept, fill):
+    x, s = inputs(2 * k, vocab, torch.float32, seed=kept)
+    mask = torch.ones(2 * k, vocab, dtype=torch.bool, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(vocab)
+    for row in mask:
+        row[torch.randperm(vocab, device="cuda", generator=g)[:kept]] = False
+    x.masked_fill_(mask, fill)
+    s[1::2] += 40.0  # other beams far ahead: their masked tokens' totals beat nothing
+    check(x, s, k, n)
+    check(x.bfloat16(), s, k, n)
+
+
 def test_extreme_values():
     x, s = inputs(4, 5000, torch.float32, spread=1.0)
     x[0] *= 1e4
