@@ -330,10 +330,9 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
   float m;
   f32x4_t acc[VD], lsum;
   const uint4 ones_bf16 = make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u);
-  // The walk. A V row that is not finite (a drafted token's that a row does not see) would
-  // reach every row, as its P of 0 times it: if some accumulator is not finite at the end, the
-  // walk is repeated with such rows taken out of the products, and they are added where they
-  // are seen.
+  // The walk. A drafted token's V row that is not finite would reach the rows that do not see
+  // it too, as their P of 0 times it: if some accumulator is not finite at the end, the walk is
+  // repeated with such rows taken out of the products, and they are added where they are seen.
   for (bool careful = false;; careful = true) {
     if (first < last) request(page0, page1, 0);
     m = kNegInf;
@@ -369,7 +368,9 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
         // the product).
         if (keys - k0 < 32) odd = ~0u << (keys - k0);
         if (careful) {
-          const uint32_t found = odd_rows_of<DV>(V) & ~odd;
+          // Of drafted keys only: the context's are seen by every row and stay in the product.
+          const uint32_t drafted = ctx - k0 < 32 ? ~0u << max(0, ctx - k0) : 0;
+          const uint32_t found = odd_rows_of<DV>(V) & drafted & ~odd;
           any_odd |= found != 0;
           odd |= found;
         }
