@@ -1,4 +1,5 @@
-"""Attention of drafted token trees on the GPU: values that are not finite in keys that every row sees.
+"""Attention of drafted token trees on the GPU: values that are not finite in keys that every row sees, and
+trees, contexts and numbers of ranges up to the largest.
 
 The formula and its bounds are those of ``test_tree_attn_gpu``: an infinity or NaN in one dimension of a
 visible key's V reaches that dimension of every row, and no other; in its K, the scores of its head.
@@ -98,3 +99,27 @@ def test_context_keys_that_are_not_finite(heads):
         for name, got in calls(q, cache, md):
             print(value, name, flush=True)
             check(got, want)
+
+
+@pytest.mark.parametrize("heads", [(1, 2, 64), (1, 2, 128)], ids=str)
+def test_trees_of_160_nodes(heads):
+    rng = random.Random(160)
+    q, cache, md = build([(c, random_tree(rng, n, b)) for c, n, b in ((0, 160, 4), (333, 160, 16), (90, 131, 1))], *heads)
+    want = formula(q, cache, md, 0.1)
+    for name, got in calls(q, cache, md):
+        print(name, flush=True)
+        check(got, want)
+
+
+@pytest.mark.parametrize("heads", [(1, 3, 64), (1, 7, 128)], ids=str)
+def test_a_context_of_32_thousand(heads):
+    q, cache, md = build([(32011, random_tree(random.Random(32), 6))], *heads)
+    check(paged_tree_attention(q, cache, md, 0.1), formula(q, cache, md, 0.1))
+
+
+@pytest.mark.parametrize("split", [1, -1])
+def test_every_number_of_ranges(split):
+    q, cache, md = build([(1400, random_tree(random.Random(2), 12)), (640, [-1, 0])], 1, 7, 64)
+    want = formula(q, cache, md, 0.1)
+    for ranges in range(1, -(-md.block_tables.shape[1] // 4) + 1):
+        check(raw_call(q, cache, md, 0.1, split, ranges), want)
