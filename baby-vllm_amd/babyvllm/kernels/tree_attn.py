@@ -12,9 +12,10 @@ rotary positions) from each node's parent.
 A row that sees no key gives zeros, and a key that a row does not see does not reach it,
 whatever it holds. Rows of ``q`` behind the last sequence are not computed. Long contexts
 run in key ranges chosen from the step's host lists: the last bits of a row can depend on
-the other sequences of the step, within the rounding of fp32 sums in another order. They
-take fp32 scratch (at most 64 MiB); without the memory for it the launch that needs none
-runs.
+the other sequences of the step. Scores, softmax statistics and sums are fp32. The weights of the
+context's whole 64-key tiles are rounded to bf16 in ranges, as in ``paged_prefill_attention``; all
+others, and all where the launch has no ranges, keep 16 bits. Ranges take fp32 scratch (at most
+64 MiB); without the memory for it the launch that needs none runs.
 """
 
 from __future__ import annotations

@@ -357,6 +357,7 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
       const unsigned char* const V = vbuf + buf * TB;
       const int k0 = j * kTreeStep;
       uint32_t odd = 0;  // V rows to leave out of the product
+      const uint32_t not_finite = careful ? odd_rows_of<DV>(V) : 0;
       if (k0 + kTreeStep > ctx || k0 + kTreeStep > keys) {
         const uint32_t seen = seen_window(word0, mask_row, a.mask_words, k0, ctx, keys) >> (4 * g);
 #pragma unroll
@@ -370,7 +371,7 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
         if (careful) {
           // Of drafted keys only: the context's are seen by every row and stay in the product.
           const uint32_t drafted = ctx - k0 < 32 ? ~0u << max(0, ctx - k0) : 0;
-          const uint32_t found = odd_rows_of<DV>(V) & drafted & ~odd;
+          const uint32_t found = not_finite & drafted & ~odd;
           any_odd |= found != 0;
           odd |= found;
         }
@@ -408,8 +409,14 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
       pb.y = pack_bf16x2_hw(p[0][2], p[0][3]);
       pb.z = pack_bf16x2_hw(p[1][0], p[1][1]);
       pb.w = pack_bf16x2_hw(p[1][2], p[1][3]);
+      // What the rounding left, as a second operand: P has 16 bits in the products.
+      uint4 rest;
+      rest.x = pack_bf16x2_hw(p[0][0] - lo_f32(pb.x), p[0][1] - hi_f32(pb.x));
+      rest.y = pack_bf16x2_hw(p[0][2] - lo_f32(pb.y), p[0][3] - hi_f32(pb.y));
+      rest.z = pack_bf16x2_hw(p[1][0] - lo_f32(pb.z), p[1][1] - hi_f32(pb.z));
+      rest.w = pack_bf16x2_hw(p[1][2] - lo_f32(pb.w), p[1][3] - hi_f32(pb.w));
 
-      const uint4 keep = keep_mask(odd);
+      const uint4 keep = keep_mask(odd), keep_rest = keep_mask(not_finite);
 #pragma unroll
       for (int c = 0; c < VD; ++c) {
         const uint2 lo = ld_tr16(reinterpret_cast<const uint16_t*>(V + v_off[c]));
@@ -417,8 +424,12 @@ __device__ __forceinline__ void tree_columns(const TreeArgs& a, unsigned char* l
         uint4 va = make_uint4(lo.x, lo.y, hi.x, hi.y);
         if (odd != 0) va = make_uint4(va.x & keep.x, va.y & keep.y, va.z & keep.z, va.w & keep.w);
         acc[c] = mfma_16x16x32(va, pb, acc[c]);
+        // (An infinity meets P once: the rest may be 0 or below.)
+        if (not_finite != 0) va = make_uint4(va.x & keep_rest.x, va.y & keep_rest.y, va.z & keep_rest.z, va.w & keep_rest.w);
+        acc[c] = mfma_16x16x32(va, rest, acc[c]);
       }
       lsum = mfma_16x16x32(ones_bf16, pb, lsum);
+      lsum = mfma_16x16x32(ones_bf16, rest, lsum);
     }
 
     if (careful) {

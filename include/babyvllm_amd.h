@@ -357,7 +357,8 @@ BVLLM_API int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t vo
  * from host sizes alone: key_tiles is ceil(seq_len / 64) summed over the sequences,
  * longest_tiles the largest of them, each -1 if unknown; bvllm_prefill_ranges the num_ranges
  * (of split_tiles without its sign). They steer the choice only; results agree within the
- * rounding of fp32 sums in another order.
+ * rounding of fp32 sums in another order and of the weights: scores, statistics and sums are fp32, the
+ * weights of whole tiles in ranges are rounded to bf16 (as bvllm_paged_prefill's), all others keep 16 bits.
  */
 BVLLM_API int32_t bvllm_tree_split_tiles(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_blocks,
