@@ -18,9 +18,12 @@
 // tokens 12 and 20, with all 10.6 and 18.5).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
-// of exponentials are fp32 within a piece (32 terms per lane) and fp64 across; totals are
-// formed and compared in fp64, so that two tokens of one beam keep the order of their
-// logits, and rounded once to fp32 on output.
+// of exponentials are fp32 within a piece (32 terms per lane) and fp64 across, so a row's lse is off by
+// less than 2^-17: exponents and their arguments by 2^-23 per unit of distance from the maximum, whose
+// average by weight is below ln V = 12 or so, sums of 32 and 64 terms by 38 * 2^-24 (as measured, 3e-7 at
+// most over 9600 rows of 1000 to 151,936 tokens). Totals of different beams that are closer than
+// that can come in either order. Totals are formed and compared in fp64, so that two
+// tokens of one beam keep the order of their logits, and rounded once to fp32 on output.
 //
 // A beam whose score is not finite, or whose logits hold a NaN, a +inf or no finite value,
 // has no distribution: all its totals are -inf.

@@ -406,8 +406,10 @@ BVLLM_API int bvllm_commit_draft_tree(void* const* k_caches, void* const* v_cach
  * scores[b] + logits[b][v] - logsumexp(logits[b]) over the num_beams rows of each group and
  * the vocabulary, in descending order, equal ones by b * vocab + v. logits
  * [num_groups * num_beams, vocab] bf16 (logits_fp32 = 0) or fp32 (1) with unit column
- * stride and any row stride (0: one row for all), scores fp32. Totals are formed and compared in fp64. out_scores fp32, out_beams
- * (within the group) and out_tokens int64, each [num_groups, num_candidates]. A beam whose
+ * stride and any row stride (0: one row for all), scores fp32. Totals are formed and compared in fp64 from
+ * a logsumexp of fp32 exponentials, off by less than 2^-17: tokens of one beam are in the order of their logits,
+ * beams of equal logits and scores tie, totals of different beams closer than that come in either order. out_scores
+ * fp32, out_beams (within the group) and out_tokens int64, each [num_groups, num_candidates]. A beam whose
  * score is not finite, or whose logits hold a NaN, a +inf or no finite value, gives totals
  * of -inf. num_beams at most 32, num_candidates at most 64 and num_beams * vocab,
  * num_beams * ceil(vocab / 2048) at most 8192. workspace holds
