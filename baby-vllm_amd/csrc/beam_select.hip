@@ -438,13 +438,16 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
   }
   __syncthreads();
 
-  // The bar: a total that at least n tokens reach, and few others. Few candidates among many
-  // pieces: lane l takes the best of pieces l, l + 64, ...; the bar is the n-th best of those
-  // 64 (1 group of 4 beams, 8 candidates: 1.0 us less than with the sets). Else, with more
-  // candidates to tell apart, 128 sets of all the work-group's threads (4 groups of 32 beams over
-  // 50,257 tokens, 64 candidates, in all: 27 us; with the bar of 64 lanes 15 more).
+  // The bar: a total that at least n tokens reach, and few others. Up to 24 candidates: lane l takes the best of
+  // pieces l, l + 64, ... and the bar is the n-th best of those 64. More: of 128 sets of all the
+  // work-group's threads, which leaves fewer tokens above it but takes more steps. In us, both launches, lanes
+  // and sets: 1 group of 4 beams, 300 pieces: 9.6 and 10.9 at n = 8, 11.5 and 12.9 at 24, 13.3 and 14.8 at
+  // 40, 25.6 and 19.9 at 64; 16 of 8, 600 pieces each: 15.5 and 16.6, 17.7 and 18.8, 21.9 and 20.6, 55.0 and
+  // 26.1; 4 of 32, 800 pieces: 14.7 and 15.5, 17.2 and 17.5, 20.5 and 19.9, 47.8 and 24.8; 1 of 30, 2250
+  // pieces: 15.4 and 14.9, 17.3 and 17.0, 20.6 and 19.7, 50.8 and 23.7; 8 of 2, 32 pieces: 9.7 and 11.1
+  // at n = 8, 15.7 and 18.5 at 24.
   uint64_t bar = 0;
-  if (!shares && n <= 24 && M >= 4 * n) {
+  if (!shares && n <= 24) {
     uint64_t best = 0;
     for (int i = lane; i < M; i += 64) best = max(best, sh.keys[i]);
     // Each wave compares every lane's best with a few of them.
@@ -479,8 +482,12 @@ __global__ __launch_bounds__(kPickThreads) void beam_pick_kernel(BeamSelectArgs 
     }
   __syncthreads();
   const int n_reach = sh.n_near;
-  // (Far more pieces than candidates: equal maxima at the bar, and not worth reading.)
-  const bool too_many = n_reach > 4 * n + 64;
+  // Far more pieces than candidates: equal maxima at the bar, and the exact choice reads fewer. In us,
+  // both launches, all of them read and the exact choice, 1 group of 8 beams of 75 pieces: n = 2, 40 pieces that
+  // reach it: 12.2 and 14.4, 72: 15.5 and 14.4; n = 8, 48: 13.2 and 15.2, 96: 19.0 and 15.2; n = 16, 64: 15.1
+  // and 18.1, 128: 22.6 and 18.2; n = 64, 160: 28.1 and 39.0, 320: 43.5 and 39.0. With 1 to 32 beams in 1 to 16
+  // groups the two are even at 45 to 61, 51 to 65, 75 to 91 and 248 to 274 pieces.
+  const bool too_many = n_reach > 4 * n + 32;
   // Their tokens that reach it are candidates: a conservative fp32 threshold sorts out nearly
   // all others. (A wave's next piece on its way meanwhile took registers that spilled: 1 group of
   // 23 fp32 beams, 46 candidates 31.4 us in all, now 20.6; 16 groups of 8 bf16 beams 19.9 and 18.6.)
