@@ -148,16 +148,17 @@ struct TreeArgs {
   void* out;      int64_t o_st, o_sh;      // [T, H, D]
   int32_t num_seqs, num_tokens, max_query_len;
   int32_t num_heads, num_kv_heads, head_dim;
-  // The context on launches of its own (split_tiles > 0): 64-key tiles per range, the most
+  // The context in ranges, beside the other keys (split_tiles > 0): 64-key tiles per range, the most
   // ranges a sequence has, whether its blocks have 64 columns (else 128), and the fp32 partials.
   int32_t split_tiles, num_ranges;
   bool narrow;
   FastDiv by_kv_heads, by_group, by_heads;  // by num_kv_heads, num_heads / num_kv_heads, num_heads (of the launches)
+  // Of a sequence's ranges, and the one behind its last of the other keys.
   float* part_out;                         // [num_ranges + 1, T, H, D], unnormalized
   float* part_ml;                          // [num_ranges + 1, T, H, 2]: reference (log2 units), sum
 };
 hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
-// 64-key tiles per range of the context's launch for the batch's shape, negative with blocks of
+// 64-key tiles per range of the context for the batch's shape, negative with blocks of
 // 64 columns, 0 without one (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles);
 

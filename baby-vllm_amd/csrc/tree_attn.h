@@ -47,8 +47,8 @@ __device__ __forceinline__ int congruent_below(int n, int x) { return (n + 7 - x
 // XCD t mod 8, so that its blocks read their keys from one L2 and every sequence loads all XCDs.
 // Only work there is has a number: the grid is larger, and work-groups without any, between the
 // others, would hold them up, since each takes its LDS and two round trips before it ends (35
-// sequences of 500 to 5000 with up to 64 tokens, 416 work-groups with work among 2304: 94 us, now
-// 62). seq < 0: the slot lies behind them, and slot is its number there. Sequences are looked at
+// sequences of 500 to 5000 with up to 64 tokens, 416 work-groups with work among 2304: 94 us, 62 with
+// this numbering). seq < 0: the slot lies behind them, and slot is its number there. Sequences are looked at
 // 64 at a time, a lane each.
 struct ContextUnit {
   int seq = -1, kv_head, block, range, first_tile, tiles;

@@ -13,8 +13,9 @@
 // whole 64-key tiles without a mask, in ranges (paged_prefill.hip, CTX); on the same launch waves
 // of their own take the rest, at most 63 context keys and the drafted ones, with the
 // masks (the tail); all leave fp32 partials that a second launch adds. (The tail on the second
-// launch, which then added the partials to its own walk: 16 trees of 64 tokens 109 us, now 91; 8
-// trees of 11 to 45 30 and 26.)
+// launch, which then added the partials to its own walk, took 109 us for 16 trees of 64 tokens where
+// the tail beside the ranges took 91, and 30 for 8 trees of 11 to 45 where it took 26; with what was
+// changed since these are 81 and 22.5.)
 //
 // What bounds it: 48 chains of 2 to 7 tokens behind 200 to 4000 read 125 MB of keys in 35 us
 // (3.6 TB/s) and 4 more on the second launch; 16 trees of 64 behind 1000 to 8000 multiply at 0.6
@@ -152,13 +153,17 @@ hipError_t launch_context_part(const TreeArgs& a, hipStream_t stream) {
 }
 
 // Slices and key waves of a 16-column tile on the launch over all keys, by the waves that each could
-// have at two per SIMD of the whole card. Measured, us, 9 tokens a tree (7 / 2 heads of 64 and 28 / 4
-// of 128), n trees behind c:
-//   D = 128, 64 to 21 waves (2 to 6 trees, c = 600): <2,8> 10.3-10.6, <2,4> 10.3-10.5, <1,4> 11.1-11.3
-//   14 to 9 (9, 14 trees): <2,4> 16.3, 17.3, <1,4> 12.0, 13.1, <1,2> 13.4, 15.4
-//   6.4 to 4.3 (20, 30): <1,4> 19.9, 20.5, <1,2> 18.4, 19.0, <1,1> 23.9, 24.9
-//   2.7, 0.7 (48 of 9, 36, c = 250): <1,2> 15.5, 46.3, <1,1> 17.2, 44.4
-//   D = 64, 128 (c = 600): <2,8> 7.0, <2,4> 7.2, <1,4> 7.6; 5.3 (48 trees): <1,4> 11.1, <1,2> 11.9
+// have at two per SIMD of the whole card. Measured, us, n tokens a tree (7 / 2 heads of 64 and 28 / 4
+// of 128), trees behind c; beside the chosen form those next to it:
+//   D = 128, n = 9, c = 600: 64 waves (2 trees): <2,4> 10.6, <1,4> 11.7; 16 (8): 11.0, 12.0; 14 (9): 16.3, <1,4> 11.9,
+//     <1,2> 15.4; 9 (14): <1,4> 12.4, <1,2> 15.7; 6.4 (20): 20.0, <1,2> 19.8, <1,1> 26.3; 4.3 (30): 21.1, 20.9, 27.1; 3.2
+//     (40): 26.8, 26.7, 28.9
+//   c = 250: 9 (14): <1,4> 9.3, <1,2> 10.1; 3.6 (36): 18.3, 15.3, <1,1> 15.7; n = 20, c = 300: 2.8 (20): 18.2, 15.7, 16.9;
+//     2.4 (24): 21.7, 19.2, 18.0; 1.9 (30): 25.6, 24.1, 21.9
+//   D = 64, n = 9, c = 600: 256 (1): <2,8> 7.4, <1,4> 8.2; 16 (16): 7.8, 8.7; 15 (17): 10.6, 8.7, <1,2> 11.4; 4.0 (64):
+//     <1,4> 11.7, <1,2> 14.5; 3.6 (72): 15.8, 15.3, <1,1> 18.7; 2.0 (128): 20.1, 18.5, 20.7
+//   n = 20, c = 300: 5.7 (20): <1,4> 8.5, <1,2> 9.2; 3.8 (30): 10.4, 9.7, <1,1> 11.2; 2.0 (56): 12.4, 11.5, 12.0;
+//     1.8 (64): <1,2> 14.4, <1,1> 13.9; 1.2 (96): 17.5, 15.6
 struct TreeShape {
   int slices, key_waves;
 };
@@ -209,16 +214,17 @@ constexpr int64_t kMaxTreeBytes = 64ll << 20;
 //     than one work-group per CU), 0.7 and 1.9 of 128, + 0.17 per range of the longest row, + 7.1
 //     per thousand 16-column tiles, the tail's.
 // Blocks of 64 columns, whose waves share a tile's keys, walk a tile in half the time where
-// work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000: 32.7 us, with 128
-// columns 37.0); they read the keys twice as often, which counts once there are more than 20
-// 128-column tiles per CU (56 at D = 64): 26 trees of up to 53 behind 2100 to 6400 take 73.8 and 64.5.
+// work-groups are few and leave fewer columns empty (a tree of 25 behind 32,000, ranges of 16 tiles: 34.8 us, with
+// 128 columns 37.3); they read the keys twice as often, which counts once there are more than 20
+// 128-column tiles per CU (56 at D = 64): 26 trees of up to 53 behind 2100 to 6400 take 59.0 in ranges of 16, 53.9
+// with 128 columns in ranges of 20.
 // The range is as short as 1.63 work-groups per CU allow (1.8 of 128 columns; sequences end ranges
 // early: half of one each), and not so short that adding partials outweighs the walk (a root of the
 // longest row's tiles). Where that is more than 16 tiles (20), and more than a 10th (6th) of the longest
-// row, it is cut shorter: long ranges leave CUs idle behind the last ones (26 sequences of 2100 to
-// 6400 with up to 53 tokens: 118 us at 84 tiles, 69 at 28). Over 200 random steps the choice
-// was 2.0% above the best of one launch and up to 22 ranges of either block on average, 15%
-// at most.
+// row, it is cut shorter: long ranges leave CUs idle behind the last ones (the same 26: 100.9 us at
+// 84 tiles, 53.9 at 20). Over 200 random steps the choice was 2.0% above the best of one launch and up to
+// 22 ranges of either block on average, 15% at most; over 30 of 64 to 200 sequences, which it was not
+// fitted to, 2.7% and 15%.
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles) {
   const bool d64 = a.head_dim == 64;
   const int64_t cols = (int64_t)a.max_query_len * (a.num_heads / a.num_kv_heads);

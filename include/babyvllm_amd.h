@@ -348,12 +348,12 @@ BVLLM_API int bvllm_embed_rows(const int64_t* ids, const void* table, int64_t vo
  * row with no visible key outputs zeros; keys that a row does not see do not reach it,
  * whatever they hold. mask_words must be at least max_query_len / 64 rounded up; scale
  * must be positive and finite.
- * split_tiles > 0 gives the whole 64-key tiles below every context length to a launch of its
- * own, cut into at most num_ranges ranges a sequence, of split_tiles tiles where that
- * suffices, whose fp32 partials in workspace (bvllm_tree_workspace_bytes(num_tokens,
- * num_heads, head_dim, num_ranges) bytes) a second launch adds to the other keys. < 0: the
- * same with ranges of -split_tiles tiles and narrower blocks (64 columns instead of 128). 0: one
- * launch over all keys, no workspace. bvllm_tree_split_tiles returns the split_tiles to use
+ * split_tiles > 0 cuts the whole 64-key tiles below every context length into at most
+ * num_ranges ranges a sequence, of split_tiles tiles where that suffices. One launch takes the
+ * ranges and, beside them, every sequence's other keys, each of which leaves an fp32 partial in
+ * workspace (bvllm_tree_workspace_bytes(num_tokens, num_heads, head_dim, num_ranges) bytes:
+ * num_ranges + 1 partials); a second adds them up. < 0: the same with ranges of -split_tiles tiles
+ * and narrower blocks (64 columns instead of 128). 0: one launch over all keys, no workspace. bvllm_tree_split_tiles returns the split_tiles to use
  * from host sizes alone: key_tiles is ceil(seq_len / 64) summed over the sequences,
  * longest_tiles the largest of them, each -1 if unknown; bvllm_prefill_ranges the num_ranges
  * (of split_tiles without its sign). They steer the choice only; results agree within the
