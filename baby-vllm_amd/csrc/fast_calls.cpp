@@ -533,10 +533,13 @@ PyObject* fast_tree(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// The layers' caches of a list: their pointers, written to, and one of them. False: not plain ones of one shape and layout.
+// The layers' caches of a list: their pointers, written to, and what they have in common. False: not plain ones of
+// one shape and layout. (The list may change once the GIL is released: nothing of it is kept, and it is not looked at
+// again after that.)
 struct Layers {
   std::vector<void*> k, v;
-  const at::Tensor* one = nullptr;
+  int64_t stride_page, stride_token, stride_head;
+  int32_t pages, heads, dim;
 };
 bool plain_layers(PyObject* o, int64_t dev, Layers& l) {
   if (!PyList_CheckExact(o)) return false;
@@ -544,17 +547,26 @@ bool plain_layers(PyObject* o, int64_t dev, Layers& l) {
   if (n < 1 || n > 4096) return false;
   l.k.resize(n);
   l.v.resize(n);
+  const at::Tensor* one = nullptr;
   for (Py_ssize_t i = 0; i < n; ++i) {
     const at::Tensor* c = plain(PyList_GET_ITEM(o, i), at::kBFloat16, dev);
     if (!plain_cache(c)) return false;
-    if (i == 0) l.one = c;
-    else if (c->sizes() != l.one->sizes() || c->strides() != l.one->strides()) return false;
+    if (i == 0) one = c;
+    else if (c->sizes() != one->sizes() || c->strides() != one->strides()) return false;
     l.k[i] = ptr(*c);
     for (Py_ssize_t j = 0; j < i; ++j)
       if (l.k[j] == l.k[i]) return false;
   }
-  return l.one->size(2) == kPage && small(l.one->size(4));
+  if (one->size(2) != kPage || !small(one->size(4))) return false;
+  l.stride_page = one->stride(1);
+  l.stride_token = one->stride(2);
+  l.stride_head = one->stride(3);
+  l.pages = (int32_t)one->size(1);
+  l.heads = (int32_t)one->size(3);
+  l.dim = (int32_t)one->size(4);
+  return true;
 }
+// Once the call is certain to be made, and with the GIL held since plain_layers.
 void write_layers(PyObject* o, Layers& l) {
   for (size_t i = 0; i < l.k.size(); ++i) {
     const at::Tensor& c = THPVariable_Unpack(PyList_GET_ITEM(o, i));
@@ -596,16 +608,15 @@ PyObject* fast_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   void* stream = PyLong_AsVoidPtr(a[9]);
   if (PyErr_Occurred()) return nullptr;
   if (max_path < 1 || max_path > 4096) return none();
+  write_layers(a[0], l);
   const at::Tensor all = new_empty({seqs * (max_path + 1)}, *ctx, at::kInt);
   at::Tensor accepted = part_of(all, 0, {seqs}), path = part_of(all, seqs, {seqs, max_path}),
              following = new_empty({seqs}, *ctx, at::kLong);
-  write_layers(a[0], l);
   int rc;
   {
     pybind11::gil_scoped_release no_gil;
-    const at::Tensor& c = *l.one;
-    rc = g.commit(l.k.data(), l.v.data(), (int32_t)l.k.size(), c.stride(1), c.stride(2), c.stride(3),
-                  (int32_t)c.size(1), (int32_t)c.size(3), (int32_t)c.size(4), (int32_t)kPage,
+    rc = g.commit(l.k.data(), l.v.data(), (int32_t)l.k.size(), l.stride_page, l.stride_token, l.stride_head, l.pages,
+                  l.heads, l.dim, (int32_t)kPage,
                   bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width, qsl->const_data_ptr<int32_t>(),
                   ctx->const_data_ptr<int32_t>(), draft->const_data_ptr<int64_t>(), target->const_data_ptr<int64_t>(),
                   parents->const_data_ptr<int32_t>(), path.mutable_data_ptr<int32_t>(),
@@ -671,9 +682,8 @@ PyObject* fast_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
   int rc;
   {
     pybind11::gil_scoped_release no_gil;
-    const at::Tensor& c = *l.one;
-    rc = g.reorder(l.k.data(), l.v.data(), (int32_t)l.k.size(), c.stride(1), c.stride(2), c.stride(3),
-                   (int32_t)c.size(1), (int32_t)c.size(3), (int32_t)c.size(4), (int32_t)kPage,
+    rc = g.reorder(l.k.data(), l.v.data(), (int32_t)l.k.size(), l.stride_page, l.stride_token, l.stride_head, l.pages,
+                   l.heads, l.dim, (int32_t)kPage,
                    bt->mutable_data_ptr<int32_t>(), rows > 1 ? bt->stride(0) : width, (int32_t)width,
                    lens->const_data_ptr<int32_t>(), beams->const_data_ptr<int64_t>(), (int32_t)groups, (int32_t)k,
                    stream);
