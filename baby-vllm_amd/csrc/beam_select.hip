@@ -14,8 +14,8 @@
 // counting that no later choice needed.
 //
 // Crowds of equal totals, of masks that leave fewer tokens than candidates among them, take the
-// exact choice (the same two sizes with one token of a row left: 20 and 32 us in all, with 20
-// tokens 12 and 20, with all 10.6 and 18.5).
+// exact choice (the same two sizes with one token of a row left: 19.4 and 30.1 us in all, with 20
+// tokens 9.8 and 16.7, with all 9.1 and 16.8).
 //
 // Pieces are cut by column, whatever a row's alignment, so equal rows get equal bits. Sums
 // of exponentials are fp32 within a piece (32 terms per lane) and fp64 across, so a row's lse is off by
