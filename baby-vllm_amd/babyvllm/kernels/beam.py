@@ -84,6 +84,7 @@ def reorder_beams(kv_caches, block_tables, seq_lens, beams):
     be the beam's own page: it stays, and its ``seq_len % 16`` tokens are copied from the
     parent's page in every layer of ``kv_caches``. A parent may be named any number of times,
     and by beams that are parents themselves: everything is read before it is overwritten.
+    Nothing is copied from or to a page outside the pool.
     """
     if block_tables.is_cuda:
         if _lib.fast().reorder(kv_caches, block_tables, seq_lens, beams, MAX_BEAMS, *_lib.current()):

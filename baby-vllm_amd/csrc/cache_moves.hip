@@ -153,16 +153,18 @@ __global__ __launch_bounds__(256) void reorder_beams_kernel(ReorderArgs a, Cache
                             (int64_t)row * a.cache.stride_token * 2;
   const ConstI32 table = (ConstI32)(a.block_tables + row0 * a.bt_stride + full);
   uint4 v[KB];
+  uint32_t taken = 0;  // beams whose parent's page is one of the pool
 #pragma unroll
   for (int b = 0; b < KB; ++b)
     if (b < K) {
-      const int p = parent(b);
-      const int page = min(max(table[(int64_t)p * a.bt_stride], 0), a.cache.num_pages - 1);
+      const int p = parent(b), entry = table[(int64_t)p * a.bt_stride];
+      const int page = min(max(entry, 0), a.cache.num_pages - 1);
       if (p != b) v[b] = ld16(at + (int64_t)page * a.cache.stride_page * 2);
+      taken |= (uint32_t)(p != b && page == entry) << b;
     }
 #pragma unroll
   for (int b = 0; b < KB; ++b)
-    if (b < K && parent(b) != b) {
+    if ((taken >> b) & 1) {
       const int page = table[(int64_t)b * a.bt_stride];
       if (page >= 0 && page < a.cache.num_pages) st16(at + (int64_t)page * a.cache.stride_page * 2, v[b]);
     }

@@ -428,8 +428,8 @@ BVLLM_API int bvllm_beam_select(const void* logits, int64_t row_stride, int32_t 
  * In block_tables (int32 [num_groups * num_beams, max_blocks], in place) the entries of the
  * seq_len / 16 full pages are taken from the parent's row; the entry of the page being
  * filled, which must be the beam's own, stays, and its seq_len mod 16 tokens are copied from
- * the parent's page in every layer, all read before any is written. Layers as in
- * bvllm_commit_draft_tree. num_beams at most 32.
+ * the parent's page in every layer, all read before any is written, none where one of the two pages is
+ * not in the pool. Layers as in bvllm_commit_draft_tree. num_beams at most 32.
  */
 BVLLM_API int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches, int32_t num_layers,
                      int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
