@@ -113,9 +113,12 @@ PyObject* launch(const at::Tensor& out, const char* what, F&& call) {
   return rc == 0 ? THPVariable_Wrap(out) : failed(rc, what);
 }
 
+at::Tensor empty_beside(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType t) {
+  return at::empty(sizes, like.options().dtype(t).requires_grad(false));
+}
 at::Tensor new_empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType t) {
   pybind11::gil_scoped_release no_gil;
-  return at::empty(sizes, like.options().dtype(t).requires_grad(false));
+  return empty_beside(sizes, like, t);
 }
 
 // A part of an allocation as a tensor of its own: a call's small results of one type share one
@@ -609,12 +612,14 @@ PyObject* fast_commit(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (PyErr_Occurred()) return nullptr;
   if (max_path < 1 || max_path > 4096) return none();
   write_layers(a[0], l);
-  const at::Tensor all = new_empty({seqs * (max_path + 1)}, *ctx, at::kInt);
-  at::Tensor accepted = part_of(all, 0, {seqs}), path = part_of(all, seqs, {seqs, max_path}),
-             following = new_empty({seqs}, *ctx, at::kLong);
+  at::Tensor accepted, path, following;
   int rc;
   {
     pybind11::gil_scoped_release no_gil;
+    const at::Tensor all = empty_beside({seqs * (max_path + 1)}, *ctx, at::kInt);
+    accepted = part_of(all, 0, {seqs});
+    path = part_of(all, seqs, {seqs, max_path});
+    following = empty_beside({seqs}, *ctx, at::kLong);
     rc = g.commit(l.k.data(), l.v.data(), (int32_t)l.k.size(), l.stride_page, l.stride_token, l.stride_head, l.pages,
                   l.heads, l.dim, (int32_t)kPage,
                   bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width, qsl->const_data_ptr<int32_t>(),
@@ -645,13 +650,15 @@ PyObject* fast_beam(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rows == 0 || vocab == 0 || !small(rows) || !small(vocab) || scores->numel() != rows) return none();
   if (beams < 1 || beams > max_beams || rows % beams || cand < 1 || cand > std::min(max_cand, beams * vocab)) return none();
   const int64_t groups = rows / beams, row_stride = rows > 1 ? x->stride(0) : vocab;
-  const at::Tensor all = new_empty({groups * cand * 2}, *x, at::kLong);
-  at::Tensor b = part_of(all, 0, {groups, cand}), t = part_of(all, groups * cand, {groups, cand}),
-             s = new_empty({groups, cand}, *x, at::kFloat);
-  at::Tensor ws = new_empty({g.beam_bytes((int32_t)rows, (int32_t)vocab) / 4}, *x, at::kFloat);
+  at::Tensor s, b, t;
   int rc;
   {
     pybind11::gil_scoped_release no_gil;
+    const at::Tensor all = empty_beside({groups * cand * 2}, *x, at::kLong);
+    b = part_of(all, 0, {groups, cand});
+    t = part_of(all, groups * cand, {groups, cand});
+    s = empty_beside({groups, cand}, *x, at::kFloat);
+    const at::Tensor ws = empty_beside({g.beam_bytes((int32_t)rows, (int32_t)vocab) / 4}, *x, at::kFloat);
     rc = g.beam(ptr(*x), row_stride, fp32 ? 1 : 0, scores->const_data_ptr<float>(), (int32_t)groups, (int32_t)beams,
                 (int32_t)vocab, (int32_t)cand, ptr(ws), s.mutable_data_ptr<float>(), b.mutable_data_ptr<int64_t>(),
                 t.mutable_data_ptr<int64_t>(), stream);
