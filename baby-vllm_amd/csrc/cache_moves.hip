@@ -7,8 +7,8 @@
 // for full batches, by HBM: one thread per 16 bytes of a row, which moves that column
 // for every row that it depends on, so that reads come before the writes that would
 // overwrite them and no thread waits for another. Measured: the commit of one tree of 8 in 24
-// layers 2.3 us, of 48 trees of 20 to 64 in 28 layers 7 (8 MB out and in); beams of one request at
-// 1003 tokens 4 us, 16 groups of 8 beams 12 (67 MB read and written, 5.5 TB/s).
+// layers 2.3 us, of 48 trees of 20 to 64 in 28 layers 7 to 8 (8 MB out and in); beams of one request at
+// 1003 tokens 3.7 us, 16 groups of 8 beams 13 (67 MB read and written, 5.2 TB/s).
 #include "bvllm_device.h"
 #include "bvllm_abi_internal.h"
 

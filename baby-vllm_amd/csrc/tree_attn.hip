@@ -33,7 +33,7 @@
 // form the operand.
 //   S^T[32 keys x 16 cols] = K Q^T,  O^T[D/DS x 16 cols] += V^T P^T   (mfma 16x16x32)
 // A walk of a few steps is a chain of round trips (metadata, table, keys, states), so waves
-// are spent until the card is full (tree_shape): one tree of 8 behind 300 takes 5.1 us on 16 waves
+// are spent until the card is full (tree_shape): one tree of 8 behind 300 takes 5.3 us on 16 waves
 // per 16 columns.
 // Sums, maxima and outputs are fp32 up to the final rounding. In the walk with masks P meets its
 // MFMA as two bf16 halves, 16 bits (one tree of 8 behind 300: 5.45 us with 8 bits, 5.57 with 16, and
