@@ -27,10 +27,11 @@ def beam_select(logits, scores, num_beams: int, num_candidates: int | None = Non
     (default ``2 * K``, at most 64) best of each group, fp32 totals, int64 beam numbers within
     the group and int64 tokens, each ``[G, num_candidates]``, in descending order, equal totals
     by ``beam * vocab + token``. Totals are added up and compared in 64 bits, but a row's logsumexp
-    is a sum of 32-bit exponentials, off by less than 2^-17 (3e-7 as measured): a beam's tokens are in the order of their
-    logits, and beams of equal logits and scores have equal totals, while totals of different
-    beams that are closer than that can come in either order. A beam whose score is not finite (an
-    unused one: -inf), or whose logits hold a NaN, a +inf or no finite value, has totals of -inf.
+    is a sum of 32-bit exponentials, off by less than 2^-17 (3e-7 as measured): a beam's
+    tokens are in the order of their logits, and beams of equal logits and scores have equal
+    totals, while totals of different beams that are closer than that can come in either
+    order. A beam whose score is not finite (an unused one: -inf), or whose logits hold a NaN,
+    a +inf or no finite value, has totals of -inf.
     """
     if num_candidates is None and logits.dim() == 2:
         num_candidates = min(2 * num_beams, num_beams * logits.shape[1])

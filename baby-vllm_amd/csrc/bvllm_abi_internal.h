@@ -159,7 +159,7 @@ struct TreeArgs {
 };
 hipError_t paged_tree_attention(const TreeArgs& a, hipStream_t stream);
 // 64-key tiles per range of the context for the batch's shape, negative with blocks of
-// 64 columns, 0 without one (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
+// 64 columns, 0: no ranges (key_tiles: ceil(seq_len / 64) of all sequences, longest_tiles: of the longest; < 0 if unknown).
 int32_t tree_split_tiles(const TreeArgs& a, int64_t key_tiles, int64_t longest_tiles);
 
 // The K and V caches of several layers, all of one shape.
