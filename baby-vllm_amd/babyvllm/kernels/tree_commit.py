@@ -19,6 +19,8 @@ import torch
 
 from babyvllm.kernels import _lib
 
+MAX_PATH = 4096
+
 
 def layer_caches(kv_caches, device):
     """(layers, their pointer arrays, one of them) after checking that all have one shape and layout."""
@@ -54,10 +56,10 @@ def commit_draft_tree(kv_caches, md, draft_tokens, target_tokens, parents, max_p
     ``kv_caches`` are the layers' caches (all of one shape, each once; none: only the walk).
     ``draft_tokens`` and ``target_tokens`` int64 ``[T]`` and ``parents`` int32 ``[T]`` (node
     numbers within the sequence, before their children; -1 for the root) follow ``md.query_start_loc``.
-    ``max_path`` bounds the accepted nodes (default ``md.max_query_len``).
+    ``max_path`` bounds the accepted nodes (default ``md.max_query_len``, at most 4096).
     """
     bt, qsl, ctx = md.block_tables, md.query_start_loc, md.context_lens
-    max_path = max(1, md.max_query_len) if max_path is None else max_path
+    max_path = min(max(1, md.max_query_len), MAX_PATH) if max_path is None else max_path
     if draft_tokens.is_cuda:
         done = _lib.fast().commit(kv_caches, bt, qsl, ctx, draft_tokens, target_tokens, parents, max_path,
                                   *_lib.current())
@@ -81,8 +83,8 @@ def commit_draft_tree(kv_caches, md, draft_tokens, target_tokens, parents, max_p
     if bt.dim() != 2 or bt.stride(1) != 1 or bt.shape[0] < num_seqs:
         raise ValueError("block_tables must be [S, W] with a unit last stride")
     max_path = int(max_path)
-    if not 1 <= max_path <= 4096:
-        raise ValueError(f"max_path must be 1 to 4096, got {max_path}")
+    if not 1 <= max_path <= MAX_PATH:
+        raise ValueError(f"max_path must be 1 to {MAX_PATH}, got {max_path}")
     caches, k, v = layer_caches(kv_caches, device)
     path = torch.empty(num_seqs, max_path, device=device, dtype=torch.int32)
     accepted = torch.empty(num_seqs, device=device, dtype=torch.int32)
