@@ -159,9 +159,38 @@ SIGNATURES = {
         _p, _i64, _i32,             # block_tables, bt_stride, max_blocks
         _p, _p, _i32, _i32, _p,     # seq_lens, beams, num_groups, num_beams, stream
     ]),
+    "bvllm_build_step_tables": (ctypes.c_int, [
+        _p, _p, _i32, _p, _i64,     # query_lens, context_lens, num_seqs, pages, num_listed
+        _i32, _i32, _i32,           # window, sinks, pad_page
+        _p, _i32, _p, _p, _p, _p,   # block_tables, width, query_start_loc, seq_lens, positions, slot_mapping
+        _i32, _i32, _p,             # num_tokens, block_size, stream
+    ]),
+    "bvllm_qk_norm_rope_append": (ctypes.c_int, [
+        _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64,  # q, k, v, strides t, h
+        _p, _p, _i32, _f32,         # q_weight, k_weight, weight_fp32, eps
+        _p, _i64, _p, _i64, _i32,   # cos, sin, rows_fp32
+        _p, _i64, _i64,             # out
+        _p, _p, _i64, _i64,         # k_cache, v_cache, slot stride, head stride
+        _i64, _p,                   # num_slots, slot_mapping
+        _i32, _i32, _i32, _i32,     # T, H, Hkv, D
+        _p,                         # stream
+    ]),
+    "bvllm_window_workspace_bytes": (ctypes.c_int64, [_i32] * 10),
+    "bvllm_paged_window_attention": (ctypes.c_int, [
+        _p, _i64, _i64,             # q
+        _p, _p, _i64, _i64, _i64,   # caches + strides
+        _i32,                       # num_blocks
+        _p, _i64, _i32,             # block_tables, bt_stride, max_blocks
+        _p, _p, _p,                 # query_start_loc, seq_lens, context_lens
+        _i32, _i32, _f32,           # window, sinks, scale
+        _p, _i64, _i64,             # out
+        _i32, _i32, _i32, _i32,     # num_seqs, num_tokens, max_query_len, single_query_seqs
+        _i32, _i32, _i32, _i32,     # H, Hkv, D, block_size
+        _p, _p,                     # workspace, stream
+    ]),
 }
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 
 # Pages (rows · table width) that the balanced launches take.

@@ -578,3 +578,120 @@ extern "C" int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches,
   a.num_groups = num_groups; a.num_beams = num_beams;
   return (int)reorder_beams(a, k_caches, v_caches, num_layers, (hipStream_t)stream);
 }
+
+extern "C" int bvllm_build_step_tables(const int32_t* query_lens, const int32_t* context_lens, int32_t num_seqs,
+                                       const int32_t* pages, int64_t num_listed, int32_t window, int32_t sinks,
+                                       int32_t pad_page, int32_t* block_tables, int32_t width,
+                                       int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions,
+                                       int64_t* slot_mapping, int32_t num_tokens, int32_t block_size, void* stream) {
+  if (num_seqs < 0 || num_tokens < 0 || num_listed < 0 || window < 0 || sinks < 0 || block_size != 16) return kBad;
+  if (width < 1 || width > 1 << 28 || !query_start_loc) return kBad;
+  if (num_seqs > 0 && (!query_lens || !context_lens || !block_tables || !seq_lens)) return kBad;
+  if ((num_listed > 0 && !pages) || (num_tokens > 0 && (!positions || !slot_mapping))) return kBad;
+  StepTablesArgs a{};
+  a.query_lens = query_lens; a.context_lens = context_lens;
+  a.pages = pages; a.num_listed = num_listed;
+  a.num_seqs = num_seqs; a.width = width; a.num_tokens = num_tokens;
+  a.window = window; a.kept_pages = (int32_t)(((int64_t)sinks + 15) >> 4);
+  a.pad_page = pad_page;
+  a.block_tables = block_tables; a.query_start_loc = query_start_loc; a.seq_lens = seq_lens;
+  a.positions = positions; a.slot_mapping = slot_mapping;
+  return (int)build_step_tables(a, (hipStream_t)stream);
+}
+
+extern "C" int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                                         const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                                         const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                                         const void* q_weight, const void* k_weight, int32_t weight_fp32, float eps,
+                                         const void* cos, int64_t cos_stride_t, const void* sin, int64_t sin_stride_t,
+                                         int32_t rows_fp32, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                         void* k_cache, void* v_cache, int64_t cache_stride_slot,
+                                         int64_t cache_stride_head, int64_t num_slots, const int64_t* slot_mapping,
+                                         int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads,
+                                         int32_t head_dim, void* stream) {
+  if (num_tokens < 0 || !valid_heads(num_heads, num_kv_heads)) return kBad;
+  if (head_dim != 64 && head_dim != 128 && head_dim != 256) return kBad;
+  if (num_tokens == 0) return 0;
+  if (!q || !k || !v || !q_weight || !k_weight || !cos || !sin || !out || !k_cache || !v_cache || !slot_mapping)
+    return kBad;
+  if (num_slots <= 0) return kBad;
+  QkNormRopeArgs a{};
+  a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
+  a.k = k; a.k_st = k_stride_t; a.k_sh = k_stride_h;
+  a.v = v; a.v_st = v_stride_t; a.v_sh = v_stride_h;
+  a.q_weight = q_weight; a.k_weight = k_weight;
+  a.weight_fp32 = weight_fp32 != 0; a.rows_fp32 = rows_fp32 != 0;
+  a.eps = eps;
+  a.cos = cos; a.cs_st = cos_stride_t;
+  a.sin = sin; a.sn_st = sin_stride_t;
+  a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.c_slot = cache_stride_slot; a.c_head = cache_stride_head;
+  a.slot_mapping = slot_mapping; a.num_slots = num_slots;
+  a.num_tokens = num_tokens; a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.vec_ok = true;
+  for (const void* p : {q, k, v, q_weight, k_weight, cos, sin, (const void*)out, (const void*)k_cache, (const void*)v_cache})
+    a.vec_ok = a.vec_ok && aligned16(p);
+  for (int64_t s : {q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, out_stride_t, out_stride_h,
+                    cache_stride_slot, cache_stride_head, cos_stride_t, sin_stride_t})
+    a.vec_ok = a.vec_ok && s % 8 == 0;
+  return (int)qk_norm_rope_append(a, (hipStream_t)stream);
+}
+
+static bool window_sizes_ok(const WindowArgs& a) {
+  if (a.num_seqs < 0 || a.num_tokens < 0 || a.max_query_len < 0 || a.single_query_seqs < -1) return false;
+  if (!valid_heads(a.num_heads, a.num_kv_heads) || (a.head_dim != 64 && a.head_dim != 128)) return false;
+  return a.window >= 1 && a.sinks >= 0;
+}
+
+extern "C" int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                                                int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                                int32_t head_dim, int32_t max_blocks, int32_t window, int32_t sinks) {
+  WindowArgs a{};
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.single_query_seqs = single_query_seqs;
+  a.max_query_len = max_query_len < num_tokens ? max_query_len : num_tokens;
+  a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  a.max_blocks = max_blocks; a.window = window; a.sinks = sinks;
+  if (!window_sizes_ok(a) || max_blocks < 1 || num_tokens == 0 || num_seqs == 0 || max_query_len == 0) return 0;
+  if ((int64_t)num_tokens * num_heads > 0x7fffffff) return 0;
+  return window_workspace_bytes(a);
+}
+
+extern "C" int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                                            const void* k_cache, const void* v_cache,
+                                            int64_t cache_stride_block, int64_t cache_stride_tok,
+                                            int64_t cache_stride_head, int32_t num_blocks,
+                                            const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                                            const int32_t* query_start_loc, const int32_t* seq_lens,
+                                            const int32_t* context_lens, int32_t window, int32_t sinks, float scale,
+                                            void* out, int64_t out_stride_t, int64_t out_stride_h,
+                                            int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                                            int32_t single_query_seqs,
+                                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                            int32_t block_size, void* workspace, void* stream) {
+  WindowArgs a{};
+  a.window = window; a.sinks = sinks;
+  a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.single_query_seqs = single_query_seqs;
+  a.max_query_len = max_query_len < num_tokens ? max_query_len : num_tokens;  // (columns are numbered in 32 bits)
+  a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
+  if (!window_sizes_ok(a) || block_size != 16 || max_query_len < 0) return kBad;
+  if (!(scale > 0.f) || scale * kLog2e > 3.4e38f) return kBad;
+  if (num_tokens == 0 || num_seqs == 0 || max_query_len == 0) return 0;
+  if (!q || !out || !block_tables || !query_start_loc || !seq_lens || !context_lens) return kBad;
+  if (!cache_ok(k_cache, v_cache, cache_stride_block, cache_stride_tok, cache_stride_head, num_blocks)) return kBad;
+  if (!aligned16(q) || !aligned16(out) || q_stride_t % 8 || q_stride_h % 8 || out_stride_t % 8 || out_stride_h % 8)
+    return kBad;
+  if (max_blocks < 1 || bt_stride < max_blocks) return kBad;
+  // Offsets inside one page are 32-bit, and so are (token, head) pairs.
+  if ((int64_t)16 * cache_stride_tok > 0x3fffffff || (int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
+  if (workspace && !aligned16(workspace)) return kBad;
+  a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
+  a.k_cache = k_cache; a.v_cache = v_cache;
+  a.c_sb = cache_stride_block; a.c_st = cache_stride_tok; a.c_sh = cache_stride_head;
+  a.num_pages = num_blocks;
+  a.block_tables = block_tables; a.bt_stride = bt_stride; a.max_blocks = max_blocks;
+  a.query_start_loc = query_start_loc; a.seq_lens = seq_lens; a.context_lens = context_lens;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
+  a.workspace = workspace;
+  return (int)paged_window_attention(a, (hipStream_t)stream);
+}

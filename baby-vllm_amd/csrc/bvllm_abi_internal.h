@@ -214,6 +214,61 @@ struct BeamSelectArgs {
 };
 hipError_t beam_select(const BeamSelectArgs& a, hipStream_t stream);
 
+// Tables and slot maps from lengths (step_tables.hip).
+struct StepTablesArgs {
+  const int32_t* query_lens;               // [S]
+  const int32_t* context_lens;             // [S]
+  const int32_t* pages; int64_t num_listed;
+  int32_t num_seqs, width, num_tokens;
+  int32_t window, kept_pages;              // window 0: none; pages of the first tokens that stay
+  int32_t pad_page;
+  int32_t* block_tables;                   // [S, width], contiguous
+  int32_t* query_start_loc;                // [S + 1]
+  int32_t* seq_lens;                       // [S]
+  int64_t* positions;                      // [num_tokens]
+  int64_t* slot_mapping;                   // [num_tokens]
+};
+hipError_t build_step_tables(const StepTablesArgs& a, hipStream_t stream);
+
+// Head norms, rotation and append (qk_norm_rope.hip).
+struct QkNormRopeArgs {
+  const void* q;  int64_t q_st, q_sh;      // [T, H, D]
+  const void* k;  int64_t k_st, k_sh;      // [T, Hkv, D]
+  const void* v;  int64_t v_st, v_sh;      // [T, Hkv, D]
+  const void* q_weight; const void* k_weight;  // [D], bf16 or fp32
+  bool weight_fp32, rows_fp32;
+  float eps;
+  const void* cos; int64_t cs_st;          // [T, D], bf16 or fp32
+  const void* sin; int64_t sn_st;
+  void* out;      int64_t o_st, o_sh;      // [T, H, D]
+  void* k_cache; void* v_cache; int64_t c_slot, c_head;  // flat [slots, Hkv, D] views
+  const int64_t* slot_mapping;             // [T]
+  int64_t num_slots;
+  int32_t num_tokens, num_heads, num_kv_heads, head_dim;
+  bool vec_ok;                             // every row start is 16-byte aligned
+};
+hipError_t qk_norm_rope_append(const QkNormRopeArgs& a, hipStream_t stream);
+
+// Attention of a sliding window and a few first tokens (window_attn.hip).
+struct WindowArgs {
+  const void* q;  int64_t q_st, q_sh;      // [T, H, D]
+  const void* k_cache; const void* v_cache;
+  int64_t c_sb, c_st, c_sh;
+  int32_t num_pages;
+  const int32_t* block_tables; int64_t bt_stride; int32_t max_blocks;
+  const int32_t* query_start_loc;          // [S+1]
+  const int32_t* seq_lens;                 // [S]
+  const int32_t* context_lens;             // [S]
+  int32_t window, sinks;
+  float scale_log2;
+  void* out;      int64_t o_st, o_sh;      // [T, H, D]
+  int32_t num_seqs, num_tokens, max_query_len, single_query_seqs;
+  int32_t num_heads, num_kv_heads, head_dim;
+  void* workspace;
+};
+hipError_t paged_window_attention(const WindowArgs& a, hipStream_t stream);
+int64_t window_workspace_bytes(const WindowArgs& a);
+
 // How a linear layer of a few tokens runs (skinny_linear.hip).
 struct LinearPlan {
   int32_t rw, kw;          // row waves x k slabs of a work-group; rw = 0: not a shape for this kernel

@@ -147,7 +147,7 @@ __device__ __forceinline__ f32x4_t page_scores(const uint4 (&kop)[D / 32], const
 //                  skips are exact, and the second saves a state's first page
 //                  after every reset (each split's start) the rescale;
 //   pv_phase:      the PV MFMAs.
-// Tokens at or past tok_limit are masked: their scores become -inf and their
+// Tokens at or past tok_limit (softmax_phase_if: those not seen) are masked: their scores become -inf and their
 // V rows are replaced by zeros where they are used (unwritten slots may hold
 // NaN, and 0·NaN would poison the PV product). The masking is branch-free so
 // that loads in flight stay in flight.
@@ -159,16 +159,15 @@ struct PagePv {
   uint2 va[D / 16];    // V^T operands (row = dim (D/16)·r + c, k = token 4g+i)
 };
 
-template <int D>
-__device__ __forceinline__ void softmax_phase(WaveState<D>& st, PagePv<D>& ph, f32x4_t s,
-                                              const RowSlice<D> (&v)[4], int tok0, int tok_limit,
-                                              float scale_log2) {
+template <int D, typename Sees>
+__device__ __forceinline__ void softmax_phase_if(WaveState<D>& st, PagePv<D>& ph, f32x4_t s,
+                                                 const RowSlice<D> (&v)[4], int tok0, Sees sees, float scale_log2) {
   constexpr int VD = D / 16;
   bool live[4];
   float sv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    live[i] = tok0 + i < tok_limit;
+    live[i] = sees(tok0 + i);
     sv[i] = live[i] ? s[i] * scale_log2 : kNegInf;
   }
   float mx = fmax_prop(fmax_prop(sv[0], sv[1]), fmax_prop(sv[2], sv[3]));
@@ -203,6 +202,13 @@ __device__ __forceinline__ void softmax_phase(WaveState<D>& st, PagePv<D>& ph, f
 }
 
 template <int D>
+__device__ __forceinline__ void softmax_phase(WaveState<D>& st, PagePv<D>& ph, f32x4_t s,
+                                              const RowSlice<D> (&v)[4], int tok0, int tok_limit,
+                                              float scale_log2) {
+  softmax_phase_if<D>(st, ph, s, v, tok0, [=](int tok) { return tok < tok_limit; }, scale_log2);
+}
+
+template <int D>
 __device__ __forceinline__ void rescale_phase(WaveState<D>& st, const PagePv<D>& ph) {
   if (__builtin_amdgcn_ballot_w64(ph.alpha != 1.f && !ph.fresh) != 0) {
 #pragma unroll
@@ -225,12 +231,11 @@ __device__ __forceinline__ void page_softmax_pv(WaveState<D>& st, f32x4_t s, con
   pv_phase<D>(st, ph);
 }
 
-// One page from registers (the work-group path): K passes through the wave's
+// Scores of a page in registers (the work-group path): K passes through the wave's
 // transpose tile into the MFMA layout.
 template <int D>
-__device__ __forceinline__ void process_page(WaveState<D>& st, const PageRegs<D>& r, const uint4 (&qb)[D / 32],
-                                             unsigned char* tile, int n, int g,
-                                             int tok0, int tok_limit, float scale_log2) {
+__device__ __forceinline__ f32x4_t register_scores(const PageRegs<D>& r, const uint4 (&qb)[D / 32],
+                                                   unsigned char* tile, int n, int g) {
   constexpr int VD = D / 16;
   constexpr int PITCH = 2 * D + 16;  // bytes; the pad keeps 16-row column reads conflict-free
 #pragma unroll
@@ -241,6 +246,15 @@ __device__ __forceinline__ void process_page(WaveState<D>& st, const PageRegs<D>
   for (int c = 0; c < D / 32; ++c) kop[c] = ld16(tile + n * PITCH + 16 * (4 * c + g));
   const f32x4_t s = page_scores<D>(kop, qb);
   asm volatile("" ::: "memory");
+  return s;
+}
+
+// One page from registers.
+template <int D>
+__device__ __forceinline__ void process_page(WaveState<D>& st, const PageRegs<D>& r, const uint4 (&qb)[D / 32],
+                                             unsigned char* tile, int n, int g,
+                                             int tok0, int tok_limit, float scale_log2) {
+  const f32x4_t s = register_scores<D>(r, qb, tile, n, g);
   page_softmax_pv<D>(st, s, r.v, tok0, tok_limit, scale_log2);
 }
 

@@ -40,7 +40,7 @@ extern "C" {
 #endif
 
 /* ABI version of this header; bumped on any signature change. */
-#define BVLLM_ABI_VERSION 11
+#define BVLLM_ABI_VERSION 12
 
 #if defined(__GNUC__)
 #define BVLLM_API __attribute__((visibility("default")))
@@ -437,6 +437,73 @@ BVLLM_API int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches, 
                      int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
                      const int32_t* seq_lens, const int64_t* beams,
                      int32_t num_groups, int32_t num_beams, void* stream);
+
+/*
+ * Block tables, row offsets and slot maps of a step from its requests' lengths (no
+ * counterpart in the reference). Request s has max(context_lens[s], 0) cached and
+ * max(query_lens[s], 0) new tokens (both int32 [num_seqs]). pages (int32 [num_listed]) holds the
+ * requests' pages one request after another, ceil((cached + new) / 16) each; with window > 0
+ * without those of the entries i with ceil(sinks / 16) <= i < (cached - window + 1) / 16, which
+ * bvllm_paged_window_attention does not read. Written: block_tables int32 [num_seqs, width],
+ * contiguous (pad_page where the request holds none), query_start_loc int32 [num_seqs + 1]
+ * (exclusive sums, at most num_tokens), seq_lens int32 [num_seqs], positions and slot_mapping
+ * int64 [num_tokens] (0 and -1 in rows behind the last request's; slot -1 too where a row's page
+ * is not in the list, behind the table's width or negative). width at most 2^28.
+ */
+BVLLM_API int bvllm_build_step_tables(const int32_t* query_lens, const int32_t* context_lens, int32_t num_seqs,
+                     const int32_t* pages, int64_t num_listed, int32_t window, int32_t sinks, int32_t pad_page,
+                     int32_t* block_tables, int32_t width, int32_t* query_start_loc, int32_t* seq_lens,
+                     int64_t* positions, int64_t* slot_mapping, int32_t num_tokens, int32_t block_size,
+                     void* stream);
+
+/*
+ * RMS norm of every query and key head, RoPE and KV-store append (no counterpart in the
+ * reference; bvllm_rope_kv_append for models that normalise heads). Each head row x of
+ * q [T, H, D] and k [T, Hkv, D] becomes x * rsqrt(mean(x^2) + eps) * weight (q_weight and
+ * k_weight [D], bf16 or, weight_fp32 = 1, fp32), then is rotated by the token's cos and sin
+ * rows ([T, D] bf16 or, rows_fp32 = 1, fp32; rotate-half, as above), all in fp32 and rounded
+ * once. q goes to out [T, H, D] (out = q with q's strides is allowed), k and raw v [T, Hkv, D]
+ * to the cache row of slot_mapping[t] and nowhere else; slots outside the cache are not
+ * written. head_dim 64, 128 or 256; any alignment of the elements' own size.
+ */
+BVLLM_API int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void* k, int64_t k_stride_t, int64_t k_stride_h,
+                     const void* v, int64_t v_stride_t, int64_t v_stride_h,
+                     const void* q_weight, const void* k_weight, int32_t weight_fp32, float eps,
+                     const void* cos, int64_t cos_stride_t, const void* sin, int64_t sin_stride_t,
+                     int32_t rows_fp32, void* out, int64_t out_stride_t, int64_t out_stride_h,
+                     void* k_cache, void* v_cache, int64_t cache_stride_slot, int64_t cache_stride_head,
+                     int64_t num_slots, const int64_t* slot_mapping,
+                     int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     void* stream);
+
+/*
+ * Attention of a sliding window and a few first tokens (no counterpart in the reference).
+ * Arguments as bvllm_paged_prefill's: row i of sequence s sits at position p = context_lens[s] + i
+ * and attends keys j <= p, below seq_lens[s] and inside the table, with j > p - window or
+ * j < sinks. A row with no visible key outputs zeros; keys that a row does not see do not reach
+ * it, whatever they hold, and table entries of pages that no row of the sequence sees may hold
+ * anything. window at least 1, sinks at least 0, scale positive and finite. single_query_seqs as
+ * in bvllm_paged_prefill (-1: unknown): it steers how the step is launched, never what is computed.
+ * workspace holds bvllm_window_workspace_bytes() bytes of the same sizes, or is NULL: then rows
+ * and blocks of few work-groups are not cut over more of them. Results agree within the rounding of
+ * fp32 sums in another order.
+ */
+BVLLM_API int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                     int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t max_blocks, int32_t window, int32_t sinks);
+BVLLM_API int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
+                     const void* k_cache, const void* v_cache,
+                     int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
+                     int32_t num_blocks,
+                     const int32_t* block_tables, int64_t bt_stride, int32_t max_blocks,
+                     const int32_t* query_start_loc, const int32_t* seq_lens,
+                     const int32_t* context_lens, int32_t window, int32_t sinks, float scale,
+                     void* out, int64_t out_stride_t, int64_t out_stride_h,
+                     int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                     int32_t single_query_seqs,
+                     int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t block_size, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }
