@@ -33,6 +33,10 @@ def fused_qk_norm_rope_and_cache(q, k, v, q_weight, k_weight, eps, cos, sin, kv_
     ``[T, D]`` per-token rows (duplicated halves), both bf16 or both fp32. ``out``: where q
     goes, ``q`` itself among others; a tensor of other memory than q, k and v.
     """
+    if out is None and q.is_cuda:
+        got = _lib.fast().norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, kv_cache, slot_mapping, *_lib.current())
+        if got is not None:
+            return got
     for name, t in (("q", q), ("k", k), ("v", v), ("q_weight", q_weight), ("k_weight", k_weight), ("cos", cos),
                     ("sin", sin), ("kv_cache", kv_cache), ("slot_mapping", slot_mapping)):
         _lib.require_rocm_tensor(name, t)

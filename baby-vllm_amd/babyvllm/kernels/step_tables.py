@@ -42,6 +42,11 @@ class StepTables(NamedTuple):
 
 def build_step_tables(query_lens, context_lens, pages, num_tokens, width, *, window=None, sinks=0, pad_page=0):
     """The step's ``StepTables``. ``window`` None: the requests hold all their pages."""
+    if query_lens.is_cuda:
+        out = _lib.fast().tables(query_lens, context_lens, pages, num_tokens, width, window, sinks, pad_page, _MAX_WIDTH,
+                                 *_lib.current())
+        if out is not None:
+            return StepTables._make(out)
     for name, t in (("query_lens", query_lens), ("context_lens", context_lens), ("pages", pages)):
         _lib.require_rocm_tensor(name, t)
         if t.device != query_lens.device:

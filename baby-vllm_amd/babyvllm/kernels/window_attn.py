@@ -25,6 +25,12 @@ _MAX = 2**31 - 1
 
 def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
     """``[T, H, D]`` attention of the step's rows, K/V read from the paged cache."""
+    if q.is_cuda:
+        out = _lib.fast().window(q, kv_cache, md.block_tables, md.query_start_loc, md.seq_lens, md.context_lens,
+                                 getattr(md, "query_start_loc_cpu", None), md.max_query_len, scale, window, sinks,
+                                 *_lib.current())
+        if out is not None:
+            return out
     for name, t in (("q", q), ("kv_cache", kv_cache), ("block_tables", md.block_tables),
                     ("query_start_loc", md.query_start_loc), ("seq_lens", md.seq_lens),
                     ("context_lens", md.context_lens)):
@@ -64,16 +70,22 @@ def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
         return out
     qsl, seq_lens, ctx_lens = md.query_start_loc.contiguous(), md.seq_lens.contiguous(), md.context_lens.contiguous()
     h = _lib.lib()
+    window, sinks = min(int(window), _MAX), min(int(sinks), _MAX)
+    single = _single_query_seqs(md, num_seqs) if max_query_len > 1 else -1
     with torch.cuda.device(q.device):
+        nbytes = h.bvllm_window_workspace_bytes(num_seqs, num_tokens, max_query_len, single, num_heads, num_kv_heads,
+                                                head_dim, bt.shape[1], window, sinks)
+        workspace = _lib.optional_scratch(nbytes, q.device) if nbytes > 0 else None
         rc = h.bvllm_paged_window_attention(
             q.data_ptr(), q.stride(0), q.stride(1),
             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
             num_blocks,
             bt.data_ptr(), bt.stride(0), bt.shape[1],
             qsl.data_ptr(), seq_lens.data_ptr(), ctx_lens.data_ptr(),
-            min(int(window), _MAX), min(int(sinks), _MAX), float(scale),
+            window, sinks, float(scale),
             out.data_ptr(), out.stride(0), out.stride(1),
-            num_seqs, num_tokens, max_query_len, _single_query_seqs(md, num_seqs),
-            num_heads, num_kv_heads, head_dim, page, None, _lib.stream_handle(q.device))
+            num_seqs, num_tokens, max_query_len, single,
+            num_heads, num_kv_heads, head_dim, page, None if workspace is None else workspace.data_ptr(),
+            _lib.stream_handle(q.device))
     _lib.check(rc, "bvllm_paged_window_attention")
     return out

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "bvllm_fast_div.h"
 
 namespace bvllm {
@@ -360,5 +362,22 @@ inline int64_t prefill_range_floats(int32_t num_ranges, int32_t num_tokens, int3
 }
 // Compute units of the current device (cached per device).
 int device_cus();
+
+// Sets a kernel's dynamic-LDS limit once per device (setting it twice, from
+// racing host threads, is harmless).
+template <typename K>
+static hipError_t allow_lds(K* kernel, std::atomic<bool> (&done)[64], int bytes) {
+  int dev = 0;
+  hipError_t err = hipGetDevice(&dev);
+  if (err != hipSuccess) return err;
+  if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
+  if (!done[dev].load(std::memory_order_acquire)) {
+    err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                              bytes);
+    if (err != hipSuccess) return err;
+    done[dev].store(true, std::memory_order_release);
+  }
+  return hipSuccess;
+}
 
 }  // namespace bvllm

@@ -49,6 +49,10 @@ struct Entry {
   decltype(&bvllm_beam_workspace_bytes) beam_bytes = nullptr;
   decltype(&bvllm_beam_select) beam = nullptr;
   decltype(&bvllm_reorder_beams) reorder = nullptr;
+  decltype(&bvllm_build_step_tables) tables = nullptr;
+  decltype(&bvllm_qk_norm_rope_append) norm_rope = nullptr;
+  decltype(&bvllm_window_workspace_bytes) window_bytes = nullptr;
+  decltype(&bvllm_paged_window_attention) window = nullptr;
 } g;
 
 struct BindName {
@@ -78,6 +82,10 @@ const BindName kNames[] = {
     {"bvllm_beam_workspace_bytes", (void**)&g.beam_bytes},
     {"bvllm_beam_select", (void**)&g.beam},
     {"bvllm_reorder_beams", (void**)&g.reorder},
+    {"bvllm_build_step_tables", (void**)&g.tables},
+    {"bvllm_qk_norm_rope_append", (void**)&g.norm_rope},
+    {"bvllm_window_workspace_bytes", (void**)&g.window_bytes},
+    {"bvllm_paged_window_attention", (void**)&g.window},
 };
 
 // The wrappers' own error for a return code (babyvllm.kernels._lib.check), bound with the addresses.
@@ -700,6 +708,158 @@ PyObject* fast_reorder(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// (query_lens, context_lens, pages, num_tokens, width, window | None, sinks, pad_page, max_width, device, stream)
+//   -> (block_tables, query_start_loc, seq_lens, positions, slot_mapping)
+PyObject* fast_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11) return none();
+  const int64_t dev = PyLong_AsLongLong(a[9]);
+  const at::Tensor* lens = plain(a[0], at::kInt, dev);
+  const at::Tensor* ctx = plain(a[1], at::kInt, dev);
+  const at::Tensor* pages = plain(a[2], at::kInt, dev);
+  for (const at::Tensor* v : {lens, ctx, pages})
+    if (!v || v->dim() != 1 || !v->is_contiguous()) return none();
+  for (int i : {3, 4, 6, 7})
+    if (!PyLong_CheckExact(a[i])) return none();
+  if (a[5] != Py_None && !PyLong_CheckExact(a[5])) return none();
+  const int64_t seqs = lens->size(0), rows = clamped(a[3]), width = clamped(a[4]), pad = clamped(a[7]);
+  const int64_t window = a[5] == Py_None ? 0 : clamped(a[5]), sinks = clamped(a[6]);
+  const int64_t max_width = PyLong_AsLongLong(a[8]);
+  void* stream = PyLong_AsVoidPtr(a[10]);
+  if (PyErr_Occurred()) return nullptr;
+  if (seqs == 0 || ctx->size(0) != seqs || !small(seqs) || !small(rows) || width < 1 || width > max_width) return none();
+  if ((a[5] != Py_None && window < 1) || sinks < 0 || pad < INT32_MIN || pad > INT32_MAX) return none();
+  at::Tensor out[5];
+  int rc;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const at::Tensor narrow = empty_beside({seqs * width + 2 * seqs + 1}, *lens, at::kInt);
+    const at::Tensor wide = empty_beside({2 * rows}, *lens, at::kLong);
+    out[0] = part_of(narrow, 0, {seqs, width});
+    out[1] = part_of(narrow, seqs * width, {seqs + 1});
+    out[2] = part_of(narrow, seqs * width + seqs + 1, {seqs});
+    out[3] = part_of(wide, 0, {rows});
+    out[4] = part_of(wide, rows, {rows});
+    rc = g.tables(lens->const_data_ptr<int32_t>(), ctx->const_data_ptr<int32_t>(), (int32_t)seqs,
+                  pages->const_data_ptr<int32_t>(), pages->size(0), (int32_t)std::min<int64_t>(window, INT32_MAX),
+                  (int32_t)std::min<int64_t>(sinks, INT32_MAX), (int32_t)pad, out[0].mutable_data_ptr<int32_t>(),
+                  (int32_t)width, out[1].mutable_data_ptr<int32_t>(), out[2].mutable_data_ptr<int32_t>(),
+                  rows > 0 ? out[3].mutable_data_ptr<int64_t>() : nullptr,
+                  rows > 0 ? out[4].mutable_data_ptr<int64_t>() : nullptr, (int32_t)rows, (int32_t)kPage, stream);
+  }
+  if (rc != 0) return failed(rc, "bvllm_build_step_tables");
+  PyObject* t = PyTuple_New(5);
+  for (int i = 0; t != nullptr && i < 5; ++i) {
+    PyObject* x = THPVariable_Wrap(out[i]);
+    if (x == nullptr) Py_CLEAR(t);
+    else PyTuple_SET_ITEM(t, i, x);
+  }
+  return t;
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, q_weight, k_weight, eps, cos, sin, kv_cache, slot_mapping, device, stream)
+PyObject* fast_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) return none();
+  const int64_t dev = PyLong_AsLongLong(a[10]);
+  const at::Tensor* q = plain(a[0], at::kBFloat16, dev);
+  const at::Tensor* k = plain(a[1], at::kBFloat16, dev);
+  const at::Tensor* v = plain(a[2], at::kBFloat16, dev);
+  const at::Tensor* c = plain(a[8], at::kBFloat16, dev);
+  const at::Tensor* slots = plain(a[9], at::kLong, dev);
+  // A pair of bf16 or of fp32 tensors.
+  auto pair = [&](int i, int j, const at::Tensor** x, const at::Tensor** y, bool& fp32) {
+    *x = plain(a[i], at::kBFloat16, dev);
+    fp32 = *x == nullptr;
+    if (fp32) *x = plain(a[i], at::kFloat, dev);
+    *y = plain(a[j], fp32 ? at::kFloat : at::kBFloat16, dev);
+    return *x != nullptr && *y != nullptr;
+  };
+  const at::Tensor *qw, *kw, *cos, *sin;
+  bool weight_fp32, rows_fp32;
+  if (!pair(3, 4, &qw, &kw, weight_fp32) || !pair(6, 7, &cos, &sin, rows_fp32)) return none();
+  if (!rows_of(q, 3) || !rows_of(k, 3) || !rows_of(v, 3) || !rows_of(cos, 2) || !rows_of(sin, 2)) return none();
+  const int64_t tokens = q->size(0), heads = q->size(1), d = q->size(2), hkv = k->size(1);
+  if (!plain_cache(c) || !c->is_contiguous() || !slots || slots->dim() != 1 || !slots->is_contiguous()) return none();
+  if (tokens == 0 || k->size(0) != tokens || k->size(2) != d || v->sizes() != k->sizes()) return none();
+  if (cos->size(0) < tokens || cos->size(1) != d || sin->sizes() != cos->sizes()) return none();
+  for (const at::Tensor* w : {qw, kw})
+    if (w->dim() != 1 || w->size(0) != d || !w->is_contiguous()) return none();
+  if (c->size(3) != hkv || c->size(4) != d || slots->size(0) < tokens || !small(tokens) || !small(heads)) return none();
+  if ((d != 64 && d != 128 && d != 256) || !PyFloat_CheckExact(a[5])) return none();
+  const float eps = (float)PyFloat_AsDouble(a[5]);
+  void* stream = PyLong_AsVoidPtr(a[11]);
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16);
+  return launch(out, "bvllm_qk_norm_rope_append", [&] {
+    void* cp = out_ptr(*c);
+    return g.norm_rope(ptr(*q), q->stride(0), q->stride(1), ptr(*k), k->stride(0), k->stride(1), ptr(*v), v->stride(0),
+                       v->stride(1), ptr(*qw), ptr(*kw), weight_fp32 ? 1 : 0, eps, ptr(*cos), cos->stride(0), ptr(*sin),
+                       sin->stride(0), rows_fp32 ? 1 : 0, ptr(out), out.stride(0), out.stride(1), cp,
+                       (char*)cp + c->stride(0) * 2, c->stride(2), c->stride(3), c->size(1) * c->size(2),
+                       slots->const_data_ptr<int64_t>(), (int32_t)tokens, (int32_t)heads, (int32_t)hkv, (int32_t)d,
+                       stream);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, kv_cache, block_tables, query_start_loc, seq_lens, context_lens, query_start_loc list, max_query_len, scale,
+//  window, sinks, device, stream)
+PyObject* fast_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 13) return none();
+  const int64_t dev = PyLong_AsLongLong(a[11]);
+  const at::Tensor* q = plain(a[0], at::kBFloat16, dev);
+  const at::Tensor* c = plain(a[1], at::kBFloat16, dev);
+  const at::Tensor* bt = plain(a[2], at::kInt, dev);
+  const at::Tensor* qsl = plain(a[3], at::kInt, dev);
+  const at::Tensor* seq = plain(a[4], at::kInt, dev);
+  const at::Tensor* ctx = plain(a[5], at::kInt, dev);
+  if (!rows_of(q, 3) || !plain_cache(c) || !rows_of(bt, 2)) return none();
+  for (const at::Tensor* v : {qsl, seq, ctx})
+    if (!v || v->dim() != 1 || !v->is_contiguous()) return none();
+  const int64_t tokens = q->size(0), heads = q->size(1), d = q->size(2), hkv = c->size(3), seqs = seq->size(0);
+  const int64_t width = bt->size(1);
+  if (tokens == 0 || seqs == 0 || width == 0 || c->size(4) != d || c->size(2) != kPage) return none();
+  if (qsl->size(0) != seqs + 1 || ctx->size(0) != seqs || bt->size(0) < seqs) return none();
+  if (!small(tokens) || !small(heads) || !small(seqs) || !small(width)) return none();
+  if (!PyLong_CheckExact(a[7]) || !PyFloat_CheckExact(a[8]) || !PyLong_CheckExact(a[9]) || !PyLong_CheckExact(a[10]))
+    return none();
+  const int64_t max_q = clamped(a[7]), window = clamped(a[9]), sinks = clamped(a[10]);
+  const float scale = (float)PyFloat_AsDouble(a[8]);
+  void* stream = PyLong_AsVoidPtr(a[12]);
+  if (PyErr_Occurred()) return nullptr;
+  if (max_q < 1 || !small(max_q) || window < 1 || sinks < 0) return none();
+  int64_t single = -1;  // sequences of one query; where all are, nobody asks
+  if (max_q > 1 && PyList_CheckExact(a[6]) && PyList_GET_SIZE(a[6]) == seqs + 1) {
+    single = 0;
+    int64_t last = 0;
+    for (int64_t i = 0; i <= seqs; ++i) {
+      PyObject* o = PyList_GET_ITEM(a[6], i);
+      if (!PyLong_CheckExact(o)) return none();
+      const int64_t at = clamped(o);
+      if (!small(at)) return none();
+      if (i > 0 && at - last == 1) ++single;
+      last = at;
+    }
+  }
+  const int32_t w = (int32_t)std::min<int64_t>(window, INT32_MAX), first = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
+  const int64_t bytes = g.window_bytes((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)single, (int32_t)heads,
+                                       (int32_t)hkv, (int32_t)d, (int32_t)width, w, first);
+  at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16), ws;
+  if (bytes > 0) ws = optional_scratch(bytes, *q);
+  return launch(out, "bvllm_paged_window_attention", [&] {
+    return g.window(ptr(*q), q->stride(0), q->stride(1), ptr(*c), v_half(*c), c->stride(1), c->stride(2), c->stride(3),
+                    (int32_t)c->size(1), bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width,
+                    qsl->const_data_ptr<int32_t>(), seq->const_data_ptr<int32_t>(), ctx->const_data_ptr<int32_t>(), w,
+                    first, scale, ptr(out), out.stride(0), out.stride(1), (int32_t)seqs, (int32_t)tokens, (int32_t)max_q,
+                    (int32_t)single, (int32_t)heads, (int32_t)hkv, (int32_t)d, (int32_t)kPage,
+                    ws.defined() ? ptr(ws) : nullptr, stream);
+  });
+  END_HANDLE_TH_ERRORS
+}
+
 // ({name: address}, check): binds the library's entry points and what raises for a return code.
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2 || !PyDict_Check(a[0]) || !PyCallable_Check(a[1]))
@@ -735,6 +895,7 @@ PyObject* names(PyObject*, PyObject*) {
 PyMethodDef kMethods[] = {
     FAST(norm), FAST(silu), FAST(rope), FAST(auto_plan), FAST(decode), FAST(prefill), FAST(linear),
     FAST(tree), FAST(commit), FAST(beam), FAST(reorder),
+    FAST(tables), FAST(norm_rope), FAST(window),
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, nullptr}, {"names", names, METH_NOARGS, nullptr}, {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_fast_calls", nullptr, -1, kMethods};

@@ -396,23 +396,6 @@ int device_cus() {
   return v;
 }
 
-// Sets a kernel's dynamic-LDS limit once per device (setting it twice, from
-// racing host threads, is harmless).
-template <typename K>
-static hipError_t allow_lds(K* kernel, std::atomic<bool> (&done)[64], int bytes) {
-  int dev = 0;
-  hipError_t err = hipGetDevice(&dev);
-  if (err != hipSuccess) return err;
-  if (dev < 0 || dev >= 64) return hipErrorInvalidDevice;
-  if (!done[dev].load(std::memory_order_acquire)) {
-    err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                              bytes);
-    if (err != hipSuccess) return err;
-    done[dev].store(true, std::memory_order_release);
-  }
-  return hipSuccess;
-}
-
 template <int D, int PF, bool GROUP>
 static hipError_t launch_stream_pf(const DecodeArgs& a, int64_t items, hipStream_t stream) {
   if (tuning(kTuneDecodeCached) == 0)

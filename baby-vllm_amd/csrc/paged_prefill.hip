@@ -37,12 +37,16 @@
 #include "bvllm_abi_internal.h"
 #include "paged_decode_wg.h"
 #include "tree_attn.h"
+#include "window_attn.h"
 
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 namespace bvllm {
+
+// Bits b < n, all for n > 31, none for n < 0.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n > 31 ? ~0u : (1u << max(n, 0)) - 1; }
 
 // Blocks of CB columns (a sequence's q_len·G (query, head) pairs, numbered
 // query-major) are numbered sequence by sequence, the blocks of a sequence last
@@ -96,6 +100,61 @@ __device__ __forceinline__ bool find_query_block(const PrefillArgs& a, int CB, i
 constexpr int kDecodeWaves = 4;
 constexpr int kDecodeDepth = 1;
 
+// A block of a step of windows (columns f0 .. of a sequence and KV head), one row after the other, each over what the
+// range has of the pages that it sees. Called for the few blocks that need it, and not inlined: the prefill kernel's walk
+// would lose registers to the call's arguments, and half its speed. So it takes the launch's arguments from the
+// kernel's own, which begin with a PrefillArgs and four integers.
+struct WindowLaunchArgs {
+  PrefillArgs blocks;
+  int32_t grid[4];
+  WindowRows rows;
+};
+typedef const uint32_t __attribute__((address_space(4)))* WindowLaunch;
+
+template <int D, int NW, bool SPL>
+__attribute__((noinline)) __device__ void window_block_rows(WindowLaunch launch, __attribute__((address_space(3))) unsigned char* lds,
+                                                            int s, int kvh, int f0, int width, int range, int ranges) {
+  static_assert(sizeof(WindowLaunchArgs) % 4 == 0 && alignof(WindowLaunchArgs) == 8 && sizeof(PrefillArgs) % 8 == 0, "argument words");
+  union Words {
+    uint32_t w[sizeof(WindowLaunchArgs) / 4];
+    WindowLaunchArgs args;
+    __device__ Words() {}
+  } words;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(words.w) / 4); ++i) words.w[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)launch[i]);
+  const PrefillArgs& a = words.args.blocks;
+  const WindowRows& rows = words.args.rows;
+  s = uniform(s); kvh = uniform(kvh); f0 = uniform(f0); range = uniform(range); ranges = uniform(ranges);
+  const int G = a.num_heads / a.num_kv_heads, groups = col_groups_per_kv(G);
+  const int q_start = uniform(a.query_start_loc[s]), q_len = uniform(a.query_start_loc[s + 1]) - q_start;
+  const int seq_len = uniform(a.seq_lens[s]), ctx = uniform(a.context_lens[s]);
+  const int f1 = min(q_len * G, f0 + width);
+  const BlockWalk walk(ctx, seq_len, a.max_blocks, rows.window, rows.sinks, f0 / G, (f1 - 1) / G);
+  const int per = 4 * a.split_tiles, k0 = SPL ? per * range : 0;
+  const int steps = (walk.end + 15) >> 4, k1 = SPL && range < ranges - 1 ? min(steps, k0 + per) : steps;
+  const bool partial = SPL && (k0 > 0 || k1 < steps);
+#pragma unroll 1
+  for (int u = f0 / G * groups; u / groups * G < f1; ++u) {
+    const int qn = u / groups;
+    const RowView view((int64_t)ctx + qn, seq_len, a.max_blocks, rows.window, rows.sinks);
+    const ColGroup cg = col_group(G, kvh * groups + u - qn * groups);
+    window_row<D, NW>(rows.rows, s, q_start + qn, cg, view, k0, k1, [&](int k) { return walk.page(k); }, (unsigned char*)lds,
+                      [&](int head, int d, f32x4_t o, float ref, float L) {
+      const int f = qn * G + head - kvh * G;
+      if (f < f0 || f >= f1) return;
+      const int64_t row = (int64_t)(q_start + qn);
+      if (!partial) {
+        st8(reinterpret_cast<uint16_t*>(a.out) + row * a.o_st + (int64_t)head * a.o_sh + d,
+            make_uint2(pack_bf16x2_hw(o[0], o[1]), pack_bf16x2_hw(o[2], o[3])));
+      } else {
+        const int64_t at = ((int64_t)range * a.num_tokens + row) * a.num_heads + head;
+        *reinterpret_cast<f32x4_t*>(a.part_out + at * D + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(ref + __log2f(L), L == 0.f ? 0.f : 1.f);
+      }
+    });
+  }
+}
+
 // MB: groups of several blocks per work-group, launched only when every
 // sequence's keys fit two 64-key tiles (the kernel has no streaming path then).
 // KS: key split inside the work-group. KS = 1: each wave owns QT column tiles
@@ -114,10 +173,15 @@ constexpr int kDecodeDepth = 1;
 // partial. A sequence's tiles are cut evenly into ranges of at most a.split_tiles, each a
 // work-group that always writes its partial. The work-groups behind them take the other keys,
 // with masks (tree_columns).
-template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false>
+// WIN: a step of a sliding window and first tokens (window_attn.h). The walk's pages are those that
+// some row of the block sees (BlockWalk), put together to tiles whatever lies between them; keys
+// that a column does not see are masked by their place in the walk. A key that some columns of a
+// block see and others do not is in a tile of all of them, where a weight of 0 leaves the product's
+// 0·V: a block whose sums are not finite is computed again, row by row (window_row).
+template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false, bool WIN = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
                                                                   int xcd_group, int per_xcd,
-                                                                  std::conditional_t<CTX, TreeArgs, DecodeArgs> dec,
+                                                                  std::conditional_t<CTX, TreeArgs, std::conditional_t<WIN, WindowRows, DecodeArgs>> dec,
                                                                   int n_dec_wgs, int bpw) {
   constexpr int KT = 64;
   constexpr int RB = 2 * D;   // bytes of one key row of K or V (no padding)
@@ -142,7 +206,14 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // otherwise fills each CU's memory queue in front of them (mixed step
   // 1 x 512 + 63 decodes: 34.6 -> 29.5 us).
   const int n_pre_wgs = (int)gridDim.x - n_dec_wgs;
-  if constexpr (!CTX) {
+  if constexpr (WIN) {
+    if ((int)blockIdx.x >= n_pre_wgs) {
+      const int dw = (int)blockIdx.x - n_pre_wgs;
+      if (dw < dec.rows.batch * dec.rows.num_splits * dec.rows.num_kv_heads * col_groups_per_kv(dec.rows.num_heads / dec.rows.num_kv_heads))
+        window_row_group<D, kDecodeWaves>(dec.rows, dec.window, dec.sinks, dw, lds);
+      return;
+    }
+  } else if constexpr (!CTX) {
     if ((int)blockIdx.x >= n_pre_wgs) {
       const int dw = (int)blockIdx.x - n_pre_wgs;
       if (dec.chunk_target > 0)  // uneven rows: cut into chunks (RowChunk)
@@ -155,7 +226,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
 
   const int G = a.num_heads / a.num_kv_heads;
   static_assert(KS == 1 || (KS == 2 && !MB && NW % 2 == 0), "key split: two halves, streaming path only");
-  static_assert(!SPL || CTX || (KS == 1 && !MB), "key ranges: single key walk only");
+  static_assert(!SPL || CTX || WIN || (KS == 1 && !MB), "key ranges: single key walk only");
+  static_assert(!WIN || (!MB && !CTX), "windows: one block at a time");
+  static_assert(!WIN || rows_lds_bytes<D, NW>(16) <= sizeof(lds), "single rows' work-group LDS");
   static_assert(!CTX || (SPL && !MB), "context tiles come in ranges");
   constexpr int CB = NW / KS * QT * 16;  // columns of a work-group's block
 
@@ -172,7 +245,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   const int grid_wgs = SPL ? n_pre_wgs / bpw : n_pre_wgs;
   int range = SPL && !CTX ? (int)blockIdx.x / grid_wgs : 0;
   const int id = SPL && !CTX ? (int)blockIdx.x - range * grid_wgs : (int)blockIdx.x;
-  int tile0 = SPL && !CTX ? range * a.split_tiles : 0;  // first key tile of the range
+  constexpr bool SHIFT = SPL && !CTX && !WIN;   // a range is the sequence shifted by its start
+  int tile0 = SHIFT ? range * a.split_tiles : 0;  // first key tile of the range
   int max_blocks = SPL ? a.max_blocks - 4 * tile0 : a.max_blocks;  // > 0: ranges start inside the table
   // The arguments that address the metadata and table loads below, read
   // with the mapping's own: otherwise their wait splits those loads' round trip.
@@ -252,11 +326,23 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // from the compiler's schedule of the rest of the step). Entries past
   // 2^28 are never needed (seq_len < 2^31 is at most 2^27 pages), which
   // keeps the byte offsets inside 32 bits.
+  BlockWalk walk;
+  int walk0 = 0;  // WIN: the range's first page of the walk
+  if constexpr (WIN) {
+    asm volatile("" : "+s"(q_start), "+s"(q_end), "+s"(seq_len), "+s"(ctx));
+    const int qn = q_end - q_start;
+    walk = BlockWalk(ctx, seq_len, a.max_blocks, dec.window, dec.sinks, qb * CB / G, (min(qn * G, (qb + 1) * CB) - 1) / G);
+    if constexpr (SPL) walk0 = PAGES_PER_TILE * range * a.split_tiles;
+  }
   typedef const char __attribute__((address_space(4)))* ConstBytes;
   const uint32_t bt_last = (uint32_t)min(max_blocks - 1, 1 << 28) * 4u;
   const uint32_t page_last = (uint32_t)(a.num_pages - 1);
   auto page_fetch = [&](int kt, int (&raw)[PAGES_PER_TILE]) __attribute__((always_inline)) {
-    if constexpr (KS == 2) {
+    if constexpr (WIN) {
+      const int k0 = kt * PAGES_PER_TILE + walk0;
+#pragma unroll
+      for (int pg = 0; pg < PAGES_PER_TILE; ++pg) raw[pg] = bts[min(walk.page(k0 + pg), max_blocks - 1)];
+    } else if constexpr (KS == 2) {
       const uint32_t o0 = (uint32_t)kt * (4u * PAGES_PER_TILE);
 #pragma unroll
       for (int pg = 0; pg < PAGES_PER_TILE; ++pg)
@@ -288,7 +374,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   }
   const int q_len = q_end - q_start;
   const int n_cols = q_len * G;
-  if constexpr (SPL && !CTX) {  // the sequence as seen from the range's first key
+  if constexpr (SHIFT) {  // the sequence as seen from the range's first key
     ctx -= KT * tile0;
     seq_len -= KT * tile0;
   }
@@ -315,7 +401,8 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   const int q_last = (min(n_cols, (blk + 1) * CB) - 1) / G;
   // (MB: the host checked that no sequence has more than two tiles' pages;
   // the clamp keeps an inconsistent seq_lens inside the staged tiles.)
-  const int hi_all = CTX ? KT * ctx_tiles : min(seq_len, ctx + q_last + 1);
+  // (WIN: places in the range's walk, here and in what follows from it.)
+  const int hi_all = WIN ? walk.end - 16 * walk0 : CTX ? KT * ctx_tiles : min(seq_len, ctx + q_last + 1);
   // (SPL: the last range takes the rest of the row, so a row longer than the host's
   // lists say is slower but no key of it is left out and no partial is out of range.)
   const int hi = min(hi_all, MB ? 2 * KT : SPL && !CTX && range < bpw - 1 ? KT * a.split_tiles : 0x7fffffff);
@@ -327,7 +414,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   const int wave_f0 = blk * CB + cw * QT * 16;
   const int wave_q0 = wave_f0 / G;  // first query index of this wave
   const bool wave_live = wave_f0 < n_cols;
-  const int wave_hi = CTX ? hi - 1 : ctx + min(q_len - 1, (wave_f0 + QT * 16 - 1) / G);  // last visible key position
+  // Last visible key position.
+  const int wave_last_q = min(q_len - 1, (wave_f0 + QT * 16 - 1) / G);
+  const int wave_hi = WIN ? walk.place(ctx + wave_last_q + 1) - 1 - 16 * walk0 : CTX ? hi - 1 : ctx + wave_last_q;
 
   int qi[QT], hl[QT];
   int qpos[QT];
@@ -421,7 +510,20 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // After the wave's loads landed: V rows of tile kt at or past hi become
   // zeros (unwritten slots may hold NaN, and 0·NaN would poison the PV
   // product). K rows there only reach scores that the mask replaces by -inf.
+  // (WIN: and those between the first tokens and the block's first window key, which no column sees.)
+  const int gap0 = WIN ? walk.sinks - 16 * walk0 : 0, gap1 = WIN ? walk.first_place - 16 * walk0 : 0;
   auto zero_v_tail = [&](int kt, int buf) __attribute__((always_inline)) {
+    if constexpr (WIN) {
+      if (max(gap0, kt * KT) < min(gap1, kt * KT + KT)) {  // uniform
+#pragma unroll
+        for (int r = 0; r < PER_T; ++r) {
+          const int row = kt * KT + (r * NW + w) * RPB + lane / CPR;
+          if (row >= gap0 && row < gap1)
+            *reinterpret_cast<u32x4_t*>(lds + (2 + buf) * TB + (r * NW + w) * 1024 + lane * 16) =
+                u32x4_t{0u, 0u, 0u, 0u};
+        }
+      }
+    }
     if (!CTX && kt * KT + KT > hi) {  // uniform
 #pragma unroll
       for (int r = 0; r < PER_T; ++r) {
@@ -439,7 +541,17 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
   // for the column iff pos > lim.
   int lim[QT];
 #pragma unroll
-  for (int ct = 0; ct < QT; ++ct) lim[ct] = min(qpos[ct], hi - 1);
+  for (int ct = 0; ct < QT; ++ct) lim[ct] = min(WIN && valid[ct] ? walk.place(qpos[ct] + 1) - 1 - 16 * walk0 : qpos[ct], hi - 1);
+  // WIN: a column's first key of its window; of the wave's columns, the first one's last key and the last one's first.
+  int low[QT];
+  int wave_lim = 0, wave_low = 0;
+  if constexpr (WIN) {
+#pragma unroll
+    for (int ct = 0; ct < QT; ++ct)
+      low[ct] = valid[ct] ? walk.place(max(qpos[ct] - dec.window + 1, 0)) - 16 * walk0 : 0;
+    wave_lim = walk.place(ctx + wave_q0 + 1) - 1 - 16 * walk0;
+    wave_low = walk.place(max(ctx + wave_last_q - dec.window + 1, 0)) - 16 * walk0;
+  }
   // 32-key halves of tiles this wave computes: up to its last visible key
   // (wave_hi) and below hi.
   const int wave_halves = wave_live ? min((hi + 31) / 32, wave_hi / 32 + 1) : 0;
@@ -475,6 +587,16 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
 #pragma unroll
     for (int ct = 0; ct < QT; ++ct) {
       const int rel = lim[ct] - k0 - 4 * g;
+      if constexpr (WIN) {
+        // Bit 16t + i: whether the column sees the key; all of them below its last one, none of [from, to).
+        const int from = gap0 - k0 - 4 * g, to = low[ct] - k0 - 4 * g;
+        const uint32_t seen = bits_below(rel + 1) & (bits_below(from) | ~bits_below(to));
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) S[ct][t][i] = (seen >> (16 * t + i)) & 1 ? S[ct][t][i] : kNegInf;
+        continue;
+      }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -483,7 +605,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
     }
   };
   // Some key of the half at k0 may be invisible to some column of the wave.
-  auto needs_mask = [&](int k0) { return !CTX && ((k0 + 31 > ctx + wave_q0) || (k0 + 32 > hi)); };
+  auto needs_mask = [&](int k0) {
+    if constexpr (WIN) return k0 + 31 > wave_lim || k0 + 32 > hi || max(gap0, k0) < min(wave_low, k0 + 32);
+    return !CTX && ((k0 + 31 > ctx + wave_q0) || (k0 + 32 > hi));
+  };
   // The scores' max of each column over a half, in log2 units (the scale is
   // > 0, so it commutes with the max): a chain of three-input maxima, then
   // across the four lane groups.
@@ -659,6 +784,9 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
 #pragma unroll
     for (int c = 0; c < KC; ++c) asm volatile("" ::"v"(qreg[ct][c].x), "v"(qreg[ct][c].y), "v"(qreg[ct][c].z), "v"(qreg[ct][c].w));
   __syncthreads();
+  // (WIN: a column may see keys that score far below 0 only behind its first half: its reference is low
+  // enough that the first of them raises it.)
+  constexpr float kNoKeyYet = WIN ? -3e38f : 0.f;
   if (KS == 1 ? wave_halves > 0 : wave_tiles > 0) {
     qk(S0, 0, KS == 2 ? kh : 0);
     if (needs_mask(32 * kh)) mask(S0, 32 * kh);
@@ -667,7 +795,7 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
     float mt[QT];
     half_max(S0, mt);
 #pragma unroll
-    for (int ct = 0; ct < QT; ++ct) m[ct] = mt[ct] == kNegInf ? 0.f : mt[ct];
+    for (int ct = 0; ct < QT; ++ct) m[ct] = mt[ct] == kNegInf ? kNoKeyYet : mt[ct];
   }
   // KS = 2: step 0 loads K(2) into K(0)'s buffer, which every wave has just
   // read for Sᵀ(0).
@@ -819,6 +947,28 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
     wait_loads();
   }
 
+  if constexpr (WIN) {
+    bool odd = false;
+#pragma unroll
+    for (int ct = 0; ct < QT; ++ct)
+#pragma unroll
+      for (int c = 0; c < VD; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) odd |= valid[ct] && kh == 0 && !(fabsf(acc[ct][c][i]) < __builtin_huge_valf());
+    // The barrier also says that no wave reads the tiles any more.
+    __shared__ int odd_waves[NW];
+    const int mine = __builtin_amdgcn_ballot_w64(odd) != 0;
+    if (lane == 0) odd_waves[w] = mine;
+    __syncthreads();
+    int any = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) any |= odd_waves[i];
+    if (uniform(any) != 0) {
+      window_block_rows<D, NW, SPL>((WindowLaunch)__builtin_amdgcn_kernarg_segment_ptr(),
+                                    (__attribute__((address_space(3))) unsigned char*)lds, s, kvh, blk * CB, CB, range, bpw);
+      return;
+    }
+  }
   if constexpr (SPL) {
     if (CTX || range > 0 || hi_all > hi) {  // one of several ranges: fp32 partials
       // Lane n + 16g holds dims 16c + 4g .. +3 of column n.
@@ -870,28 +1020,10 @@ __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a
 // 1 x (8000+64) in 16 ranges from 23 to 33 us).
 constexpr int kMergeBatch = 8;
 
-template <int D, int CB>
-__global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int blocks_per_token) {
-  constexpr int TPR = D / 4;  // threads per (token, head)
-  const int t = (int)blockIdx.x / blocks_per_token;
-  const int it = ((int)blockIdx.x - t * blocks_per_token) * 256 + (int)threadIdx.x;
-  // The token's sequence: the number of sequences that start at or before it, less one.
-  int s = -1;
-  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
-    const int i = s0 + lane_id();
-    const bool before = i < a.num_seqs && a.query_start_loc[i] <= t;
-    s += __popcll(__builtin_amdgcn_ballot_w64(before));
-  }
-  const int head = it / TPR, d = 4 * (it - head * TPR);
-  if (s < 0 || head >= a.num_heads) return;
-  s = uniform(s);
-  const int q_start = a.query_start_loc[s], q_len = a.query_start_loc[s + 1] - q_start;
-  const int seq_len = a.seq_lens[s], ctx = a.context_lens[s];
-  if (t >= q_start + q_len || (q_len == 1 && a.single_query_seqs != 0)) return;
-  const int G = a.num_heads / a.num_kv_heads;
-  const int blk = ((t - q_start) * G + head % G) / CB;
-  const int q_last = (min(q_len * G, (blk + 1) * CB) - 1) / G;
-  const int hi = min(seq_len, ctx + q_last + 1);
+// Adds the ranges of the 4 dims d .. of one (token, head), whose block walks `hi` keys. ODD: sums may be
+// infinite, and a range that is loaded but not there must not meet them with its weight of 0.
+template <int D, bool ODD = false>
+__device__ __forceinline__ void merge_ranges(const PrefillArgs& a, int t, int head, int d, int hi) {
   const int keys = 64 * a.split_tiles;
   if (hi <= keys || a.num_ranges == 1) return;  // a single range wrote the output itself
   const int nr = min((hi + keys - 1) / keys, a.num_ranges);
@@ -920,6 +1052,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int b
 #pragma unroll
     for (int k = 0; k < kMergeBatch; ++k) {
       const float wgt = r0 + k < nr && x[k].y != 0.f ? fast_exp2(x[k].x - M) : 0.f;
+      if (ODD && (r0 + k >= nr || x[k].y == 0.f)) continue;
       den = __builtin_fmaf(wgt, x[k].y, den);
 #pragma unroll
       for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(wgt, o[k][i], num[i]);
@@ -928,6 +1061,57 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int b
   const float inv = den > 0.f ? 1.f / den : 0.f;
   st8(reinterpret_cast<uint16_t*>(a.out) + (int64_t)t * a.o_st + (int64_t)head * a.o_sh + d,
       make_uint2(pack_bf16x2_hw(num[0] * inv, num[1] * inv), pack_bf16x2_hw(num[2] * inv, num[3] * inv)));
+}
+
+template <int D, int CB>
+__global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillArgs a, int blocks_per_token) {
+  constexpr int TPR = D / 4;  // threads per (token, head)
+  const int t = (int)blockIdx.x / blocks_per_token;
+  const int it = ((int)blockIdx.x - t * blocks_per_token) * 256 + (int)threadIdx.x;
+  // The token's sequence: the number of sequences that start at or before it, less one.
+  int s = -1;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    const int i = s0 + lane_id();
+    const bool before = i < a.num_seqs && a.query_start_loc[i] <= t;
+    s += __popcll(__builtin_amdgcn_ballot_w64(before));
+  }
+  const int head = it / TPR, d = 4 * (it - head * TPR);
+  if (s < 0 || head >= a.num_heads) return;
+  s = uniform(s);
+  const int q_start = a.query_start_loc[s], q_len = a.query_start_loc[s + 1] - q_start;
+  const int seq_len = a.seq_lens[s], ctx = a.context_lens[s];
+  if (t >= q_start + q_len || (q_len == 1 && a.single_query_seqs != 0)) return;
+  const int G = a.num_heads / a.num_kv_heads;
+  const int blk = ((t - q_start) * G + head % G) / CB;
+  const int q_last = (min(q_len * G, (blk + 1) * CB) - 1) / G;
+  const int hi = min(seq_len, ctx + q_last + 1);
+  merge_ranges<D>(a, t, head, d, hi);
+}
+
+// The same for the ranges of a step of windows.
+template <int D, int CB>
+__global__ __launch_bounds__(256) void window_prefill_merge_kernel(PrefillArgs a, int blocks_per_token, int window, int first_tokens) {
+  constexpr int TPR = D / 4;  // threads per (token, head)
+  const int t = (int)blockIdx.x / blocks_per_token;
+  const int it = ((int)blockIdx.x - t * blocks_per_token) * 256 + (int)threadIdx.x;
+  // The token's sequence: the number of sequences that start at or before it, less one.
+  int s = -1;
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 64) {
+    const int i = s0 + lane_id();
+    const bool before = i < a.num_seqs && a.query_start_loc[i] <= t;
+    s += __popcll(__builtin_amdgcn_ballot_w64(before));
+  }
+  const int head = it / TPR, d = 4 * (it - head * TPR);
+  if (s < 0 || head >= a.num_heads) return;
+  s = uniform(s);
+  const int q_start = a.query_start_loc[s], q_len = a.query_start_loc[s + 1] - q_start;
+  const int seq_len = a.seq_lens[s], ctx = a.context_lens[s];
+  if (t >= q_start + q_len || (q_len == 1 && a.single_query_seqs != 0)) return;
+  const int G = a.num_heads / a.num_kv_heads;
+  const int blk = ((t - q_start) * G + head % G) / CB;
+  const int q_last = (min(q_len * G, (blk + 1) * CB) - 1) / G;
+  const BlockWalk walk(ctx, seq_len, a.max_blocks, window, first_tokens, blk * CB / G, q_last);
+  merge_ranges<D, true>(a, t, head, d, walk.end);
 }
 
 // Decode view of a prefill batch: row b is sequence b; the decode work-group
@@ -1172,6 +1356,45 @@ hipError_t paged_prefill(const PrefillArgs& a, hipStream_t stream) {
   if (err != hipSuccess || a.row_part_out == nullptr || a.single_query_seqs == 0) return err;
   return decode_merge_chunks(single_query_view(a), stream);
 }
+
+// A step of windows: prefill work-groups of one of the forms above, and behind them those of the single rows.
+template <int D, int QT, int KS, bool SPL>
+static hipError_t launch_prefill_window(const PrefillArgs& a, const WindowRows& rows, hipStream_t stream) {
+  const PrefillGrid p = plan_prefill(a, 4 / KS * QT * 16);
+  const int64_t wgs = p.prefill_wgs * (SPL ? a.num_ranges : 1);
+  const int64_t row_wgs = a.single_query_seqs != 0 ? (decode_col_groups(rows.rows) * a.num_seqs * rows.rows.num_splits + 7) / 8 * 8 : 0;
+  if (wgs + row_wgs == 0) return hipSuccess;
+  if (wgs + row_wgs > 0x7ffffff0) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, SPL, false, true>), dim3((unsigned)(row_wgs + wgs)),
+                     dim3(4 * 64), 0, stream, a, (int)p.bound, p.dense_qb, p.xcd_group, (int)p.per_xcd, rows, (int)row_wgs,
+                     SPL ? a.num_ranges : 1);
+  hipError_t err = hipGetLastError();
+  if (err != hipSuccess || !SPL) return err;
+  const int per_token = (a.num_heads * (D / 4) + 255) / 256;
+  const int64_t blocks = (int64_t)a.num_tokens * per_token;
+  if (blocks > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((window_prefill_merge_kernel<D, 4 / KS * QT * 16>), dim3((unsigned)blocks), dim3(256), 0, stream, a,
+                     per_token, rows.window, rows.sinks);
+  return hipGetLastError();
+}
+
+template <int D, bool SPL>
+static hipError_t prefill_window_dim(const PrefillArgs& a, const WindowRows& rows, int columns, hipStream_t stream) {
+  if (columns == 128) return launch_prefill_window<D, 2, 1, SPL>(a, rows, stream);
+  if (columns == 64) return launch_prefill_window<D, 2, 2, SPL>(a, rows, stream);
+  return launch_prefill_window<D, 1, 2, SPL>(a, rows, stream);
+}
+
+hipError_t paged_prefill_window(const PrefillArgs& a, const WindowRows& rows, int columns, hipStream_t stream) {
+  const bool ranges = a.split_tiles > 0;
+  if (a.head_dim == 64)
+    return ranges ? prefill_window_dim<64, true>(a, rows, columns, stream) : prefill_window_dim<64, false>(a, rows, columns, stream);
+  if (a.head_dim == 128)
+    return ranges ? prefill_window_dim<128, true>(a, rows, columns, stream) : prefill_window_dim<128, false>(a, rows, columns, stream);
+  return hipErrorInvalidValue;
+}
+
+int64_t prefill_work_groups(const PrefillArgs& a, int columns) { return plan_prefill(a, columns).prefill_wgs; }
 
 // The device's own rule for the cut (find_row_chunk): no merge launch where it would
 // find nothing to do. And none where the longest row ends with the other sequences' blocks

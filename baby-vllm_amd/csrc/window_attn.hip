@@ -1,102 +1,96 @@
-// Attention of a sliding window and a few first tokens over the paged cache.
-//
-// The row at position p of its sequence (context_lens[s] + its number among the sequence's
-// rows) sees key j iff j <= p, j < seq_lens[s], j lies inside the table, and j > p - window or
-// j < sinks. Softmax over the visible keys as elsewhere; a row without one gives zeros.
-//
-// A row's visible pages are those of its first tokens, [0, sink_pages), and those of its
-// window, [first, end): walk step k is page k, or k + skip behind the first ones. Pages between
-// are not touched, whatever the table says of them.
-#include "paged_decode_wg.h"
+// Attention of a sliding window and a few first tokens over the paged cache: the launches of single rows
+// and the sum of their runs (window_attn.h); prompts run on the prefill kernel (paged_prefill.hip).
+#include "window_attn.h"
 
 #include <algorithm>
 
 namespace bvllm {
 
-namespace {
-
-// What a row sees: keys [0, sinks) and [lo, limit), on `count` pages.
-struct RowView {
-  int lo, sinks, limit;
-  int sink_pages, skip, count;
-  __device__ __forceinline__ RowView(int64_t pos, int seq_len, int max_blocks, int window, int first_tokens) {
-    limit = (int)max((int64_t)0, min(min(pos + 1, (int64_t)seq_len), (int64_t)16 * max_blocks));
-    lo = (int)max((int64_t)0, min(pos - window + 1, (int64_t)limit));
-    sinks = min(first_tokens, lo);
-    sink_pages = (sinks + 15) >> 4;
-    const int first = max(lo >> 4, sink_pages);
-    skip = first - sink_pages;
-    count = sink_pages + max(0, ((limit + 15) >> 4) - first);
-  }
-  __device__ __forceinline__ int page(int k) const { return k < sink_pages ? k : k + skip; }
-  __device__ __forceinline__ bool sees(int tok) const { return tok < limit && (tok >= lo || tok < sinks); }
-};
-
-// One work-group per (row, column group): its four waves take the row's visible pages in turn
-// and merge their states in LDS, as a decode row's.
-template <int D>
-__global__ __launch_bounds__(256) void window_rows_kernel(DecodeArgs a, int num_rows, int window, int first_tokens) {
-  constexpr int NW = 4, KC = D / 32, VD = D / 16;
-  __shared__ __attribute__((aligned(16))) unsigned char smem[decode_lds_bytes<D, NW>()];
-  const int G = a.num_heads / a.num_kv_heads;
-  const int ncg = a.num_kv_heads * col_groups_per_kv(G);
-  const int row = (int)blockIdx.x / ncg;
-  const ColGroup cg = col_group(G, (int)blockIdx.x - row * ncg);
-  const int lane = lane_id(), n = lane & 15, g = lane >> 4, w = wave_id();
-
-  // The row's sequence: the last one that starts at or before it.
-  int s = -1;
-  for (int s0 = 0; s0 < a.batch; s0 += 64) {
-    const int i = s0 + lane;
-    s += __popcll(__builtin_amdgcn_ballot_w64(i < a.batch && a.query_start_loc[i] <= row));
-  }
-  s = uniform(s);
-  if (s < 0 || row >= uniform(a.query_start_loc[s + 1])) return;
-  const int64_t pos = (int64_t)uniform(a.context_lens[s]) + (row - uniform(a.query_start_loc[s]));
-  const RowView view(pos, uniform(a.seq_lens[s]), a.max_blocks, window, first_tokens);
-
-  uint4 qb[KC];
-  const uint16_t* qrow = reinterpret_cast<const uint16_t*>(a.q) + (int64_t)row * a.q_sb + (int64_t)(cg.head0 + n) * a.q_sh;
-#pragma unroll
-  for (int c = 0; c < KC; ++c) qb[c] = n < cg.cols ? ld16(qrow + 8 * (4 * c + g)) : make_uint4(0, 0, 0, 0);
-
-  WaveState<D> st;
-  st.m = kNegInf;
-  st.l = 0.f;
-#pragma unroll
-  for (int c = 0; c < VD; ++c) st.acc[c] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  uint32_t off[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) off[j] = (uint32_t)((4 * g + j) * a.c_st + VD * n);
-  unsigned char* tile = smem + w * kTileBytes<D>;
-  const uint16_t* kc = reinterpret_cast<const uint16_t*>(a.k_cache) + (int64_t)cg.kvh * a.c_sh;
-  const uint16_t* vc = reinterpret_cast<const uint16_t*>(a.v_cache) + (int64_t)cg.kvh * a.c_sh;
-  const int32_t* bt = a.block_tables + (int64_t)s * a.bt_stride;
-
-  for (int k = w; k < view.count; k += NW) {
-    const int page = view.page(k);
-    const int64_t p = (int64_t)min(max(uniform(bt[page]), 0), a.num_pages - 1) * a.c_sb;
-    PageRegs<D> r;
-    load_page<D>(r, kc + p, vc + p, off);
-    wait_page<0, D>(r);
-    const f32x4_t scores = register_scores<D>(r, qb, tile, n, g);
-    PagePv<D> ph;
-    softmax_phase_if<D>(st, ph, scores, r.v, 16 * page + 4 * g, [&](int tok) { return view.sees(tok); }, a.scale_log2);
-    rescale_phase<D>(st, ph);
-    pv_phase<D>(st, ph);
-  }
-  float* merge = reinterpret_cast<float*>(smem + NW * kTileBytes<D>);
-  // (A NaN score: the sums hold it, and the merge's maximum, which passes over NaN, must not see none.)
-  if (st.m != st.m) st.m = 0.f;
-  save_state<D>(merge, st, w, lane);
-  __syncthreads();
-  merge_states<D>(a, merge, w, cg.cols, row, cg.head0, lane);
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64) void window_rows_kernel(WindowRows w) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  window_row_group<D, NW>(w.rows, w.window, w.sinks, (int)blockIdx.x, smem);
 }
 
-}  // namespace
+// Adds a row's runs: out = Σ 2^(lse_r − M)·o_r / Σ 2^(lse_r − M) in their order, one thread per 4 dims,
+// kMergeBatch runs' loads at once.
+constexpr int kMergeBatch = 8;
 
 template <int D>
-static hipError_t launch_window(const WindowArgs& w, hipStream_t stream) {
+__global__ __launch_bounds__(256) void window_merge_kernel(WindowRows w, int per_row) {
+  const DecodeArgs& a = w.rows;
+  const int b = (int)blockIdx.x / per_row;
+  const int it = ((int)blockIdx.x - b * per_row) * 256 + (int)threadIdx.x;
+  const int row = uniform(a.query_start_loc[b]), row_end = uniform(a.query_start_loc[b + 1]);
+  const int seq_len = uniform(a.seq_lens[b]), ctx = uniform(a.context_lens[b]);
+  if (row_end - row != 1) return;
+  const Runs runs(RowView(ctx, seq_len, a.max_blocks, w.window, w.sinks).count, a.num_splits);
+  const int head = it / (D / 4), d = 4 * (it - head * (D / 4));
+  if (runs.live == 1 || head >= a.num_heads) return;
+  const int64_t part = ((int64_t)b * a.num_heads + head) * a.num_splits;
+  float M = kNegInf, den = 0.f;
+  f32x4_t num = {0.f, 0.f, 0.f, 0.f};
+  for (int r0 = 0; r0 < runs.live; r0 += kMergeBatch) {
+    float lse[kMergeBatch];
+    f32x4_t o[kMergeBatch];
+#pragma unroll
+    for (int k = 0; k < kMergeBatch; ++k) {
+      const int64_t p = part + min(r0 + k, runs.live - 1);
+      lse[k] = a.part_lse[p];
+      o[k] = *reinterpret_cast<const f32x4_t*>(a.part_out + p * D + d);
+    }
+    float Mb = M;
+#pragma unroll
+    for (int k = 0; k < kMergeBatch; ++k) Mb = fmaxf(Mb, lse[k]);
+    const float ref = Mb == kNegInf ? 0.f : Mb;
+    const float alpha = fast_exp2(M - ref);
+    den *= alpha;
+    num *= alpha;
+    M = Mb;
+#pragma unroll
+    for (int k = 0; k < kMergeBatch; ++k) {
+      const float wgt = r0 + k < runs.live ? fast_exp2(lse[k] - ref) : 0.f;
+      den += wgt;
+      if (r0 + k < runs.live) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) num[i] = __builtin_fmaf(wgt, o[k][i], num[i]);
+      }
+    }
+  }
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  st8(reinterpret_cast<uint16_t*>(a.out) + (int64_t)row * a.o_sb + (int64_t)head * a.o_sh + d,
+      make_uint2(pack_bf16x2_hw(num[0] * inv, num[1] * inv), pack_bf16x2_hw(num[2] * inv, num[3] * inv)));
+}
+
+// How the single rows of a step are cut: work-groups of `waves` waves, `splits` of them per (row, column group).
+// Times (us) as measured here, rows of equal length: 5 of start, with 0.18 per page of a work-group at
+// D = 128 (the waves of a work-group share what a CU takes: 4, 8 or 16 of them make no difference) and
+// 0.09 at D = 64 (0.14 on four waves), and 2.3 of the second launch. So rows are cut until every CU has a
+// work-group, into runs of 8 pages at least, where that saves more than the second launch costs (one row
+// of 7B, 4097 keys: 46.4 whole, 11.2 in 32 runs; 1025: 14.2 and 8.7; 257: 6.0 and 7.4. 32 rows, 1025:
+// 18.6 and 18.3. 48 rows, 4097, a work-group per CU but 64 idle: 70.3 and 76.2). Eight waves at D = 64 but for
+// a few pages (64 keys: 4.5 against 4.4), and at D = 128 while half of the CUs are idle (one row, 1025
+// keys: 8.7 against 9.0); else four (64 rows, 1025: 24.8 against 25.1, 96 rows: 39.4 against 41.2).
+constexpr int64_t kMaxRowBytes = 64ll << 20;  // of their partials
+
+struct RowPlan {
+  int waves, splits;
+};
+
+static RowPlan row_plan(const WindowArgs& a, int64_t rows, int64_t max_bytes) {
+  const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)a.window + 15) / 16 + 1 + ((int64_t)a.sinks + 15) / 16);
+  const int G = a.num_heads / a.num_kv_heads;
+  const int64_t units = std::max<int64_t>(1, rows * a.num_kv_heads * ((G + 15) / 16)), cus = device_cus();
+  const int64_t room = max_bytes / ((int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4);
+  const int64_t splits = std::min({cus / units, pages / 8, room});
+  RowPlan p{4, 1};
+  if (splits > 1 && (a.head_dim == 128 ? 0.18 : 0.09) * (double)(pages - (pages + splits - 1) / splits) > 3.5)
+    p.splits = (int)splits;
+  p.waves = a.head_dim == 64 ? (pages < 8 ? 4 : 8) : (2 * units * p.splits <= cus ? 8 : 4);
+  return p;
+}
+
+static DecodeArgs rows_of_step(const WindowArgs& w) {
   DecodeArgs a{};
   a.q = w.q; a.q_sb = w.q_st; a.q_sh = w.q_sh;
   a.k_cache = w.k_cache; a.v_cache = w.v_cache;
@@ -107,13 +101,138 @@ static hipError_t launch_window(const WindowArgs& w, hipStream_t stream) {
   a.scale_log2 = w.scale_log2;
   a.out = w.out; a.o_sb = w.o_st; a.o_sh = w.o_sh;
   a.batch = w.num_seqs; a.num_heads = w.num_heads; a.num_kv_heads = w.num_kv_heads; a.head_dim = w.head_dim;
-  const int64_t wgs = (int64_t)w.num_tokens * decode_col_groups(a);
+  return a;
+}
+
+template <int D, int NW>
+static hipError_t launch_rows(const WindowRows& w, hipStream_t stream) {
+  const DecodeArgs& a = w.rows;
+  const int G = a.num_heads / a.num_kv_heads;
+  const int64_t wgs = (int64_t)a.batch * decode_col_groups(a) * a.num_splits;
   if (wgs > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((window_rows_kernel<D>), dim3((unsigned)wgs), dim3(256), 0, stream, a, w.num_tokens, w.window, w.sinks);
+  static std::atomic<bool> done[64] = {};
+  hipError_t err = allow_lds(&window_rows_kernel<D, NW>, done, (int)rows_lds_bytes<D, NW>(16));
+  if (err != hipSuccess) return err;
+  const size_t lds = rows_lds_bytes<D, NW>(std::min(G, 16));
+  hipLaunchKernelGGL((window_rows_kernel<D, NW>), dim3((unsigned)wgs), dim3(NW * 64), lds, stream, w);
   return hipGetLastError();
 }
 
-int64_t window_workspace_bytes(const WindowArgs&) { return 0; }
+static PrefillArgs blocks_of_step(const WindowArgs& w) {
+  PrefillArgs a{};
+  a.q = w.q; a.q_st = w.q_st; a.q_sh = w.q_sh;
+  a.k_cache = w.k_cache; a.v_cache = w.v_cache;
+  a.c_sb = w.c_sb; a.c_st = w.c_st; a.c_sh = w.c_sh;
+  a.num_pages = w.num_pages;
+  a.block_tables = w.block_tables; a.bt_stride = w.bt_stride; a.max_blocks = w.max_blocks;
+  a.query_start_loc = w.query_start_loc; a.seq_lens = w.seq_lens; a.context_lens = w.context_lens;
+  a.scale_log2 = w.scale_log2;
+  a.out = w.out; a.o_st = w.o_st; a.o_sh = w.o_sh;
+  a.num_seqs = w.num_seqs; a.num_tokens = w.num_tokens; a.max_query_len = w.max_query_len;
+  a.num_heads = w.num_heads; a.num_kv_heads = w.num_kv_heads; a.head_dim = w.head_dim;
+  a.single_query_seqs = w.single_query_seqs;
+  return a;
+}
+
+// How a step runs: its single rows, the columns of its prefill blocks, the ranges (of split_tiles tiles, 0: none) that
+// these are walked in.
+struct WindowPlan {
+  RowPlan rows;
+  int columns, split_tiles, num_ranges;
+  int64_t row_floats, range_floats;  // of their partials
+};
+
+// What a launch of the blocks takes (us), fitted to 9,232 random steps (prompts of 2 to 8192 tokens of up to 64 sequences
+// behind up to 16,000, windows of 32 to 8192, 7B and 0.5B heads; rms 19%): a start, and per tile of a walk less with one
+// work-group per CU than with two; every further round of two per CU has its own start. Ranges
+// add a launch and their partials' bytes. Of the forms below, the best by these takes 1.02 times the best as measured on
+// average, 1.24 in one step of 100 (128 columns without ranges always: 1.18, 64 or 32: 1.25).
+struct BlockCost {
+  double start, tile_one, tile_two, round;
+};
+constexpr BlockCost kBlockCost[2][3] = {
+    {{5.8, 1.20, 1.43, 3.6}, {7.2, 0.64, 0.73, 4.9}, {6.5, 0.50, 0.53, 4.0}},   // D = 64: 128, 64, 32 columns
+    {{7.0, 1.41, 1.93, 5.9}, {9.0, 0.83, 1.03, 6.9}, {7.5, 0.65, 0.69, 5.3}}};  // D = 128
+constexpr double kRangeLaunch = 4.9, kRangeBytesPerUs = 16e6;
+constexpr int64_t kMaxRangeBytes = 64ll << 20;  // of the ranges' partials
+
+static void plan_blocks(const WindowArgs& w, WindowPlan& p) {
+  const PrefillArgs a = blocks_of_step(w);
+  const int64_t group = a.num_heads / a.num_kv_heads, cus = device_cus();
+  const int64_t range_bytes = prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4;
+  double best = 0;
+  for (int form = 0; form < 3; ++form) {
+    const int columns = 128 >> form;
+    const BlockCost& c = kBlockCost[a.head_dim == 128][form];
+    // The longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
+    const int64_t rows = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
+    const int64_t pages = std::min<int64_t>(a.max_blocks, (w.window + rows + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
+    const int64_t tiles = (pages + 3) / 4, blocks = prefill_work_groups(a, columns);
+    for (int64_t split : {0, 4, 8, 12, 16, 24, 32}) {
+      if (split >= tiles) break;
+      const int64_t ranges = split > 0 ? (tiles + split - 1) / split : 1;
+      if (ranges > 1 && ranges * range_bytes > kMaxRangeBytes) continue;
+      const double walk = (double)(split > 0 ? split : tiles);
+      const int64_t full = blocks * ranges / (2 * cus), rest = blocks * ranges - full * 2 * cus;
+      double t = c.start - c.round + (double)full * (c.round + c.tile_two * walk);
+      if (rest > 0) t += c.round + (rest > cus ? c.tile_two : c.tile_one) * walk;
+      if (split > 0) t += kRangeLaunch + 2.0 * (double)(ranges * range_bytes) / kRangeBytesPerUs;
+      if (best == 0 || t < best) {
+        best = t;
+        p.columns = columns;
+        p.split_tiles = (int)split;
+        p.num_ranges = (int)ranges;
+      }
+    }
+  }
+}
+
+static WindowPlan window_plan(const WindowArgs& a) {
+  WindowPlan p{{4, 1}, 128, 0, 1, 0, 0};
+  if (a.max_query_len == 1) p.rows = row_plan(a, std::min(a.num_tokens, a.num_seqs), kMaxRowBytes);
+  else plan_blocks(a, p);
+  // (The ranges' partials, behind the rows', are 16-byte aligned.)
+  if (p.rows.splits > 1) p.row_floats = ((int64_t)a.num_seqs * a.num_heads * p.rows.splits * (a.head_dim + 1) + 3) / 4 * 4;
+  if (p.split_tiles > 0) p.range_floats = prefill_range_floats(p.num_ranges, a.num_tokens, a.num_heads, a.head_dim);
+  return p;
+}
+
+template <int D>
+static hipError_t launch_window(const WindowArgs& w, hipStream_t stream) {
+  WindowPlan p = window_plan(w);
+  if (w.workspace == nullptr) {
+    p.rows.splits = 1;
+    p.split_tiles = 0;
+    p.num_ranges = 1;
+    p.row_floats = 0;
+  }
+  WindowRows r{rows_of_step(w), w.window, w.sinks};
+  float* ws = reinterpret_cast<float*>(w.workspace);
+  r.rows.num_splits = p.rows.splits;
+  r.rows.part_out = ws;
+  r.rows.part_lse = ws + (int64_t)w.num_seqs * w.num_heads * p.rows.splits * D;
+  hipError_t err;
+  if (w.max_query_len == 1) {
+    err = p.rows.waves == 4 ? launch_rows<D, 4>(r, stream) : launch_rows<D, 8>(r, stream);
+  } else {
+    PrefillArgs a = blocks_of_step(w);
+    a.split_tiles = p.split_tiles;
+    a.num_ranges = p.num_ranges;
+    a.part_out = ws + p.row_floats;
+    a.part_ml = a.part_out + (int64_t)p.num_ranges * w.num_tokens * w.num_heads * D;
+    err = paged_prefill_window(a, r, p.columns, stream);
+  }
+  if (err != hipSuccess || p.rows.splits == 1 || w.single_query_seqs == 0) return err;
+  const int per_row = (w.num_heads * (D / 4) + 255) / 256;
+  if ((int64_t)w.num_seqs * per_row > 0x7fffffff) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((window_merge_kernel<D>), dim3((unsigned)(w.num_seqs * per_row)), dim3(256), 0, stream, r, per_row);
+  return hipGetLastError();
+}
+
+int64_t window_workspace_bytes(const WindowArgs& a) {
+  const WindowPlan p = window_plan(a);
+  return 4 * (p.row_floats + p.range_floats);
+}
 
 hipError_t paged_window_attention(const WindowArgs& a, hipStream_t stream) {
   switch (a.head_dim) {
