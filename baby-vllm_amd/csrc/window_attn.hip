@@ -77,8 +77,13 @@ struct RowPlan {
   int waves, splits;
 };
 
+// The pages that a row can see at most.
+static int64_t max_row_pages(const WindowArgs& a) {
+  return std::min<int64_t>(a.max_blocks, ((int64_t)a.window + 15) / 16 + 1 + ((int64_t)a.sinks + 15) / 16);
+}
+
 static RowPlan row_plan(const WindowArgs& a, int64_t rows, int64_t max_bytes) {
-  const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)a.window + 15) / 16 + 1 + ((int64_t)a.sinks + 15) / 16);
+  const int64_t pages = max_row_pages(a);
   const int G = a.num_heads / a.num_kv_heads;
   const int64_t units = std::max<int64_t>(1, rows * a.num_kv_heads * ((G + 15) / 16)), cus = device_cus();
   const int64_t room = max_bytes / ((int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4);
@@ -156,17 +161,26 @@ constexpr BlockCost kBlockCost[2][3] = {
 constexpr double kRangeLaunch = 4.9, kRangeBytesPerUs = 16e6;
 constexpr int64_t kMaxRangeBytes = 64ll << 20;  // of the ranges' partials
 
+// The step's single rows run beside the blocks, on four waves a run: 5 us and 0.18 (D = 128) or 0.14 per page. Where they
+// would take longer than the blocks they are cut, for a launch that adds their runs (4.5 us with its partials; 6 rows of
+// 2140 to 8560 keys beside prompts of 3 to 5 tokens 87 -> 33 us).
+constexpr double kRunLaunch = 4.5;
+
 static void plan_blocks(const WindowArgs& w, WindowPlan& p) {
   const PrefillArgs a = blocks_of_step(w);
   const int64_t group = a.num_heads / a.num_kv_heads, cus = device_cus();
   const int64_t range_bytes = prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4;
+  const int64_t row_pages = max_row_pages(w);
+  const int64_t rows = w.single_query_seqs >= 0 ? w.single_query_seqs : w.num_seqs;
+  const int64_t units = rows * a.num_kv_heads * ((group + 15) / 16);
+  const int64_t row_bytes = (int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4;
   double best = 0;
   for (int form = 0; form < 3; ++form) {
     const int columns = 128 >> form;
     const BlockCost& c = kBlockCost[a.head_dim == 128][form];
     // The longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
-    const int64_t rows = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
-    const int64_t pages = std::min<int64_t>(a.max_blocks, (w.window + rows + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
+    const int64_t span = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
+    const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
     const int64_t tiles = (pages + 3) / 4, blocks = prefill_work_groups(a, columns);
     for (int64_t split : {0, 4, 8, 12, 16, 24, 32}) {
       if (split >= tiles) break;
@@ -177,11 +191,18 @@ static void plan_blocks(const WindowArgs& w, WindowPlan& p) {
       double t = c.start - c.round + (double)full * (c.round + c.tile_two * walk);
       if (rest > 0) t += c.round + (rest > cus ? c.tile_two : c.tile_one) * walk;
       if (split > 0) t += kRangeLaunch + 2.0 * (double)(ranges * range_bytes) / kRangeBytesPerUs;
-      if (best == 0 || t < best) {
-        best = t;
-        p.columns = columns;
-        p.split_tiles = (int)split;
-        p.num_ranges = (int)ranges;
+      for (int64_t runs = 1; runs <= 16; runs *= 2) {
+        if (runs > 1 && (units * runs + blocks * ranges > 2 * cus || row_pages < 8 * runs || runs * row_bytes > kMaxRowBytes)) break;
+        const double row = 5 + (a.head_dim == 128 ? 0.18 : 0.14) * (double)((row_pages + runs - 1) / runs);
+        const double both = rows > 0 ? std::max(t, row) + (runs > 1 ? kRunLaunch : 0) : t;
+        if (best == 0 || both < best) {
+          best = both;
+          p.columns = columns;
+          p.split_tiles = (int)split;
+          p.num_ranges = (int)ranges;
+          p.rows.splits = (int)runs;
+        }
+        if (rows == 0) break;
       }
     }
   }
