@@ -596,6 +596,7 @@ extern "C" int bvllm_build_step_tables(const int32_t* query_lens, const int32_t*
   a.pad_page = pad_page;
   a.block_tables = block_tables; a.query_start_loc = query_start_loc; a.seq_lens = seq_lens;
   a.positions = positions; a.slot_mapping = slot_mapping;
+  a.vec_ok = aligned16(block_tables);
   return (int)build_step_tables(a, (hipStream_t)stream);
 }
 

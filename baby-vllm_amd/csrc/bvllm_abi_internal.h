@@ -225,6 +225,7 @@ struct StepTablesArgs {
   int32_t window, kept_pages;              // window 0: none; pages of the first tokens that stay
   int32_t pad_page;
   int32_t* block_tables;                   // [S, width], contiguous
+  bool vec_ok;                             // 16-byte aligned
   int32_t* query_start_loc;                // [S + 1]
   int32_t* seq_lens;                       // [S]
   int64_t* positions;                      // [num_tokens]
