@@ -3,7 +3,9 @@
 ``ModelConfig`` carries the Qwen2 architecture fields the reference reads from
 a checkpoint's config.json. There is no network here, so besides
 ``from_hf(path)`` (a local directory) the two shapes the benchmarks use are
-available as presets: ``qwen2_5_7b()`` and ``qwen2_5_0_5b()``.
+available as presets: ``qwen2_5_7b()`` and ``qwen2_5_0_5b()``. ``sliding_window``,
+``attention_sinks`` and ``qk_norm`` are this build's own: set them on a config for a
+model with those; ``from_hf`` and the presets leave them off.
 """
 
 from __future__ import annotations
@@ -26,6 +28,11 @@ class ModelConfig:
     rope_theta: float
     tie_word_embeddings: bool
     block_size: int = 16
+    # Of models whose layers attend a sliding window and the first `attention_sinks` tokens (None: all
+    # keys), and that normalise every query and key head before the rotation.
+    sliding_window: int | None = None
+    attention_sinks: int = 0
+    qk_norm: bool = False
 
     @property
     def head_dim(self) -> int:

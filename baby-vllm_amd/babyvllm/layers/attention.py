@@ -4,8 +4,9 @@ Mirrors ``Attention`` of babyvllm/layers/attention.py:35-68: with a forward
 context and a cache, a step whose ``max_query_len == 1`` runs
 ``paged_decode_attention`` (with ``max_seq_len`` = the step's context bucket),
 any longer step runs ``paged_prefill_attention``; a step with a ``tree_mask`` (drafted
-token trees, not in the reference) runs ``paged_tree_attention``. This build has no torch
-attention path: a call on a non-ROCm tensor, without a KV cache or without a
+token trees, not in the reference) runs ``paged_tree_attention``. A layer with a ``window``
+(not in the reference) runs ``paged_window_attention`` for every step but those trees, which it
+refuses. This build has no torch attention path: a call on a non-ROCm tensor, without a KV cache or without a
 forward context raises instead of silently computing elsewhere.
 
 ``BABYVLLM_PREFILL_ATTN`` is the reference's switch for multi-token steps
@@ -30,13 +31,16 @@ class Attention(nn.Module):
     """Paged attention over a flattened (varlen) token batch."""
 
     def __init__(self, num_heads: int, head_dim: int, num_kv_heads: int,
-                 scale: float | None = None):
+                 scale: float | None = None, window: int | None = None, sinks: int = 0):
         super().__init__()
+        if (window is not None and window < 1) or sinks < 0:
+            raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
         self.num_queries_per_kv = num_heads // num_kv_heads
         self.scale = scale if scale is not None else head_dim ** -0.5
+        self.window, self.sinks = window, sinks
         self.kv_cache = None
 
     def forward(self, q, k, v):
@@ -49,8 +53,13 @@ class Attention(nn.Module):
             raise RuntimeError(f"Attention runs only on a ROCm device, got {q.device}")
         md = ctx.attn_metadata
         if getattr(md, "tree_mask", None) is not None:
+            if self.window is not None:
+                raise RuntimeError("drafted token trees attend all keys: not for a layer with a window")
             from babyvllm.kernels.tree_attn import paged_tree_attention
             return paged_tree_attention(q, self.kv_cache, md, self.scale)
+        if self.window is not None:
+            from babyvllm.kernels.window_attn import paged_window_attention
+            return paged_window_attention(q, self.kv_cache, md, self.scale, self.window, self.sinks)
         if md.max_query_len == 1 and self.kv_cache.shape[2] >= 16:
             from babyvllm.kernels.paged_attn import paged_decode_attention
             return paged_decode_attention(q, self.kv_cache, md.block_tables, md.seq_lens,

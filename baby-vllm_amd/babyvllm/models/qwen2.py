@@ -9,6 +9,11 @@ paged cache through the step's slot_mapping), paged attention (HIP decode or pre
 kernel), the output GEMM, add + RMSNorm, the gate/up GEMM, SiLU·mul and the down
 GEMM. Steps of few tokens (decode) run the GEMMs on the HIP kernel, gate/up with
 SiLU·mul in its epilogue; the others on hipBLASLt through torch, with the HIP SiLU·mul.
+
+Two things that the reference's model does not have: with ``cfg.qk_norm`` every query and key
+head is normalised (``self_attn.q_norm``, ``k_norm``) by the launch that rotates and appends
+it, and with ``cfg.sliding_window`` the layers attend that window and ``cfg.attention_sinks``
+first tokens.
 """
 
 from __future__ import annotations
@@ -22,6 +27,7 @@ import torch.nn.functional as F
 from babyvllm.kernels.activation import fused_silu_mul
 from babyvllm.kernels.embed import embed_rows
 from babyvllm.kernels.linear import gated_linear, skinny_linear
+from babyvllm.kernels.qk_norm_rope import fused_qk_norm_rope_and_cache
 from babyvllm.kernels.rope import fused_rope_and_cache
 from babyvllm.layers.attention import Attention
 from babyvllm.layers.layernorm import RMSNorm
@@ -65,7 +71,12 @@ class Qwen2Attention(nn.Module):
         self.kv_size = self.num_kv_heads * self.head_dim
         self.qkv_proj = Linear(cfg.hidden_size, self.q_size + 2 * self.kv_size, bias=True)
         self.o_proj = Linear(self.q_size, cfg.hidden_size, bias=False)
-        self.attn = Attention(self.num_heads, self.head_dim, self.num_kv_heads)
+        self.attn = Attention(self.num_heads, self.head_dim, self.num_kv_heads, window=cfg.sliding_window,
+                              sinks=cfg.attention_sinks)
+        self.q_norm = self.k_norm = None
+        if cfg.qk_norm:
+            self.q_norm = RMSNorm(self.head_dim, eps=cfg.rms_norm_eps)
+            self.k_norm = RMSNorm(self.head_dim, eps=cfg.rms_norm_eps)
 
     def forward(self, x, cos, sin):
         qkv = self.qkv_proj(x)
@@ -76,8 +87,12 @@ class Qwen2Attention(nn.Module):
         ctx = get_forward_context()
         if ctx is None or self.attn.kv_cache is None:
             raise RuntimeError("Qwen2Attention needs a KV cache and a forward context")
-        q, k = fused_rope_and_cache(q, k, v, cos, sin, kv_cache=self.attn.kv_cache,
-                                    slot_mapping=ctx.attn_metadata.slot_mapping)
+        slots = ctx.attn_metadata.slot_mapping
+        if self.q_norm is not None:
+            q = fused_qk_norm_rope_and_cache(q, k, v, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps, cos, sin,
+                                             self.attn.kv_cache, slots)
+        else:
+            q, k = fused_rope_and_cache(q, k, v, cos, sin, kv_cache=self.attn.kv_cache, slot_mapping=slots)
         o = self.attn(q, k, v)
         return self.o_proj(o.reshape(-1, self.q_size))
 

@@ -14,8 +14,8 @@
   edited in place) by a single non-blocking copy into a device buffer of the
   same layout, which every captured graph reads; the attention kernels see
   ``max_seq_len`` = the context bucket, so the captured grid fits every replay.
-* Any other step runs eagerly with metadata built from the scheduler output,
-  then takes each sequence's last row of hidden states to the LM head.
+* Any other step runs eagerly with metadata built from the scheduler output (its
+  lengths and pages in one copy, tables and slots on the GPU), then takes each sequence's last row of hidden states to the LM head.
 Greedy requests (temperature 0) are sampled with the HIP argmax kernel;
 others with torch softmax / top-p / multinomial on the host side of the path.
 """
@@ -28,6 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from babyvllm.kernels.argmax import greedy_argmax
+from babyvllm.kernels.step_tables import build_step_tables
 from babyvllm.layers.attention import Attention
 from babyvllm.models.qwen2 import Qwen2ForCausalLM
 from babyvllm.worker.context import AttentionMetadata, set_forward_context
@@ -137,19 +138,29 @@ class ModelRunner:
             check_inputs(ids, max(seq_lens) - 1, self.model.model.table_sizes())
         width = max(len(t) for t in tables)
         dev = self.device
+        host = dict(query_start_loc_cpu=qsl, seq_lens_cpu=seq_lens, context_lens_cpu=ctx_lens,
+                    max_query_len=max(qsl[i + 1] - qsl[i] for i in range(len(tables))), max_seq_len=max(seq_lens))
+        input_ids = torch.tensor(ids, dtype=torch.int64, device=dev)
+        if dev.type == "cuda" and self.block_size == 16:
+            # Lengths and pages go over in one copy; the GPU makes the tables, slots and positions of them.
+            n = len(tables)
+            packed = [b - a for a, b in zip(qsl, qsl[1:])] + ctx_lens
+            for t, length in zip(tables, seq_lens):
+                packed += t[:-(-length // 16)]
+            packed = torch.tensor(packed, dtype=torch.int32, device=dev)
+            ctx = packed[n:2 * n]
+            step = build_step_tables(packed[:n], ctx, packed[2 * n:], len(ids), width)
+            return input_ids, step.positions, AttentionMetadata(
+                slot_mapping=step.slot_mapping, block_tables=step.block_tables, query_start_loc=step.query_start_loc,
+                seq_lens=step.seq_lens, context_lens=ctx, **host)
         md = AttentionMetadata(
             slot_mapping=torch.tensor(slots, dtype=torch.int64, device=dev),
             block_tables=torch.tensor([t + [0] * (width - len(t)) for t in tables], dtype=torch.int32,
                                       device=dev),
             query_start_loc=torch.tensor(qsl, dtype=torch.int32, device=dev),
             seq_lens=torch.tensor(seq_lens, dtype=torch.int32, device=dev),
-            context_lens=torch.tensor(ctx_lens, dtype=torch.int32, device=dev),
-            query_start_loc_cpu=qsl, seq_lens_cpu=seq_lens, context_lens_cpu=ctx_lens,
-            max_query_len=max(qsl[i + 1] - qsl[i] for i in range(len(tables))),
-            max_seq_len=max(seq_lens),
-        )
-        return (torch.tensor(ids, dtype=torch.int64, device=dev),
-                torch.tensor(positions, dtype=torch.int64, device=dev), md)
+            context_lens=torch.tensor(ctx_lens, dtype=torch.int32, device=dev), **host)
+        return input_ids, torch.tensor(positions, dtype=torch.int64, device=dev), md
 
     def _sample(self, logits, seqs) -> dict[int, int]:
         tokens = torch.empty(logits.shape[0], dtype=torch.int64, device=logits.device)
