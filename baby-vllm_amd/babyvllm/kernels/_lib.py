@@ -175,7 +175,8 @@ SIGNATURES = {
         _i32, _i32, _i32, _i32,     # T, H, Hkv, D
         _p,                         # stream
     ]),
-    "bvllm_window_workspace_bytes": (ctypes.c_int64, [_i32] * 10),
+    "bvllm_window_plan": (ctypes.c_int, [_i32] * 10 + [_p]),
+    "bvllm_window_workspace_bytes": (ctypes.c_int64, [_i32] * 6),
     "bvllm_paged_window_attention": (ctypes.c_int, [
         _p, _i64, _i64,             # q
         _p, _p, _i64, _i64, _i64,   # caches + strides
@@ -186,7 +187,8 @@ SIGNATURES = {
         _p, _i64, _i64,             # out
         _i32, _i32, _i32, _i32,     # num_seqs, num_tokens, max_query_len, single_query_seqs
         _i32, _i32, _i32, _i32,     # H, Hkv, D, block_size
-        _p, _p,                     # workspace, stream
+        _p, _i32, _i32, _i32, _i32,  # workspace, columns, split_tiles, num_ranges, row_runs
+        _p,                         # stream
     ]),
 }
 

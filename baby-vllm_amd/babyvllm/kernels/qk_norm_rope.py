@@ -31,7 +31,7 @@ def fused_qk_norm_rope_and_cache(q, k, v, q_weight, k_weight, eps, cos, sin, kv_
 
     ``q_weight`` and ``k_weight``: ``[D]`` vectors, both bf16 or both fp32. ``cos`` and ``sin``:
     ``[T, D]`` per-token rows (duplicated halves), both bf16 or both fp32. ``out``: where q
-    goes, ``q`` itself among others; a tensor of other memory than q, k and v.
+    goes: ``q`` itself, or a tensor that shares no memory with the others.
     """
     if out is None and q.is_cuda:
         got = _lib.fast().norm_rope(q, k, v, q_weight, k_weight, eps, cos, sin, kv_cache, slot_mapping, *_lib.current())
@@ -79,8 +79,9 @@ def fused_qk_norm_rope_and_cache(q, k, v, q_weight, k_weight, eps, cos, sin, kv_
         if any(n > 1 and step == 0 for n, step in zip(out.shape, out.stride())):
             raise ValueError("out's elements must not share memory")
         in_place = out.data_ptr() == q.data_ptr() and out.stride() == q.stride()
-        if num_tokens and not in_place and any(_overlap(out, t) for t in (q, k, v)):
-            raise ValueError("out must be q itself or share no memory with q, k and v")
+        others = (q_weight, k_weight, cos, sin, kv_cache, slot_mapping)
+        if num_tokens and any(_overlap(out, t) for t in (others if in_place else (q, k, v) + others)):
+            raise ValueError("out must be q itself or share no memory with the other tensors")
     if num_tokens == 0:
         return out
     slot_mapping = slot_mapping.contiguous()

@@ -23,6 +23,7 @@ width or negative has slot -1; negative lengths count as 0.
 
 from __future__ import annotations
 
+import operator
 from typing import NamedTuple
 
 import torch
@@ -58,7 +59,8 @@ def build_step_tables(query_lens, context_lens, pages, num_tokens, width, *, win
     num_seqs = query_lens.shape[0]
     if context_lens.shape[0] != num_seqs:
         raise ValueError(f"context_lens has {context_lens.shape[0]} requests, query_lens {num_seqs}")
-    num_tokens, width = int(num_tokens), int(width)
+    num_tokens, width, sinks, pad_page = (operator.index(v) for v in (num_tokens, width, sinks, pad_page))
+    window = None if window is None else operator.index(window)
     if not 0 <= num_tokens < 2**31 or not 1 <= width <= _MAX_WIDTH:
         raise ValueError(f"num_tokens must be from 0 to 2^31 - 1 and width from 1 to 2^28, got {num_tokens} and {width}")
     if not -2**31 <= pad_page < 2**31:
@@ -76,7 +78,7 @@ def build_step_tables(query_lens, context_lens, pages, num_tokens, width, *, win
     with torch.cuda.device(device):
         rc = _lib.lib().bvllm_build_step_tables(
             query_lens.data_ptr(), context_lens.data_ptr(), num_seqs, pages.data_ptr(), pages.shape[0],
-            0 if window is None else min(int(window), 2**31 - 1), min(int(sinks), 2**31 - 1), int(pad_page),
+            0 if window is None else min(window, 2**31 - 1), min(sinks, 2**31 - 1), pad_page,
             out.block_tables.data_ptr(), width, out.query_start_loc.data_ptr(), out.seq_lens.data_ptr(),
             out.positions.data_ptr(), out.slot_mapping.data_ptr(), num_tokens, 16, _lib.stream_handle(device))
     _lib.check(rc, "bvllm_build_step_tables")

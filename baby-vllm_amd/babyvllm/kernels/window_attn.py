@@ -11,9 +11,18 @@ Pages that no row of a sequence sees are not read for a result: their table entr
 page (``build_step_tables`` with the same ``window`` and ``sinks`` leaves them out), so that a
 cache can give them back. A row that sees no key gives zeros, and a key that a row does not see
 does not reach it, whatever it holds. Rows of ``q`` behind the last sequence are not computed.
+
+``md.max_query_len`` bounds the query rows of every sequence. Few rows behind long windows are cut over more
+work-groups, chosen from host sizes and (outside a capture) the list ``md.query_start_loc_cpu``: the last bits of a row can
+depend on the other sequences of the step. That takes fp32 scratch (at most 128 MiB); without the memory
+for it the launch that needs none runs. Scores, softmax statistics and sums are fp32; the weights are rounded to bf16, as in
+``paged_prefill_attention``.
 """
 
 from __future__ import annotations
+
+import ctypes
+import operator
 
 import torch
 
@@ -25,10 +34,12 @@ _MAX = 2**31 - 1
 
 def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
     """``[T, H, D]`` attention of the step's rows, K/V read from the paged cache."""
+    # (A captured step is replayed with other sequences than its host lists': they do not steer it.)
+    host_lists = not (q.is_cuda and torch._C._cuda_isCurrentStreamCapturing())
     if q.is_cuda:
         out = _lib.fast().window(q, kv_cache, md.block_tables, md.query_start_loc, md.seq_lens, md.context_lens,
-                                 getattr(md, "query_start_loc_cpu", None), md.max_query_len, scale, window, sinks,
-                                 *_lib.current())
+                                 getattr(md, "query_start_loc_cpu", None) if host_lists else None, md.max_query_len,
+                                 scale, window, sinks, *_lib.current())
         if out is not None:
             return out
     for name, t in (("q", q), ("kv_cache", kv_cache), ("block_tables", md.block_tables),
@@ -37,6 +48,7 @@ def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
         _lib.require_rocm_tensor(name, t)
         if t.device != q.device:
             raise RuntimeError(f"{name} is on {t.device}, q on {q.device}")
+    window, sinks = min(operator.index(window), _MAX), min(operator.index(sinks), _MAX)
     if window < 1 or sinks < 0:
         raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
     if q.dim() != 3 or q.stride(-1) != 1:
@@ -70,12 +82,16 @@ def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
         return out
     qsl, seq_lens, ctx_lens = md.query_start_loc.contiguous(), md.seq_lens.contiguous(), md.context_lens.contiguous()
     h = _lib.lib()
-    window, sinks = min(int(window), _MAX), min(int(sinks), _MAX)
-    single = _single_query_seqs(md, num_seqs) if max_query_len > 1 else -1
+    single = _single_query_seqs(md, num_seqs) if max_query_len > 1 and host_lists else -1
     with torch.cuda.device(q.device):
-        nbytes = h.bvllm_window_workspace_bytes(num_seqs, num_tokens, max_query_len, single, num_heads, num_kv_heads,
-                                                head_dim, bt.shape[1], window, sinks)
+        plan = (ctypes.c_int32 * 4)()
+        _lib.check(h.bvllm_window_plan(num_seqs, num_tokens, max_query_len, single, num_heads, num_kv_heads, head_dim,
+                                       bt.shape[1], window, sinks, plan), "bvllm_window_plan")
+        columns, split_tiles, num_ranges, row_runs = plan
+        nbytes = h.bvllm_window_workspace_bytes(num_seqs, num_tokens, num_heads, head_dim, num_ranges, row_runs)
         workspace = _lib.optional_scratch(nbytes, q.device) if nbytes > 0 else None
+        if workspace is None:
+            split_tiles, num_ranges, row_runs = 0, 0, 1
         rc = h.bvllm_paged_window_attention(
             q.data_ptr(), q.stride(0), q.stride(1),
             k_cache.data_ptr(), v_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
@@ -86,6 +102,6 @@ def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
             out.data_ptr(), out.stride(0), out.stride(1),
             num_seqs, num_tokens, max_query_len, single,
             num_heads, num_kv_heads, head_dim, page, None if workspace is None else workspace.data_ptr(),
-            _lib.stream_handle(q.device))
+            columns, split_tiles, num_ranges, row_runs, _lib.stream_handle(q.device))
     _lib.check(rc, "bvllm_paged_window_attention")
     return out

@@ -644,17 +644,27 @@ static bool window_sizes_ok(const WindowArgs& a) {
   return a.window >= 1 && a.sinks >= 0;
 }
 
-extern "C" int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
-                                                int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads,
-                                                int32_t head_dim, int32_t max_blocks, int32_t window, int32_t sinks) {
+extern "C" int bvllm_window_plan(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+                                 int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads,
+                                 int32_t head_dim, int32_t max_blocks, int32_t window, int32_t sinks, int32_t* plan) {
   WindowArgs a{};
   a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.single_query_seqs = single_query_seqs;
   a.max_query_len = max_query_len < num_tokens ? max_query_len : num_tokens;
   a.num_heads = num_heads; a.num_kv_heads = num_kv_heads; a.head_dim = head_dim;
   a.max_blocks = max_blocks; a.window = window; a.sinks = sinks;
-  if (!window_sizes_ok(a) || max_blocks < 1 || num_tokens == 0 || num_seqs == 0 || max_query_len == 0) return 0;
-  if ((int64_t)num_tokens * num_heads > 0x7fffffff) return 0;
-  return window_workspace_bytes(a);
+  if (!window_sizes_ok(a) || max_blocks < 1 || max_query_len < 0 || !plan) return kBad;
+  if ((int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
+  WindowPlan p{128, 0, 0, 1};
+  if (num_tokens > 0 && num_seqs > 0 && max_query_len > 0) p = window_plan(a);
+  plan[0] = p.columns; plan[1] = p.split_tiles; plan[2] = p.num_ranges; plan[3] = p.row_runs;
+  return 0;
+}
+
+extern "C" int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t num_heads,
+                                                int32_t head_dim, int32_t num_ranges, int32_t row_runs) {
+  if (num_seqs <= 0 || num_tokens <= 0 || num_heads <= 0 || head_dim <= 0 || num_ranges < 0 || row_runs < 1) return 0;
+  return 4 * (window_row_floats(num_seqs, num_heads, head_dim, row_runs) +
+              prefill_range_floats(num_ranges, num_tokens, num_heads, head_dim));
 }
 
 extern "C" int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
@@ -668,7 +678,8 @@ extern "C" int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, i
                                             int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                                             int32_t single_query_seqs,
                                             int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                            int32_t block_size, void* workspace, void* stream) {
+                                            int32_t block_size, void* workspace, int32_t columns,
+                                            int32_t split_tiles, int32_t num_ranges, int32_t row_runs, void* stream) {
   WindowArgs a{};
   a.window = window; a.sinks = sinks;
   a.num_seqs = num_seqs; a.num_tokens = num_tokens; a.single_query_seqs = single_query_seqs;
@@ -684,7 +695,12 @@ extern "C" int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, i
   if (max_blocks < 1 || bt_stride < max_blocks) return kBad;
   // Offsets inside one page are 32-bit, and so are (token, head) pairs.
   if ((int64_t)16 * cache_stride_tok > 0x3fffffff || (int64_t)num_tokens * num_heads > 0x7fffffff) return kBad;
-  if (workspace && !aligned16(workspace)) return kBad;
+  if ((columns != 128 && columns != 64 && columns != 32) || split_tiles < 0 || split_tiles > 1 << 20) return kBad;
+  // (More ranges or runs than the table's tiles and pages make would stay empty.)
+  if (split_tiles > 0 ? num_ranges < 1 || num_ranges > prefill_ranges(max_blocks, split_tiles, -1) : num_ranges != 0)
+    return kBad;
+  if (row_runs < 1 || row_runs > (max_blocks < 4096 ? max_blocks : 4096)) return kBad;
+  if ((split_tiles > 0 || row_runs > 1) && (!workspace || !aligned16(workspace))) return kBad;
   a.q = q; a.q_st = q_stride_t; a.q_sh = q_stride_h;
   a.k_cache = k_cache; a.v_cache = v_cache;
   a.c_sb = cache_stride_block; a.c_st = cache_stride_tok; a.c_sh = cache_stride_head;
@@ -693,6 +709,6 @@ extern "C" int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, i
   a.query_start_loc = query_start_loc; a.seq_lens = seq_lens; a.context_lens = context_lens;
   a.scale_log2 = scale * kLog2e;
   a.out = out; a.o_st = out_stride_t; a.o_sh = out_stride_h;
-  a.workspace = workspace;
-  return (int)paged_window_attention(a, (hipStream_t)stream);
+  return (int)paged_window_attention(a, WindowPlan{columns, split_tiles, num_ranges, row_runs},
+                                     reinterpret_cast<float*>(workspace), (hipStream_t)stream);
 }

@@ -267,10 +267,18 @@ struct WindowArgs {
   void* out;      int64_t o_st, o_sh;      // [T, H, D]
   int32_t num_seqs, num_tokens, max_query_len, single_query_seqs;
   int32_t num_heads, num_kv_heads, head_dim;
-  void* workspace;
 };
-hipError_t paged_window_attention(const WindowArgs& a, hipStream_t stream);
-int64_t window_workspace_bytes(const WindowArgs& a);
+// How a step runs: the columns of its prefill blocks, the tiles of the ranges that these are walked in (0: none) and
+// their number, the runs of its single rows.
+struct WindowPlan {
+  int32_t columns, split_tiles, num_ranges, row_runs;
+};
+WindowPlan window_plan(const WindowArgs& a);
+// fp32 values of the rows' partials, a multiple of 4, and of the ranges' behind them.
+inline int64_t window_row_floats(int32_t num_seqs, int32_t num_heads, int32_t head_dim, int32_t runs) {
+  return runs > 1 ? ((int64_t)num_seqs * num_heads * runs * (head_dim + 1) + 3) / 4 * 4 : 0;
+}
+hipError_t paged_window_attention(const WindowArgs& a, const WindowPlan& p, float* workspace, hipStream_t stream);
 
 // How a linear layer of a few tokens runs (skinny_linear.hip).
 struct LinearPlan {

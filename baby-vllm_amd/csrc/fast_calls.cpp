@@ -51,6 +51,7 @@ struct Entry {
   decltype(&bvllm_reorder_beams) reorder = nullptr;
   decltype(&bvllm_build_step_tables) tables = nullptr;
   decltype(&bvllm_qk_norm_rope_append) norm_rope = nullptr;
+  decltype(&bvllm_window_plan) window_plan = nullptr;
   decltype(&bvllm_window_workspace_bytes) window_bytes = nullptr;
   decltype(&bvllm_paged_window_attention) window = nullptr;
 } g;
@@ -84,6 +85,7 @@ const BindName kNames[] = {
     {"bvllm_reorder_beams", (void**)&g.reorder},
     {"bvllm_build_step_tables", (void**)&g.tables},
     {"bvllm_qk_norm_rope_append", (void**)&g.norm_rope},
+    {"bvllm_window_plan", (void**)&g.window_plan},
     {"bvllm_window_workspace_bytes", (void**)&g.window_bytes},
     {"bvllm_paged_window_attention", (void**)&g.window},
 };
@@ -845,17 +847,21 @@ PyObject* fast_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
   }
   const int32_t w = (int32_t)std::min<int64_t>(window, INT32_MAX), first = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
-  const int64_t bytes = g.window_bytes((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)single, (int32_t)heads,
-                                       (int32_t)hkv, (int32_t)d, (int32_t)width, w, first);
+  int32_t plan[4];  // columns, split_tiles, num_ranges, row_runs
+  if (g.window_plan((int32_t)seqs, (int32_t)tokens, (int32_t)max_q, (int32_t)single, (int32_t)heads, (int32_t)hkv,
+                    (int32_t)d, (int32_t)width, w, first, plan) != 0)
+    return none();
+  const int64_t bytes = g.window_bytes((int32_t)seqs, (int32_t)tokens, (int32_t)heads, (int32_t)d, plan[2], plan[3]);
   at::Tensor out = new_empty({tokens, heads, d}, *q, at::kBFloat16), ws;
   if (bytes > 0) ws = optional_scratch(bytes, *q);
+  if (!ws.defined()) plan[1] = plan[2] = 0, plan[3] = 1;
   return launch(out, "bvllm_paged_window_attention", [&] {
     return g.window(ptr(*q), q->stride(0), q->stride(1), ptr(*c), v_half(*c), c->stride(1), c->stride(2), c->stride(3),
                     (int32_t)c->size(1), bt->const_data_ptr<int32_t>(), bt->stride(0), (int32_t)width,
                     qsl->const_data_ptr<int32_t>(), seq->const_data_ptr<int32_t>(), ctx->const_data_ptr<int32_t>(), w,
                     first, scale, ptr(out), out.stride(0), out.stride(1), (int32_t)seqs, (int32_t)tokens, (int32_t)max_q,
                     (int32_t)single, (int32_t)heads, (int32_t)hkv, (int32_t)d, (int32_t)kPage,
-                    ws.defined() ? ptr(ws) : nullptr, stream);
+                    ws.defined() ? ptr(ws) : nullptr, plan[0], plan[1], plan[2], plan[3], stream);
   });
   END_HANDLE_TH_ERRORS
 }

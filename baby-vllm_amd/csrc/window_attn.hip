@@ -62,37 +62,37 @@ __global__ __launch_bounds__(256) void window_merge_kernel(WindowRows w, int per
       make_uint2(pack_bf16x2_hw(num[0] * inv, num[1] * inv), pack_bf16x2_hw(num[2] * inv, num[3] * inv)));
 }
 
-// How the single rows of a step are cut: work-groups of `waves` waves, `splits` of them per (row, column group).
-// Times (us) as measured here, rows of equal length: 5 of start, with 0.18 per page of a work-group at
-// D = 128 (the waves of a work-group share what a CU takes: 4, 8 or 16 of them make no difference) and
-// 0.09 at D = 64 (0.14 on four waves), and 2.3 of the second launch. So rows are cut until every CU has a
-// work-group, into runs of 8 pages at least, where that saves more than the second launch costs (one row
+// The runs of a step of single rows, work-groups of `waves` waves each. Times (us) as measured here, rows of equal length: 5
+// of start, with 0.18 per page of a work-group at D = 128 (the waves of a work-group share what a CU takes: 4, 8 or 16
+// of them make no difference) and 0.09 at D = 64 (0.14 on four waves), and 2.3 of the second launch. So rows are cut until
+// every CU has a work-group, into runs of 8 pages at least, where that saves more than the second launch costs (one row
 // of 7B, 4097 keys: 46.4 whole, 11.2 in 32 runs; 1025: 14.2 and 8.7; 257: 6.0 and 7.4. 32 rows, 1025:
-// 18.6 and 18.3. 48 rows, 4097, a work-group per CU but 64 idle: 70.3 and 76.2). Eight waves at D = 64 but for
+// 18.6 and 18.3. 48 rows, 4097, where 64 CUs are idle: 70.3 and 76.2). Eight waves at D = 64 but for
 // a few pages (64 keys: 4.5 against 4.4), and at D = 128 while half of the CUs are idle (one row, 1025
 // keys: 8.7 against 9.0); else four (64 rows, 1025: 24.8 against 25.1, 96 rows: 39.4 against 41.2).
 constexpr int64_t kMaxRowBytes = 64ll << 20;  // of their partials
-
-struct RowPlan {
-  int waves, splits;
-};
 
 // The pages that a row can see at most.
 static int64_t max_row_pages(const WindowArgs& a) {
   return std::min<int64_t>(a.max_blocks, ((int64_t)a.window + 15) / 16 + 1 + ((int64_t)a.sinks + 15) / 16);
 }
-
-static RowPlan row_plan(const WindowArgs& a, int64_t rows, int64_t max_bytes) {
-  const int64_t pages = max_row_pages(a);
+// (Row, column group) pairs of so many rows.
+static int64_t row_units(const WindowArgs& a, int64_t rows) {
   const int G = a.num_heads / a.num_kv_heads;
-  const int64_t units = std::max<int64_t>(1, rows * a.num_kv_heads * ((G + 15) / 16)), cus = device_cus();
-  const int64_t room = max_bytes / ((int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4);
-  const int64_t splits = std::min({cus / units, pages / 8, room});
-  RowPlan p{4, 1};
-  if (splits > 1 && (a.head_dim == 128 ? 0.18 : 0.09) * (double)(pages - (pages + splits - 1) / splits) > 3.5)
-    p.splits = (int)splits;
-  p.waves = a.head_dim == 64 ? (pages < 8 ? 4 : 8) : (2 * units * p.splits <= cus ? 8 : 4);
-  return p;
+  return std::max<int64_t>(1, rows * a.num_kv_heads * ((G + 15) / 16));
+}
+
+static int32_t runs_of_rows(const WindowArgs& a) {
+  const int64_t pages = max_row_pages(a), units = row_units(a, std::min(a.num_tokens, a.num_seqs));
+  const int64_t room = kMaxRowBytes / ((int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4);
+  const int64_t runs = std::min({device_cus() / units, pages / 8, room});
+  const bool pays = runs > 1 && (a.head_dim == 128 ? 0.18 : 0.09) * (double)(pages - (pages + runs - 1) / runs) > 3.5;
+  return pays ? (int32_t)runs : 1;
+}
+
+static int waves_of_rows(const WindowArgs& a, int32_t runs) {
+  if (a.head_dim == 64) return max_row_pages(a) < 8 ? 4 : 8;
+  return 2 * row_units(a, std::min(a.num_tokens, a.num_seqs)) * runs <= device_cus() ? 8 : 4;
 }
 
 static DecodeArgs rows_of_step(const WindowArgs& w) {
@@ -139,14 +139,6 @@ static PrefillArgs blocks_of_step(const WindowArgs& w) {
   return a;
 }
 
-// How a step runs: its single rows, the columns of its prefill blocks, the ranges (of split_tiles tiles, 0: none) that
-// these are walked in.
-struct WindowPlan {
-  RowPlan rows;
-  int columns, split_tiles, num_ranges;
-  int64_t row_floats, range_floats;  // of their partials
-};
-
 // What a launch of the blocks takes (us), fitted to 9,232 random steps (prompts of 2 to 8192 tokens of up to 64 sequences
 // behind up to 16,000, windows of 32 to 8192, 7B and 0.5B heads; rms 19%): a start, and per tile of a walk less with one
 // work-group per CU than with two; every further round of two per CU has its own start. Ranges
@@ -166,14 +158,15 @@ constexpr int64_t kMaxRangeBytes = 64ll << 20;  // of the ranges' partials
 // 2140 to 8560 keys beside prompts of 3 to 5 tokens 87 -> 33 us).
 constexpr double kRunLaunch = 4.5;
 
-static void plan_blocks(const WindowArgs& w, WindowPlan& p) {
+static WindowPlan plan_blocks(const WindowArgs& w) {
   const PrefillArgs a = blocks_of_step(w);
   const int64_t group = a.num_heads / a.num_kv_heads, cus = device_cus();
   const int64_t range_bytes = prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4;
   const int64_t row_pages = max_row_pages(w);
   const int64_t rows = w.single_query_seqs >= 0 ? w.single_query_seqs : w.num_seqs;
-  const int64_t units = rows * a.num_kv_heads * ((group + 15) / 16);
+  const int64_t units = row_units(w, rows);
   const int64_t row_bytes = (int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4;
+  WindowPlan p{128, 0, 0, 1};
   double best = 0;
   for (int form = 0; form < 3; ++form) {
     const int columns = 128 >> form;
@@ -197,68 +190,47 @@ static void plan_blocks(const WindowArgs& w, WindowPlan& p) {
         const double both = rows > 0 ? std::max(t, row) + (runs > 1 ? kRunLaunch : 0) : t;
         if (best == 0 || both < best) {
           best = both;
-          p.columns = columns;
-          p.split_tiles = (int)split;
-          p.num_ranges = (int)ranges;
-          p.rows.splits = (int)runs;
+          p = {columns, (int32_t)split, split > 0 ? (int32_t)ranges : 0, (int32_t)runs};
         }
         if (rows == 0) break;
       }
     }
   }
-}
-
-static WindowPlan window_plan(const WindowArgs& a) {
-  WindowPlan p{{4, 1}, 128, 0, 1, 0, 0};
-  if (a.max_query_len == 1) p.rows = row_plan(a, std::min(a.num_tokens, a.num_seqs), kMaxRowBytes);
-  else plan_blocks(a, p);
-  // (The ranges' partials, behind the rows', are 16-byte aligned.)
-  if (p.rows.splits > 1) p.row_floats = ((int64_t)a.num_seqs * a.num_heads * p.rows.splits * (a.head_dim + 1) + 3) / 4 * 4;
-  if (p.split_tiles > 0) p.range_floats = prefill_range_floats(p.num_ranges, a.num_tokens, a.num_heads, a.head_dim);
   return p;
 }
 
+WindowPlan window_plan(const WindowArgs& a) {
+  return a.max_query_len == 1 ? WindowPlan{128, 0, 0, runs_of_rows(a)} : plan_blocks(a);
+}
+
 template <int D>
-static hipError_t launch_window(const WindowArgs& w, hipStream_t stream) {
-  WindowPlan p = window_plan(w);
-  if (w.workspace == nullptr) {
-    p.rows.splits = 1;
-    p.split_tiles = 0;
-    p.num_ranges = 1;
-    p.row_floats = 0;
-  }
+static hipError_t launch_window(const WindowArgs& w, const WindowPlan& p, float* workspace, hipStream_t stream) {
   WindowRows r{rows_of_step(w), w.window, w.sinks};
-  float* ws = reinterpret_cast<float*>(w.workspace);
-  r.rows.num_splits = p.rows.splits;
-  r.rows.part_out = ws;
-  r.rows.part_lse = ws + (int64_t)w.num_seqs * w.num_heads * p.rows.splits * D;
+  r.rows.num_splits = p.row_runs;
+  r.rows.part_out = workspace;
+  r.rows.part_lse = workspace + (int64_t)w.num_seqs * w.num_heads * p.row_runs * D;
   hipError_t err;
   if (w.max_query_len == 1) {
-    err = p.rows.waves == 4 ? launch_rows<D, 4>(r, stream) : launch_rows<D, 8>(r, stream);
+    err = waves_of_rows(w, p.row_runs) == 4 ? launch_rows<D, 4>(r, stream) : launch_rows<D, 8>(r, stream);
   } else {
     PrefillArgs a = blocks_of_step(w);
     a.split_tiles = p.split_tiles;
     a.num_ranges = p.num_ranges;
-    a.part_out = ws + p.row_floats;
+    a.part_out = workspace + window_row_floats(w.num_seqs, w.num_heads, D, p.row_runs);
     a.part_ml = a.part_out + (int64_t)p.num_ranges * w.num_tokens * w.num_heads * D;
     err = paged_prefill_window(a, r, p.columns, stream);
   }
-  if (err != hipSuccess || p.rows.splits == 1 || w.single_query_seqs == 0) return err;
+  if (err != hipSuccess || p.row_runs == 1 || w.single_query_seqs == 0) return err;
   const int per_row = (w.num_heads * (D / 4) + 255) / 256;
   if ((int64_t)w.num_seqs * per_row > 0x7fffffff) return hipErrorInvalidValue;
   hipLaunchKernelGGL((window_merge_kernel<D>), dim3((unsigned)(w.num_seqs * per_row)), dim3(256), 0, stream, r, per_row);
   return hipGetLastError();
 }
 
-int64_t window_workspace_bytes(const WindowArgs& a) {
-  const WindowPlan p = window_plan(a);
-  return 4 * (p.row_floats + p.range_floats);
-}
-
-hipError_t paged_window_attention(const WindowArgs& a, hipStream_t stream) {
+hipError_t paged_window_attention(const WindowArgs& a, const WindowPlan& p, float* workspace, hipStream_t stream) {
   switch (a.head_dim) {
-    case 64: return launch_window<64>(a, stream);
-    case 128: return launch_window<128>(a, stream);
+    case 64: return launch_window<64>(a, p, workspace, stream);
+    case 128: return launch_window<128>(a, p, workspace, stream);
     default: return hipErrorInvalidValue;
   }
 }

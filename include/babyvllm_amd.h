@@ -484,14 +484,22 @@ BVLLM_API int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int64
  * j < sinks. A row with no visible key outputs zeros; keys that a row does not see do not reach
  * it, whatever they hold, and table entries of pages that no row of the sequence sees may hold
  * anything. window at least 1, sinks at least 0, scale positive and finite. single_query_seqs as
- * in bvllm_paged_prefill (-1: unknown): it steers how the step is launched, never what is computed.
- * workspace holds bvllm_window_workspace_bytes() bytes of the same sizes, or is NULL: then rows
- * and blocks of few work-groups are not cut over more of them. Results agree within the rounding of
- * fp32 sums in another order.
+ * in bvllm_paged_prefill (-1: unknown).
+ * How the step is launched: sequences of several queries run in blocks of `columns` (128, 64 or 32) (query,
+ * head) pairs; split_tiles > 0 cuts a block's walk over the keys it sees into num_ranges ranges of
+ * split_tiles 64-key tiles (the last one runs to its end, so any num_ranges from 1 to that of the table
+ * computes every key), each a work-group of its own. A single query's pages are cut into row_runs (at least
+ * 1) runs. Both leave fp32 partials in workspace, which a further launch each adds;
+ * bvllm_window_workspace_bytes() of the same num_ranges (0 without ranges) and row_runs says how much,
+ * and may be 0. bvllm_window_plan writes the four to use, from host sizes alone (plan[0..3]: columns, split_tiles,
+ * num_ranges, row_runs; partials of either kind are at most 64 MiB). They steer the choice only: results agree
+ * within the rounding of fp32 sums in another order.
  */
-BVLLM_API int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
+BVLLM_API int bvllm_window_plan(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                     int32_t max_blocks, int32_t window, int32_t sinks);
+                     int32_t max_blocks, int32_t window, int32_t sinks, int32_t* plan);
+BVLLM_API int64_t bvllm_window_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t num_heads,
+                     int32_t head_dim, int32_t num_ranges, int32_t row_runs);
 BVLLM_API int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                      const void* k_cache, const void* v_cache,
                      int64_t cache_stride_block, int64_t cache_stride_tok, int64_t cache_stride_head,
@@ -503,7 +511,8 @@ BVLLM_API int bvllm_paged_window_attention(const void* q, int64_t q_stride_t, in
                      int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t single_query_seqs,
                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                     int32_t block_size, void* workspace, void* stream);
+                     int32_t block_size, void* workspace, int32_t columns, int32_t split_tiles,
+                     int32_t num_ranges, int32_t row_runs, void* stream);
 
 #ifdef __cplusplus
 }

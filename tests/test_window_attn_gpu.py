@@ -127,34 +127,41 @@ def check(got, want):
     assert (rows <= row_tol).all(), f"a row's norm is off by {(rows / row_tol).max().item():.3g} times the bound"
 
 
-def raw_call(q, cache, md, scale, window, sinks, cut=True, single=-1):
-    """The C entry: with or without the workspace that lets rows and blocks be cut."""
+def raw_call(q, cache, md, scale, window, sinks, columns=128, split=0, runs=1, single=-1):
+    """The C entry with a choice of blocks, of the ranges of their walks and of the runs of single rows."""
     from babyvllm.kernels import _lib
     h = _lib.lib()
     t, heads, d = q.shape
     seqs, hkv, bt, k = md.seq_lens.shape[0], cache.shape[3], md.block_tables, cache[0]
+    runs = min(runs, bt.shape[1])
+    # Every range that the table's keys can make, and fewer, where the last one takes what is left.
+    ranges = cdiv(cdiv(bt.shape[1], 4), split) if split else 0
+    ranges = max(1, ranges * 2 // 3) if split % 2 else ranges
     out = torch.full((t, heads, d), NAN, device="cuda", dtype=torch.bfloat16)
-    window, sinks = min(window, 2**31 - 1), min(sinks, 2**31 - 1)
-    nbytes = h.bvllm_window_workspace_bytes(seqs, t, md.max_query_len, single, heads, hkv, d, bt.shape[1], window, sinks)
-    ws = torch.full((max(4, nbytes // 4),), NAN, device="cuda")
+    ws = torch.full((max(4, h.bvllm_window_workspace_bytes(seqs, t, heads, d, ranges, runs) // 4),), NAN, device="cuda")
     rc = h.bvllm_paged_window_attention(
         q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), cache[1].data_ptr(), *k.stride()[:3], cache.shape[1],
         bt.data_ptr(), bt.stride(0), bt.shape[1], md.query_start_loc.data_ptr(), md.seq_lens.data_ptr(),
-        md.context_lens.data_ptr(), window, sinks, scale, out.data_ptr(), out.stride(0), out.stride(1), seqs, t,
-        md.max_query_len, single, heads, hkv, d, 16, ws.data_ptr() if cut and nbytes else None,
+        md.context_lens.data_ptr(), min(window, 2**31 - 1), min(sinks, 2**31 - 1), scale, out.data_ptr(), out.stride(0),
+        out.stride(1), seqs, t, md.max_query_len, single, heads, hkv, d, 16, ws.data_ptr(), columns, split, ranges, runs,
         _lib.stream_handle(q.device))
     _lib.check(rc, "bvllm_paged_window_attention")
     return out
 
 
-def run(q, cache, md, window, sinks, scale=None):
-    """The public call and the C entry with what steers it: all against the formula."""
+# Blocks of every width, whole and in ranges of a tile, of two and of three, single rows whole and in runs of a page and more.
+FORMS = [(128, 0, 1), (64, 0, 2), (32, 0, 3), (128, 1, 1), (64, 1, 5), (32, 1, 1000), (128, 2, 1), (64, 3, 2), (32, 2, 1)]
+
+
+def run(q, cache, md, window, sinks, scale=None, forms=()):
+    """The public call, and the C entry's forms: all against the formula."""
     scale = q.shape[-1] ** -0.5 if scale is None else scale
     want = formula(q, cache, md, scale, window, sinks)
     got = paged_window_attention(q, cache, md, scale, window, sinks)
     check(got, want)
-    check(raw_call(q, cache, md, scale, window, sinks), want)
-    check(raw_call(q, cache, md, scale, window, sinks, cut=False), want)
+    for form in forms:
+        print(window, sinks, form, flush=True)
+        check(raw_call(q, cache, md, scale, window, sinks, *form), want)
     return got
 
 
@@ -173,9 +180,10 @@ VIEWS = [(1, 0), (1, 1), (5, 3), (16, 0), (17, 4), (33, 16), (64, 40), (100, 4),
 @pytest.mark.parametrize("heads", HEADS, ids=str)
 @pytest.mark.parametrize("name", SPECS)
 def test_against_the_formula(name, heads):
-    for window, sinks in VIEWS:
+    for i, (window, sinks) in enumerate(VIEWS):
         print(window, sinks, flush=True)
-        run(*build(SPECS[name], *heads, window, sinks, seed=len(name)), window, sinks)
+        run(*build(SPECS[name], *heads, window, sinks, seed=len(name)), window, sinks,
+            forms=FORMS if name in ("behind", "mixed_and_empty") else FORMS[i % 3::3])
 
 
 @pytest.mark.parametrize("specs,heads,window,sinks", [
@@ -184,22 +192,27 @@ def test_against_the_formula(name, heads):
     ([(0, 600)], (1, 32, 64), 1000, 0), ([(3000, 1)] * 3, (1, 40, 128), 1024, 4),
 ], ids=str)
 def test_long_sequences(specs, heads, window, sinks):
-    run(*build(specs, *heads, window, sinks, q_view=True, width_extra=5), window, sinks)
+    run(*build(specs, *heads, window, sinks, q_view=True, width_extra=5), window, sinks, forms=[(128, 7, 4), (64, 16, 9), (32, 0, 1)])
 
 
 def test_many_sequences_of_mixed_lengths():
     rng = random.Random(9)
     specs = [(rng.choice([0, 3, 50, 333, 1200]), rng.choice([1, 1, rng.randint(1, 40)])) for _ in range(130)]
-    run(*build(specs, 2, 7, 64, 100, 4), 100, 4)
-    run(*build([(c, 1) for c, _ in specs], 2, 7, 64, 100, 20), 100, 20)
+    q, cache, md = build(specs, 2, 7, 64, 100, 4)
+    run(q, cache, md, 100, 4, forms=FORMS)
+    singles = sum(n == 1 for _, n in specs)
+    check(raw_call(q, cache, md, 0.125, 100, 4, 64, 0, 1, singles), formula(q, cache, md, 0.125, 100, 4))
+    check(raw_call(q, cache, md, 0.125, 100, 4, 64, 0, 1, 0), formula(q, cache, md, 0.125, 100, 4))  # in blocks too
+    run(*build([(c, 1) for c, _ in specs], 2, 7, 64, 100, 20), 100, 20, forms=FORMS)
 
 
 def test_rows_behind_the_last_sequence_are_left_as_they_are():
     for specs in ([(40, 1), (100, 1)], [(40, 9), (100, 1)]):
         q, cache, md = build(specs, 2, 7, 64, 30, 2, rows_behind=70)
-        got = raw_call(q, cache, md, 0.1, 30, 2)
-        check(got, formula(q, cache, md, 0.1, 30, 2))
-        assert torch.isnan(got[md.query_start_loc_cpu[-1]:]).all()
+        for form in FORMS:
+            got = raw_call(q, cache, md, 0.1, 30, 2, *form)
+            check(got, formula(q, cache, md, 0.1, 30, 2))
+            assert torch.isnan(got[md.query_start_loc_cpu[-1]:]).all()
 
 
 def test_rows_without_a_visible_key_give_zeros():
@@ -207,10 +220,10 @@ def test_rows_without_a_visible_key_give_zeros():
     # Of the first sequence, nothing of what its row's window reaches is there; of the others, not all.
     md.seq_lens = i32([100, 45, 0, 0])
     md.seq_lens_cpu = md.seq_lens.tolist()
-    got = run(q, cache, md, 20, 0)
+    got = run(q, cache, md, 20, 0, forms=FORMS)
     assert not got[0].any() and not got[21:].any() and got[1:5].any()
     md.block_tables = md.block_tables[:, :3].contiguous()  # and tables that end before the window
-    run(q, cache, md, 20, 0)
+    run(q, cache, md, 20, 0, forms=FORMS)
 
 
 @pytest.mark.parametrize("value", [NAN, INF, -INF])
@@ -228,7 +241,7 @@ def test_values_that_are_not_finite_reach_the_rows_that_see_them(heads, value):
                     cache[1, page, p % PAGE, :, (7 * s + 13 * j) % heads[2]] = value
                 elif math.isnan(value):
                     cache[0, page, p % PAGE, 0, (7 * s + 13 * j) % heads[2]] = value
-        run(q, cache, md, window, sinks)
+        run(q, cache, md, window, sinks, forms=FORMS)
 
 
 def test_large_scores_and_weights_that_vanish():
@@ -239,8 +252,8 @@ def test_large_scores_and_weights_that_vanish():
         cache[0, ..., 0] = sign * (ramp + torch.arange(cache.shape[1], device="cuda").to(torch.bfloat16)[:, None, None] % 7 * 30)
         q[..., 0] = 3.0
         want = formula(q, cache, md, 0.125, 50, 2)
-        for got in (paged_window_attention(q, cache, md, 0.125, 50, 2), raw_call(q, cache, md, 0.125, 50, 2, cut=False)):
-            got = got.cpu().double()
+        for form in FORMS:
+            got = raw_call(q, cache, md, 0.125, 50, 2, *form).cpu().double()
             # (Scores of some thousands have errors of their own: 64 products of up to 630, 2^-24 each, a unit of the
             # exponent's 2^-13: weights off by at most 2^-10.)
             tol = want[1] + 2 ** -9 * want[1] * 2 ** 8
@@ -257,7 +270,7 @@ def test_pages_past_2_31_elements():
     for ctx, new in ((80, 1), (50, 40)):
         q = torch.randn(new, hkv * 2, d, device="cuda", dtype=torch.bfloat16)
         md = AttentionMetadata(None, table, i32([0, new]), i32([ctx + new]), i32([ctx]), [0, new], [ctx + new], [ctx], new, ctx + new)
-        run(q, cache, md, window, 1)
+        run(q, cache, md, window, 1, forms=FORMS[::2])
 
 
 @pytest.mark.parametrize("kind", ["decode", "mixed"])
@@ -282,6 +295,26 @@ def test_captured_steps_replay_with_other_lengths(kind):
         check(got, formula(q, cache, md, 0.1, window, sinks))
         check(again, formula(q, cache, md, 0.1, 33, 0))
         assert torch.equal(paged_window_attention(q, cache, md, 0.1, window, sinks), got)
+
+
+def test_a_captured_step_takes_other_sequences():
+    # One token of each but one sequence at first, prompts of all later: nothing of the captured step's host lists stays.
+    q, cache, md = build([(300, 16)] * 6, 2, 7, 64, 10**6, 0)
+    md.query_start_loc.copy_(i32([0, 1, 2, 3, 4, 20, 20]))
+    md.query_start_loc_cpu, md.max_query_len = md.query_start_loc.tolist(), 96
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = paged_window_attention(q, cache, md, 0.1, 100, 4)
+    for new in ([16] * 6, [1] * 6, [91, 1, 1, 1, 1, 1], [0, 0, 96, 0, 0, 0], [1, 1, 1, 1, 16, 0]):
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        md.query_start_loc.copy_(i32(starts))
+        md.context_lens.copy_(i32([316 - n for n in new]))
+        graph.replay()
+        torch.cuda.synchronize()
+        check(got, formula(q, cache, md, 0.1, 100, 4))
 
 
 def test_on_two_streams_at_once():
@@ -314,6 +347,8 @@ def test_refusals():
     q, cache, md = build([(40, 1), (20, 9)], 2, 7, 64, 100, 4)
     call = lambda q=q, cache=cache, md=md, w=16, k=4: paged_window_attention(q, cache, md, 0.1, w, k)  # noqa: E731
     from dataclasses import replace
+    with pytest.raises(TypeError):
+        call(w=16.5)
     for w, k in ((0, 4), (-1, 4), (16, -1)):
         with pytest.raises(ValueError, match="window"):
             call(w=w, k=k)
