@@ -44,38 +44,56 @@ __device__ __forceinline__ void store8(uint16_t* p, const uint4& v) {
   }
 }
 
-__device__ __forceinline__ void widen(const uint4& c, float (&f)[8]) {
-  const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[2 * i] = lo_f32(w[i]);
-    f[2 * i + 1] = hi_f32(w[i]);
-  }
-}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// 8 values of a row of cos, sin or a weight, bf16 or fp32.
-template <bool ALIGNED>
-__device__ __forceinline__ void load_floats(const void* base, bool fp32, int64_t at, float (&f)[8]) {
-  if (fp32) {
+// 8 values as they lie in memory, bf16 or fp32, widened where they are used. (The type is the kernel's: a branch on it
+// around the loads waited for each of them by itself, 8192 tokens of 7B with bf16 rows and weights 37.8 us.)
+template <bool FP32>
+struct Eight {
+  uint4 w[FP32 ? 2 : 1];
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (FP32) return __uint_as_float(word(w[i / 4], i % 4));
+    else return i & 1 ? hi_f32(word(w[0], i / 2)) : lo_f32(word(w[0], i / 2));
+  }
+};
+
+// Of a row of cos, sin or a weight.
+template <bool ALIGNED, bool FP32>
+__device__ __forceinline__ Eight<FP32> load_eight(const void* base, int64_t at) {
+  Eight<FP32> r;
+  if constexpr (FP32) {
     const float* p = reinterpret_cast<const float*>(base) + at;
     if constexpr (ALIGNED) {
-      const uint4 a = ld16(p), b = ld16(p + 4);
-      const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(w[i]);
+      r.w[0] = ld16(p);
+      r.w[1] = ld16(p + 4);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = p[i];
+      for (int i = 0; i < 2; ++i)
+        r.w[i] = make_uint4(__float_as_uint(p[4 * i]), __float_as_uint(p[4 * i + 1]), __float_as_uint(p[4 * i + 2]),
+                            __float_as_uint(p[4 * i + 3]));
     }
   } else {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(base) + at;
     if constexpr (ALIGNED) {
-      widen(ld16(p), f);
+      r.w[0] = ld16(p);
     } else {
+      uint32_t x[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = bf16_to_f32(p[i]);
+      for (int i = 0; i < 4; ++i) x[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
+      r.w[0] = make_uint4(x[0], x[1], x[2], x[3]);
     }
   }
+  return r;
+}
+
+// Sum over groups of N lanes: pairs, quads, then mirrors, which exchange lanes that hold the same.
+template <int N>
+__device__ __forceinline__ float row_sum(float x) {
+  x += __uint_as_float(dpp<kQuadSwap1>(__float_as_uint(x)));
+  x += __uint_as_float(dpp<kQuadSwap2>(__float_as_uint(x)));
+  if constexpr (N > 4) x += __uint_as_float(dpp<kRowHalfMirror>(__float_as_uint(x)));
+  if constexpr (N > 8) x += __uint_as_float(dpp<kRowMirror>(__float_as_uint(x)));
+  return x;
 }
 
 __device__ __forceinline__ uint4 narrow(const float (&f)[8]) {
@@ -83,7 +101,7 @@ __device__ __forceinline__ uint4 narrow(const float (&f)[8]) {
                     pack_bf16x2_hw(f[6], f[7]));
 }
 
-template <int D, bool ALIGNED>
+template <int D, bool ALIGNED, bool ROWS_FP32, bool WEIGHT_FP32>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a, int32_t units) {
   constexpr int HALF = D / 2;
   constexpr int RC = D / 16, RPU = 64 / RC;  // lanes per rotated row, rows per unit
@@ -113,24 +131,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a, int
   const int head = live ? (is_k ? row - a.num_heads : row) : 0;
   const uint16_t* src = is_k ? reinterpret_cast<const uint16_t*>(a.k) + t * a.k_st + head * a.k_sh
                              : reinterpret_cast<const uint16_t*>(a.q) + t * a.q_st + head * a.q_sh;
-  float x1[8], x2[8], w1[8], w2[8], c1[8], c2[8], s1[8], s2[8];
-  widen(load8<ALIGNED>(src + 8 * c), x1);
-  widen(load8<ALIGNED>(src + HALF + 8 * c), x2);
-  load_floats<ALIGNED>(is_k ? a.k_weight : a.q_weight, a.weight_fp32, 8 * c, w1);
-  load_floats<ALIGNED>(is_k ? a.k_weight : a.q_weight, a.weight_fp32, HALF + 8 * c, w2);
-  load_floats<ALIGNED>(a.cos, a.rows_fp32, t * a.cs_st + 8 * c, c1);
-  load_floats<ALIGNED>(a.cos, a.rows_fp32, t * a.cs_st + HALF + 8 * c, c2);
-  load_floats<ALIGNED>(a.sin, a.rows_fp32, t * a.sn_st + 8 * c, s1);
-  load_floats<ALIGNED>(a.sin, a.rows_fp32, t * a.sn_st + HALF + 8 * c, s2);
+  // All loads of the lane, then the sums.
+  const Eight<false> a1 = {{load8<ALIGNED>(src + 8 * c)}}, a2 = {{load8<ALIGNED>(src + HALF + 8 * c)}};
+  const void* weight = is_k ? a.k_weight : a.q_weight;
+  const Eight<WEIGHT_FP32> w1 = load_eight<ALIGNED, WEIGHT_FP32>(weight, 8 * c);
+  const Eight<WEIGHT_FP32> w2 = load_eight<ALIGNED, WEIGHT_FP32>(weight, HALF + 8 * c);
+  const int64_t cs = t * a.cs_st + 8 * c, sn = t * a.sn_st + 8 * c;
+  const Eight<ROWS_FP32> c1 = load_eight<ALIGNED, ROWS_FP32>(a.cos, cs), c2 = load_eight<ALIGNED, ROWS_FP32>(a.cos, cs + HALF);
+  const Eight<ROWS_FP32> s1 = load_eight<ALIGNED, ROWS_FP32>(a.sin, sn), s2 = load_eight<ALIGNED, ROWS_FP32>(a.sin, sn + HALF);
+  __builtin_amdgcn_sched_barrier(0);
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(x1[i], x1[i], __builtin_fmaf(x2[i], x2[i], sum));
-#pragma unroll
-  for (int d = 1; d < RC; d <<= 1) sum += __shfl_xor(sum, d, 64);
+  for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(a1[i], a1[i], __builtin_fmaf(a2[i], a2[i], sum));
+  sum = row_sum<RC>(sum);
   const float r = 1.f / sqrtf(sum * (1.f / D) + a.eps);
+  float x1[8], x2[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y1 = x1[i] * r * w1[i], y2 = x2[i] * r * w2[i];
+    const float y1 = a1[i] * r * w1[i], y2 = a2[i] * r * w2[i];
     x1[i] = y1 * c1[i] - y2 * s1[i];
     x2[i] = y2 * c2[i] + y1 * s2[i];
   }
@@ -141,16 +159,24 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkNormRopeArgs a, int
   store8<ALIGNED>(dst + HALF + 8 * c, narrow(x2));
 }
 
+template <int D, bool ALIGNED, bool ROWS_FP32>
+void launch(const QkNormRopeArgs& a, unsigned blocks, int32_t units, hipStream_t stream) {
+  if (a.weight_fp32)
+    hipLaunchKernelGGL((qk_norm_rope_kernel<D, ALIGNED, ROWS_FP32, true>), dim3(blocks), dim3(256), 0, stream, a, units);
+  else
+    hipLaunchKernelGGL((qk_norm_rope_kernel<D, ALIGNED, ROWS_FP32, false>), dim3(blocks), dim3(256), 0, stream, a, units);
+}
+
 template <int D>
 hipError_t launch(const QkNormRopeArgs& a, hipStream_t stream) {
   constexpr int RPU = 64 / (D / 16), VPU = 64 / (D / 8);
   const int64_t units = ((int64_t)a.num_heads + a.num_kv_heads + RPU - 1) / RPU + (a.num_kv_heads + VPU - 1) / VPU;
   const int64_t blocks = (a.num_tokens * units + 3) / 4;
   if (units > 0x7fffffff || blocks > 0x7fffffff) return hipErrorInvalidValue;
-  if (a.vec_ok)
-    hipLaunchKernelGGL((qk_norm_rope_kernel<D, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, (int32_t)units);
-  else
-    hipLaunchKernelGGL((qk_norm_rope_kernel<D, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, (int32_t)units);
+  if (a.vec_ok && a.rows_fp32) launch<D, true, true>(a, (unsigned)blocks, (int32_t)units, stream);
+  else if (a.vec_ok) launch<D, true, false>(a, (unsigned)blocks, (int32_t)units, stream);
+  else if (a.rows_fp32) launch<D, false, true>(a, (unsigned)blocks, (int32_t)units, stream);
+  else launch<D, false, false>(a, (unsigned)blocks, (int32_t)units, stream);
   return hipGetLastError();
 }
 
