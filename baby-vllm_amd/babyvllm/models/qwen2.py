@@ -88,7 +88,12 @@ class Qwen2Attention(nn.Module):
         if ctx is None or self.attn.kv_cache is None:
             raise RuntimeError("Qwen2Attention needs a KV cache and a forward context")
         slots = ctx.attn_metadata.slot_mapping
-        if self.q_norm is not None:
+        # The fused form skips the norm modules' calls: only where nothing is attached to them.
+        if self.q_norm is not None and not (type(self.q_norm) is type(self.k_norm) is RMSNorm and not _has_hooks(self.q_norm)
+                                            and not _has_hooks(self.k_norm) and self.q_norm.eps == self.k_norm.eps):
+            q, k = self.q_norm(q.contiguous())[0], self.k_norm(k.contiguous())[0]
+            q, k = fused_rope_and_cache(q, k, v, cos, sin, kv_cache=self.attn.kv_cache, slot_mapping=slots)
+        elif self.q_norm is not None:
             q = fused_qk_norm_rope_and_cache(q, k, v, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps, cos, sin,
                                              self.attn.kv_cache, slots)
         else:

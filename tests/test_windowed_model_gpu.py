@@ -180,6 +180,19 @@ def test_generation_against_a_plain_model(options):
         assert a[:clear] == b[:clear]
 
 
+def test_norm_modules_with_hooks_are_called():
+    cfg = config(qk_norm=True)
+    plain, hooked = llm_of(cfg, graphs=False), llm_of(cfg, graphs=False)
+    seen = []
+    for layer in hooked.model_runner.model.model.layers:
+        layer.self_attn.k_norm.register_forward_hook(lambda m, a, out: seen.append(out[0].shape))
+    _, a = G.generate_recording(plain, prompts(), 4)
+    _, b = G.generate_recording(hooked, prompts(), 4)
+    assert seen and all(s[1:] == (2, 64) for s in seen)
+    # (Three roundings of q and k more: of the normed value, of both products of the rotation.)
+    assert max((x[0] - y[0]).abs().max().item() for x, y in zip(a, b)) <= LOGIT_MAX_TOL
+
+
 def test_a_window_of_everything_is_no_window():
     full, wide = llm_of(config()), llm_of(config(sliding_window=4096))
     _, a = G.generate_recording(full, prompts(), 4)
