@@ -142,8 +142,10 @@ static PrefillArgs blocks_of_step(const WindowArgs& w) {
 // What a launch of the blocks takes (us), fitted to 9,232 random steps (prompts of 2 to 8192 tokens of up to 64 sequences
 // behind up to 16,000, windows of 32 to 8192, 7B and 0.5B heads; rms 19%): a start, and per tile of a walk less with one
 // work-group per CU than with two; every further round of two per CU has its own start. Ranges
-// add a launch and their partials' bytes. Of the forms below, the best by these takes 1.02 times the best as measured on
-// average, 1.24 in one step of 100 (128 columns without ranges always: 1.18, 64 or 32: 1.25).
+// add a launch and their partials' bytes. With ranges of 4, 8, 12, 16, 24 or 32 tiles, the best form by these takes 1.02 times
+// the best as measured on average, 1.24 in one step of 100 (128 columns without ranges always: 1.18, 64 or 32: 1.25). Cuts into
+// ranges about as long as each other take 0.96 times as long as those, over 8914 random steps of 2 to 400 new tokens behind
+// 1000 to 16,000 (0.83 in one step of 100, 1.12 in another).
 struct BlockCost {
   double start, tile_one, tile_two, round;
 };
@@ -175,9 +177,10 @@ static WindowPlan plan_blocks(const WindowArgs& w) {
     const int64_t span = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
     const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
     const int64_t tiles = (pages + 3) / 4, blocks = prefill_work_groups(a, columns);
-    for (int64_t split : {0, 4, 8, 12, 16, 24, 32}) {
-      if (split >= tiles) break;
-      const int64_t ranges = split > 0 ? (tiles + split - 1) / split : 1;
+    for (int64_t most : {0, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32}) {
+      if (most >= tiles) break;
+      // As few ranges as of so many tiles at most, all about as long.
+      const int64_t ranges = most > 0 ? (tiles + most - 1) / most : 1, split = most > 0 ? (tiles + ranges - 1) / ranges : 0;
       if (ranges > 1 && ranges * range_bytes > kMaxRangeBytes) continue;
       const double walk = (double)(split > 0 ? split : tiles);
       const int64_t full = blocks * ranges / (2 * cus), rest = blocks * ranges - full * 2 * cus;

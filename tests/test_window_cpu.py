@@ -94,7 +94,7 @@ def test_plans_fit_what_the_call_takes_and_their_scratch_is_bounded():
         seqs, longest = rng.randint(1, rng.choice([1, 8, 300])), rng.choice([1, 1, rng.randint(2, 100), rng.randint(2, 9000)])
         tokens = rng.randint(longest, longest * seqs)
         heads, hkv, d = rng.choice([(28, 4, 128), (14, 2, 64), (8, 8, 64), (40, 1, 128), (64, 64, 128)])
-        width = rng.choice([1, 7, 130, 2049, 1 << 27])
+        width = rng.choice([1, 7, rng.randint(17, 700), 2049, 1 << 27])
         columns, split, ranges, runs, nbytes = plan(
             seqs, tokens, longest, rng.choice([-1, 0, rng.randint(0, seqs)]), heads, hkv, d, width,
             rng.choice([1, 40, 1024, 8192, 2**31 - 1]), rng.choice([0, 4, 300, 2**31 - 1]))
