@@ -157,12 +157,37 @@ constexpr int64_t kMaxRangeBytes = 64ll << 20;  // of the ranges' partials
 
 // The step's single rows run beside the blocks, on four waves a run: 5 us and 0.18 (D = 128) or 0.14 per page. Where they
 // would take longer than the blocks they are cut, for a launch that adds their runs (4.5 us with its partials; 6 rows of
-// 2140 to 8560 keys beside prompts of 3 to 5 tokens 87 -> 33 us).
-constexpr double kRunLaunch = 4.5;
+// 2140 to 8560 keys beside prompts of 3 to 5 tokens 87 -> 33 us). Where a CU has no place for them beside the blocks, their
+// last work-groups start as blocks end, of which some end early: half a row's time more. (Over 4136 random steps in which it
+// matters, the form chosen takes 1.04 times the best tried; 1.07 with a quarter of a row's time, 1.16 with none,
+// 1.04 with all of it. Rows in turn on as many work-groups as find a place: 1.02 times as long, a row beside a block is slow.)
+constexpr double kRunLaunch = 4.5, kLateRows = 0.5;
+
+// A row's work-group, in so many runs.
+static double row_time(const WindowArgs& w, int64_t runs) {
+  return 5 + (w.head_dim == 128 ? 0.18 : 0.14) * (double)((max_row_pages(w) + runs - 1) / runs);
+}
+
+// How long the step's single rows (or runs of them) outlast so many work-groups of blocks: those that find no place beside
+// the blocks' last round start as blocks end.
+static double rows_after(const WindowArgs& w, int columns, int64_t walk, int64_t blocks, int64_t rows, int64_t runs) {
+  const BlockCost& c = kBlockCost[w.head_dim == 128][columns == 128 ? 0 : columns == 64 ? 1 : 2];
+  const int64_t slots = 2 * device_cus(), last = blocks % slots;
+  const double row = row_time(w, runs), round = c.round + c.tile_two * (double)walk;
+  return last > 0 && rows * runs <= slots - last ? std::max(0.0, row - round) : kLateRows * row;
+}
+
+// The tiles of the longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
+static int64_t block_tiles(const WindowArgs& w, int columns) {
+  const int64_t group = w.num_heads / w.num_kv_heads;
+  const int64_t span = std::min<int64_t>(w.max_query_len, (columns + group - 1) / group + 1);
+  const int64_t pages = std::min<int64_t>(w.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
+  return (pages + 3) / 4;
+}
 
 static WindowPlan plan_blocks(const WindowArgs& w) {
   const PrefillArgs a = blocks_of_step(w);
-  const int64_t group = a.num_heads / a.num_kv_heads, cus = device_cus();
+  const int64_t cus = device_cus();
   const int64_t range_bytes = prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4;
   const int64_t row_pages = max_row_pages(w);
   const int64_t rows = w.single_query_seqs >= 0 ? w.single_query_seqs : w.num_seqs;
@@ -173,10 +198,7 @@ static WindowPlan plan_blocks(const WindowArgs& w) {
   for (int form = 0; form < 3; ++form) {
     const int columns = 128 >> form;
     const BlockCost& c = kBlockCost[a.head_dim == 128][form];
-    // The longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
-    const int64_t span = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
-    const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
-    const int64_t tiles = (pages + 3) / 4, blocks = prefill_work_groups(a, columns);
+    const int64_t tiles = block_tiles(w, columns), blocks = prefill_work_groups(a, columns);
     for (int64_t most : {0, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32}) {
       if (most >= tiles) break;
       // As few ranges as of so many tiles at most, all about as long.
@@ -189,8 +211,8 @@ static WindowPlan plan_blocks(const WindowArgs& w) {
       if (split > 0) t += kRangeLaunch + 2.0 * (double)(ranges * range_bytes) / kRangeBytesPerUs;
       for (int64_t runs = 1; runs <= 16; runs *= 2) {
         if (runs > 1 && (units * runs + blocks * ranges > 2 * cus || row_pages < 8 * runs || runs * row_bytes > kMaxRowBytes)) break;
-        const double row = 5 + (a.head_dim == 128 ? 0.18 : 0.14) * (double)((row_pages + runs - 1) / runs);
-        const double both = rows > 0 ? std::max(t, row) + (runs > 1 ? kRunLaunch : 0) : t;
+        const double after = rows > 0 ? rows_after(w, columns, split > 0 ? split : tiles, blocks * ranges, units, runs) : 0;
+        const double both = t + after + (runs > 1 ? kRunLaunch : 0);
         if (best == 0 || both < best) {
           best = both;
           p = {columns, (int32_t)split, split > 0 ? (int32_t)ranges : 0, (int32_t)runs};
