@@ -6,7 +6,7 @@ the tensors that the cache and attention kernels take (``AttentionMetadata``), o
 without a look at the lengths on the host: one launch on the current stream, capturable.
 
 * ``query_lens`` and ``context_lens``: int32 ``[S]``, new and cached tokens of each request
-  (0 new ones for a row that is not in use).
+  (0 new ones for a row that is not in use); at most 2^20 requests.
 * ``pages``: int32 ``[P]``, the requests' pages one request after another, each in the order of
   its positions: ``ceil((context + new) / 16)`` of them. With a ``window`` only those of its
   first ``sinks`` tokens and those from the page of position ``context - window + 1`` on: what
@@ -31,6 +31,7 @@ import torch
 from babyvllm.kernels import _lib
 
 _MAX_WIDTH = 1 << 28  # of a sequence of 2^31 tokens and more
+_MAX_SEQS = 1 << 20
 
 
 class StepTables(NamedTuple):
@@ -59,6 +60,8 @@ def build_step_tables(query_lens, context_lens, pages, num_tokens, width, *, win
     num_seqs = query_lens.shape[0]
     if context_lens.shape[0] != num_seqs:
         raise ValueError(f"context_lens has {context_lens.shape[0]} requests, query_lens {num_seqs}")
+    if num_seqs > _MAX_SEQS:
+        raise ValueError(f"at most 2^20 requests, got {num_seqs}")
     num_tokens, width, sinks, pad_page = (operator.index(v) for v in (num_tokens, width, sinks, pad_page))
     window = None if window is None else operator.index(window)
     if not 0 <= num_tokens < 2**31 or not 1 <= width <= _MAX_WIDTH:

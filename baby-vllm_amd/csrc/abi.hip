@@ -585,7 +585,7 @@ extern "C" int bvllm_build_step_tables(const int32_t* query_lens, const int32_t*
                                        int32_t* query_start_loc, int32_t* seq_lens, int64_t* positions,
                                        int64_t* slot_mapping, int32_t num_tokens, int32_t block_size, void* stream) {
   if (num_seqs < 0 || num_tokens < 0 || num_listed < 0 || window < 0 || sinks < 0 || block_size != 16) return kBad;
-  if (width < 1 || width > 1 << 28 || !query_start_loc) return kBad;
+  if (width < 1 || width > 1 << 28 || num_seqs > 1 << 20 || !query_start_loc) return kBad;  // (a work-group reads all lengths)
   if (num_seqs > 0 && (!query_lens || !context_lens || !block_tables || !seq_lens)) return kBad;
   if ((num_listed > 0 && !pages) || (num_tokens > 0 && (!positions || !slot_mapping))) return kBad;
   StepTablesArgs a{};
@@ -641,6 +641,7 @@ extern "C" int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int6
 static bool window_sizes_ok(const WindowArgs& a) {
   if (a.num_seqs < 0 || a.num_tokens < 0 || a.max_query_len < 0 || a.single_query_seqs < -1) return false;
   if (!valid_heads(a.num_heads, a.num_kv_heads) || (a.head_dim != 64 && a.head_dim != 128)) return false;
+  if (a.num_tokens > 0 && a.single_query_seqs > (a.num_seqs < a.num_tokens ? a.num_seqs : a.num_tokens)) return false;
   return a.window >= 1 && a.sinks >= 0;
 }
 

@@ -729,7 +729,7 @@ PyObject* fast_tables(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t max_width = PyLong_AsLongLong(a[8]);
   void* stream = PyLong_AsVoidPtr(a[10]);
   if (PyErr_Occurred()) return nullptr;
-  if (seqs == 0 || ctx->size(0) != seqs || !small(seqs) || !small(rows) || width < 1 || width > max_width) return none();
+  if (seqs == 0 || ctx->size(0) != seqs || seqs > 1 << 20 || !small(rows) || width < 1 || width > max_width) return none();
   if ((a[5] != Py_None && window < 1) || sinks < 0 || pad < INT32_MIN || pad > INT32_MAX) return none();
   at::Tensor out[5];
   int rc;

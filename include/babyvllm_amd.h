@@ -448,7 +448,7 @@ BVLLM_API int bvllm_reorder_beams(void* const* k_caches, void* const* v_caches, 
  * contiguous (pad_page where the request holds none), query_start_loc int32 [num_seqs + 1]
  * (exclusive sums, at most num_tokens), seq_lens int32 [num_seqs], positions and slot_mapping
  * int64 [num_tokens] (0 and -1 in rows behind the last request's; slot -1 too where a row's page
- * is not in the list, behind the table's width or negative). width at most 2^28.
+ * is not in the list, behind the table's width or negative). width at most 2^28, num_seqs at most 2^20.
  */
 BVLLM_API int bvllm_build_step_tables(const int32_t* query_lens, const int32_t* context_lens, int32_t num_seqs,
                      const int32_t* pages, int64_t num_listed, int32_t window, int32_t sinks, int32_t pad_page,
@@ -484,7 +484,7 @@ BVLLM_API int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int64
  * j < sinks. A row with no visible key outputs zeros; keys that a row does not see do not reach
  * it, whatever they hold, and table entries of pages that no row of the sequence sees may hold
  * anything. window at least 1, sinks at least 0, scale positive and finite. single_query_seqs as
- * in bvllm_paged_prefill (-1: unknown).
+ * in bvllm_paged_prefill (-1: unknown), at most num_seqs and num_tokens.
  * How the step is launched: sequences of several queries run in blocks of `columns` (128, 64 or 32) (query,
  * head) pairs; split_tiles > 0 cuts a block's walk over the keys it sees into num_ranges ranges of
  * split_tiles 64-key tiles (the last one runs to its end, so any num_ranges from 1 to that of the table

@@ -21,7 +21,7 @@ def tables(**k):
 
 def test_step_tables_refuses_on_the_host():
     bad = [dict(s=-1), dict(t=-1), dict(listed=-1), dict(window=-1), dict(sinks=-1), dict(bs=32), dict(width=0),
-           dict(width=(1 << 28) + 1), dict(new=None), dict(ctx=None), dict(pages=None), dict(bt=None), dict(qsl=None),
+           dict(width=(1 << 28) + 1), dict(s=(1 << 20) + 1), dict(new=None), dict(ctx=None), dict(pages=None), dict(bt=None), dict(qsl=None),
            dict(seq=None), dict(pos=None), dict(slots=None)]
     assert [k for k in bad if tables(**k) != BAD] == []
 
@@ -60,7 +60,7 @@ def test_window_attention_refuses_on_the_host():
            dict(mb=0), dict(bts=7), dict(t=1 << 28), dict(st=1 << 28), dict(columns=16),
            dict(columns=256), dict(split=-1), dict(split=1 << 21, ranges=1), dict(split=1), dict(split=1, ranges=3), dict(ranges=1),
            dict(split=2, ranges=1, ws=None), dict(split=2, ranges=1, ws=P + 4), dict(runs=0), dict(runs=9), dict(runs=2, ws=None),
-           dict(runs=2, ws=P + 8)]
+           dict(runs=2, ws=P + 8), dict(single=3), dict(s=40, single=17)]
     assert [k for k in bad if window(**{"t": 16, **k}) != BAD] == []
 
 
@@ -86,7 +86,7 @@ def test_plans_fit_what_the_call_takes_and_their_scratch_is_bounded():
         assert plan(*none, -1, 28, 4, 128, 64, 64, 4) == (128, 0, 0, 1, 0)
     for bad in ((-1, 1, 1, -1, 28, 4, 128, 64, 64, 4), (1, 1, 1, -1, 27, 4, 128, 64, 64, 4), (1, 1, 1, -1, 28, 4, 96, 64, 64, 4),
                 (1, 1, 1, -1, 28, 4, 128, 0, 64, 4), (1, 1, 1, -1, 28, 4, 128, 64, 0, 4), (1, 1, 1, -1, 28, 4, 128, 64, 64, -1),
-                (1, 1, -1, -1, 28, 4, 128, 64, 64, 4), (1, 1 << 28, 1, -1, 28, 4, 128, 64, 64, 4)):
+                (1, 1, -1, -1, 28, 4, 128, 64, 64, 4), (2, 9, 8, 3, 28, 4, 128, 64, 64, 4), (20, 9, 8, 10, 28, 4, 128, 64, 64, 4), (1, 1 << 28, 1, -1, 28, 4, 128, 64, 64, 4)):
         assert plan(*bad) is None
     rng = random.Random(0)
     taken = set()
@@ -96,7 +96,7 @@ def test_plans_fit_what_the_call_takes_and_their_scratch_is_bounded():
         heads, hkv, d = rng.choice([(28, 4, 128), (14, 2, 64), (8, 8, 64), (40, 1, 128), (64, 64, 128)])
         width = rng.choice([1, 7, rng.randint(17, 700), 2049, 1 << 27])
         columns, split, ranges, runs, nbytes = plan(
-            seqs, tokens, longest, rng.choice([-1, 0, rng.randint(0, seqs)]), heads, hkv, d, width,
+            seqs, tokens, longest, rng.choice([-1, 0, rng.randint(0, min(seqs, tokens))]), heads, hkv, d, width,
             rng.choice([1, 40, 1024, 8192, 2**31 - 1]), rng.choice([0, 4, 300, 2**31 - 1]))
         assert 0 <= nbytes <= 129 << 20 and (nbytes > 0) == (split > 0 or runs > 1)
         assert 1 <= runs <= min(width, 4096) and columns in (128, 64, 32)
