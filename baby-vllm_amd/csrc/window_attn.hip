@@ -163,42 +163,25 @@ constexpr int64_t kMaxRangeBytes = 64ll << 20;  // of the ranges' partials
 // 1.04 with all of it. Rows in turn on as many work-groups as find a place: 1.02 times as long, a row beside a block is slow.)
 constexpr double kRunLaunch = 4.5, kLateRows = 0.5;
 
-// A row's work-group, in so many runs.
-static double row_time(const WindowArgs& w, int64_t runs) {
-  return 5 + (w.head_dim == 128 ? 0.18 : 0.14) * (double)((max_row_pages(w) + runs - 1) / runs);
-}
-
-// How long the step's single rows (or runs of them) outlast so many work-groups of blocks: those that find no place beside
-// the blocks' last round start as blocks end.
-static double rows_after(const WindowArgs& w, int columns, int64_t walk, int64_t blocks, int64_t rows, int64_t runs) {
-  const BlockCost& c = kBlockCost[w.head_dim == 128][columns == 128 ? 0 : columns == 64 ? 1 : 2];
-  const int64_t slots = 2 * device_cus(), last = blocks % slots;
-  const double row = row_time(w, runs), round = c.round + c.tile_two * (double)walk;
-  return last > 0 && rows * runs <= slots - last ? std::max(0.0, row - round) : kLateRows * row;
-}
-
-// The tiles of the longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
-static int64_t block_tiles(const WindowArgs& w, int columns) {
-  const int64_t group = w.num_heads / w.num_kv_heads;
-  const int64_t span = std::min<int64_t>(w.max_query_len, (columns + group - 1) / group + 1);
-  const int64_t pages = std::min<int64_t>(w.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
-  return (pages + 3) / 4;
-}
-
 static WindowPlan plan_blocks(const WindowArgs& w) {
   const PrefillArgs a = blocks_of_step(w);
-  const int64_t cus = device_cus();
+  const int64_t group = a.num_heads / a.num_kv_heads, cus = device_cus();
   const int64_t range_bytes = prefill_range_floats(1, a.num_tokens, a.num_heads, a.head_dim) * 4;
   const int64_t row_pages = max_row_pages(w);
   const int64_t rows = w.single_query_seqs >= 0 ? w.single_query_seqs : w.num_seqs;
   const int64_t units = row_units(w, rows);
   const int64_t row_bytes = (int64_t)a.num_seqs * a.num_heads * (a.head_dim + 1) * 4;
+  double row_us[5];  // a row's work-group, in 1, 2, .. 16 runs
+  for (int i = 0; i < 5; ++i) row_us[i] = 5 + (a.head_dim == 128 ? 0.18 : 0.14) * (double)((row_pages + (1 << i) - 1) >> i);
   WindowPlan p{128, 0, 0, 1};
   double best = 0;
   for (int form = 0; form < 3; ++form) {
     const int columns = 128 >> form;
     const BlockCost& c = kBlockCost[a.head_dim == 128][form];
-    const int64_t tiles = block_tiles(w, columns), blocks = prefill_work_groups(a, columns);
+    // The longest walk that there can be: the window of a block's rows, the first tokens' pages, inside the table.
+    const int64_t span = std::min<int64_t>(a.max_query_len, (columns + group - 1) / group + 1);
+    const int64_t pages = std::min<int64_t>(a.max_blocks, ((int64_t)w.window + span + 15) / 16 + 1 + ((int64_t)w.sinks + 15) / 16);
+    const int64_t tiles = (pages + 3) / 4, blocks = prefill_work_groups(a, columns);
     for (int64_t most : {0, 4, 5, 6, 7, 8, 10, 12, 14, 16, 20, 24, 28, 32}) {
       if (most >= tiles) break;
       // As few ranges as of so many tiles at most, all about as long.
@@ -209,10 +192,13 @@ static WindowPlan plan_blocks(const WindowArgs& w) {
       double t = c.start - c.round + (double)full * (c.round + c.tile_two * walk);
       if (rest > 0) t += c.round + (rest > cus ? c.tile_two : c.tile_one) * walk;
       if (split > 0) t += kRangeLaunch + 2.0 * (double)(ranges * range_bytes) / kRangeBytesPerUs;
-      for (int64_t runs = 1; runs <= 16; runs *= 2) {
-        if (runs > 1 && (units * runs + blocks * ranges > 2 * cus || row_pages < 8 * runs || runs * row_bytes > kMaxRowBytes)) break;
-        const double after = rows > 0 ? rows_after(w, columns, split > 0 ? split : tiles, blocks * ranges, units, runs) : 0;
-        const double both = t + after + (runs > 1 ? kRunLaunch : 0);
+      const int64_t places = rest > 0 ? 2 * cus - rest : 0;  // beside the last round
+      for (int i = 0; i < 5; ++i) {
+        const int64_t runs = 1 << i;
+        if (i > 0 && (units * runs + blocks * ranges > 2 * cus || row_pages < 8 * runs || runs * row_bytes > kMaxRowBytes)) break;
+        // How long the rows outlast the blocks.
+        const double after = units * runs <= places ? std::max(0.0, row_us[i] - c.round - c.tile_two * walk) : kLateRows * row_us[i];
+        const double both = t + (rows > 0 ? after : 0) + (runs > 1 ? kRunLaunch : 0);
         if (best == 0 || both < best) {
           best = both;
           p = {columns, (int32_t)split, split > 0 ? (int32_t)ranges : 0, (int32_t)runs};
