@@ -231,7 +231,9 @@ static hipError_t launch_window(const WindowArgs& w, const WindowPlan& p, float*
     a.part_ml = a.part_out + (int64_t)p.num_ranges * w.num_tokens * w.num_heads * D;
     err = paged_prefill_window(a, r, p.columns, stream);
   }
-  if (err != hipSuccess || p.row_runs == 1 || w.single_query_seqs == 0) return err;
+  // (Steps of one row a sequence run on the rows' work-groups whatever the count says; longer ones with a count of 0 have none.)
+  const bool has_rows = w.max_query_len == 1 || w.single_query_seqs != 0;
+  if (err != hipSuccess || p.row_runs == 1 || !has_rows) return err;
   const int per_row = (w.num_heads * (D / 4) + 255) / 256;
   if ((int64_t)w.num_seqs * per_row > 0x7fffffff) return hipErrorInvalidValue;
   hipLaunchKernelGGL((window_merge_kernel<D>), dim3((unsigned)(w.num_seqs * per_row)), dim3(256), 0, stream, r, per_row);
