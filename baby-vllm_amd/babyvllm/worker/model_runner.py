@@ -14,8 +14,9 @@
   edited in place) by a single non-blocking copy into a device buffer of the
   same layout, which every captured graph reads; the attention kernels see
   ``max_seq_len`` = the context bucket, so the captured grid fits every replay.
-* Any other step runs eagerly with metadata built from the scheduler output (its
-  lengths and pages in one copy, tables and slots on the GPU), then takes each sequence's last row of hidden states to the LM head.
+* Any other step runs eagerly with metadata built from the scheduler output (tokens and
+  slots in one copy, lengths and pages in another, tables and positions made of them on the
+  GPU), then takes each sequence's last row of hidden states to the LM head.
 Greedy requests (temperature 0) are sampled with the HIP argmax kernel;
 others with torch softmax / top-p / multinomial on the host side of the path.
 """
@@ -122,13 +123,12 @@ class ModelRunner:
     # ----------------------------------------------------------- eager steps
 
     def prepare_inputs(self, scheduler_output):
-        ids, positions, slots, tables = [], [], [], []
+        ids, slots, tables = [], [], []
         qsl, seq_lens, ctx_lens = [0], [], []
         for seq in scheduler_output.scheduled_sequences:
             n = scheduler_output.num_scheduled_tokens[seq.seq_id]
             ctx = seq.num_computed_tokens
             ids.extend(seq.token_ids[ctx:ctx + n])
-            positions.extend(range(ctx, ctx + n))
             slots.extend(scheduler_output.slot_mappings[seq.seq_id])
             tables.append(scheduler_output.block_tables[seq.seq_id])
             qsl.append(qsl[-1] + n)
@@ -140,9 +140,11 @@ class ModelRunner:
         dev = self.device
         host = dict(query_start_loc_cpu=qsl, seq_lens_cpu=seq_lens, context_lens_cpu=ctx_lens,
                     max_query_len=max(qsl[i + 1] - qsl[i] for i in range(len(tables))), max_seq_len=max(seq_lens))
-        input_ids = torch.tensor(ids, dtype=torch.int64, device=dev)
+        # The slots are the scheduler's: it may store a token elsewhere than its table says, or nowhere.
+        wide = torch.tensor(ids + slots, dtype=torch.int64, device=dev)
+        input_ids, slot_mapping = wide[:len(ids)], wide[len(ids):]
         if dev.type == "cuda" and self.block_size == 16:
-            # Lengths and pages go over in one copy; the GPU makes the tables, slots and positions of them.
+            # Lengths and pages go over in one copy; the GPU makes the tables and positions of them.
             n = len(tables)
             packed = [b - a for a, b in zip(qsl, qsl[1:])] + ctx_lens
             for t, length in zip(tables, seq_lens):
@@ -151,10 +153,11 @@ class ModelRunner:
             ctx = packed[n:2 * n]
             step = build_step_tables(packed[:n], ctx, packed[2 * n:], len(ids), width)
             return input_ids, step.positions, AttentionMetadata(
-                slot_mapping=step.slot_mapping, block_tables=step.block_tables, query_start_loc=step.query_start_loc,
+                slot_mapping=slot_mapping, block_tables=step.block_tables, query_start_loc=step.query_start_loc,
                 seq_lens=step.seq_lens, context_lens=ctx, **host)
+        positions = [p for ctx, length in zip(ctx_lens, seq_lens) for p in range(ctx, length)]
         md = AttentionMetadata(
-            slot_mapping=torch.tensor(slots, dtype=torch.int64, device=dev),
+            slot_mapping=slot_mapping,
             block_tables=torch.tensor([t + [0] * (width - len(t)) for t in tables], dtype=torch.int32,
                                       device=dev),
             query_start_loc=torch.tensor(qsl, dtype=torch.int32, device=dev),
