@@ -64,3 +64,14 @@ def test_the_schedulers_slots_are_the_steps():
         written = (rows != 3.0).flatten(2).any(-1)  # [2, slots]
         for half in written:
             assert half.nonzero().flatten().tolist() == sorted(x for x in given if x >= 0)
+
+
+@pytest.mark.parametrize("short", [0, 1, 2])
+def test_a_table_that_ends_before_its_request_is_refused(short):
+    # Its neighbours' pages would be taken for its own, and theirs for the next requests'.
+    runner = runner_of()
+    out = step_of(SPECS, TABLES)
+    seq = out.scheduled_sequences[short].seq_id
+    out.block_tables[seq] = out.block_tables[seq][:-1] if short != 1 else out.block_tables[seq][:2]
+    with pytest.raises(ValueError, match=f"request {seq} "):
+        runner.prepare_inputs(out)
