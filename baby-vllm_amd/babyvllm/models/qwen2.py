@@ -43,6 +43,11 @@ def _has_hooks(m: nn.Module) -> bool:
                 or g._global_backward_pre_hooks or "forward" in m.__dict__)
 
 
+def _normed(out):
+    """The normed tensor of a norm module's result: (normed, residual) as RMSNorm's, or the tensor itself."""
+    return out if isinstance(out, torch.Tensor) else out[0]
+
+
 class Qwen2MLP(nn.Module):
     def __init__(self, hidden_size: int, intermediate_size: int):
         super().__init__()
@@ -91,7 +96,7 @@ class Qwen2Attention(nn.Module):
         # The fused form skips the norm modules' calls: only where nothing is attached to them.
         if self.q_norm is not None and not (type(self.q_norm) is type(self.k_norm) is RMSNorm and not _has_hooks(self.q_norm)
                                             and not _has_hooks(self.k_norm) and self.q_norm.eps == self.k_norm.eps):
-            q, k = self.q_norm(q.contiguous())[0], self.k_norm(k.contiguous())[0]
+            q, k = _normed(self.q_norm(q.contiguous())), _normed(self.k_norm(k.contiguous()))
             q, k = fused_rope_and_cache(q, k, v, cos, sin, kv_cache=self.attn.kv_cache, slot_mapping=slots)
         elif self.q_norm is not None:
             q = fused_qk_norm_rope_and_cache(q, k, v, self.q_norm.weight, self.k_norm.weight, self.q_norm.eps, cos, sin,
