@@ -35,6 +35,8 @@ class Attention(nn.Module):
         super().__init__()
         if (window is not None and window < 1) or sinks < 0:
             raise ValueError(f"window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+        if window is None and sinks:
+            raise ValueError(f"{sinks} first tokens stay visible beside a window, and there is no window")
         self.num_heads = num_heads
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
