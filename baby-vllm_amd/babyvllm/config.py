@@ -5,13 +5,16 @@ a checkpoint's config.json. There is no network here, so besides
 ``from_hf(path)`` (a local directory) the two shapes the benchmarks use are
 available as presets: ``qwen2_5_7b()`` and ``qwen2_5_0_5b()``. ``sliding_window``,
 ``attention_sinks`` and ``qk_norm`` are this build's own: set them on a config for a
-model with those; ``from_hf`` and the presets leave them off.
+model with those. ``from_hf`` takes a checkpoint's ``sliding_window`` where every layer uses
+it, and warns where only some do (one window is for all layers here: those then attend all
+keys); the presets leave all three off.
 """
 
 from __future__ import annotations
 
 import json
 import os
+import warnings
 from dataclasses import dataclass
 
 
@@ -57,8 +60,25 @@ class ModelConfig:
             num_attention_heads=c["num_attention_heads"], num_key_value_heads=c["num_key_value_heads"],
             rms_norm_eps=c["rms_norm_eps"], max_position_embeddings=c["max_position_embeddings"],
             rope_theta=c["rope_theta"], tie_word_embeddings=c.get("tie_word_embeddings", False),
-            block_size=block_size,
+            block_size=block_size, sliding_window=_window_of(c),
         )
+
+
+def _window_of(c: dict) -> int | None:
+    """The window of a checkpoint's layers: of those that ``layer_types`` names, or else of the ones from
+    ``max_window_layers`` (28) on. None where no layer has one that hides a key."""
+    window = c.get("sliding_window") if c.get("use_sliding_window", False) else None
+    if window is None or window >= c["max_position_embeddings"]:
+        return None
+    layers = c["num_hidden_layers"]
+    types = c.get("layer_types")
+    windowed = types.count("sliding_attention") if types else layers - min(layers, c.get("max_window_layers", 28))
+    if windowed == layers:
+        return window
+    if windowed:
+        warnings.warn(f"{windowed} of {layers} layers have a sliding window of {window}: here they attend all keys, which "
+                      "differs for sequences longer than that")
+    return None
 
 
 def qwen2_5_7b(block_size: int = 16) -> ModelConfig:
