@@ -41,6 +41,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <type_traits>
 
 namespace bvllm {
@@ -109,6 +110,9 @@ struct WindowLaunchArgs {
   int32_t grid[4];
   WindowRows rows;
 };
+static_assert(offsetof(WindowLaunchArgs, blocks) == 0 && offsetof(WindowLaunchArgs, grid) == sizeof(PrefillArgs) &&
+                  offsetof(WindowLaunchArgs, rows) == sizeof(PrefillArgs) + 16 && alignof(WindowRows) == 8,
+              "arguments lie behind one another, each at its own alignment");
 typedef const uint32_t __attribute__((address_space(4)))* WindowLaunch;
 
 template <int D, int NW, bool SPL>
@@ -1365,6 +1369,9 @@ static hipError_t launch_prefill_window(const PrefillArgs& a, const WindowRows& 
   const int64_t row_wgs = a.single_query_seqs != 0 ? (decode_col_groups(rows.rows) * a.num_seqs * rows.rows.num_splits + 7) / 8 * 8 : 0;
   if (wgs + row_wgs == 0) return hipSuccess;
   if (wgs + row_wgs > 0x7ffffff0) return hipErrorInvalidValue;
+  // (What window_block_rows reads as WindowLaunchArgs.)
+  static_assert(std::is_same_v<decltype(&paged_prefill_kernel<D, 4, QT, false, KS, SPL, false, true>),
+                               void (*)(PrefillArgs, int, int, int, int, WindowRows, int, int)>, "the kernel's arguments");
   hipLaunchKernelGGL((paged_prefill_kernel<D, 4, QT, false, KS, SPL, false, true>), dim3((unsigned)(row_wgs + wgs)),
                      dim3(4 * 64), 0, stream, a, (int)p.bound, p.dense_qb, p.xcd_group, (int)p.per_xcd, rows, (int)row_wgs,
                      SPL ? a.num_ranges : 1);
