@@ -51,7 +51,7 @@ struct Lengths {
 __global__ __launch_bounds__(kThreads) void step_tables_kernel(StepTablesArgs a, int64_t entries, FastDiv by_width,
                                                                int row_groups) {
   __shared__ int64_t list_start[kChunk];
-  __shared__ int32_t row_start[kChunk + 1], ctx[kChunk], pages[kChunk], gone[kChunk];
+  __shared__ int32_t row_start[kChunk], ctx[kChunk], pages[kChunk], gone[kChunk];
   __shared__ Lengths wave_sum[kThreads / 64];
 
   const int tid = (int)threadIdx.x, lane = lane_id(), wave = wave_id();
@@ -124,7 +124,6 @@ __global__ __launch_bounds__(kThreads) void step_tables_kernel(StepTablesArgs a,
       at.pages += p[k] - g[k];
     }
     const int32_t rows_end = (int32_t)min(before.tokens, (int64_t)a.num_tokens);
-    if (tid == 0) row_start[kChunk] = rows_end;
     __syncthreads();
 
     // The thread's table entries, of one or of several rows, as far as they lie in the chunk.
