@@ -15,8 +15,8 @@ does not reach it, whatever it holds. Rows of ``q`` behind the last sequence are
 ``md.max_query_len`` bounds the query rows of every sequence. Few rows behind long windows are cut over more
 work-groups, chosen from host sizes and (outside a capture) the list ``md.query_start_loc_cpu``: the last bits of a row can
 depend on the other sequences of the step. That takes fp32 scratch (at most 128 MiB); without the memory
-for it the launch that needs none runs. Scores, softmax statistics and sums are fp32; the weights are rounded to bf16, as in
-``paged_prefill_attention``.
+for it the launch that needs none runs. Scores, softmax statistics and sums are fp32. The weights of sequences of one row keep
+16 bits, those of several rows are rounded to bf16, as in ``paged_prefill_attention``.
 """
 
 from __future__ import annotations

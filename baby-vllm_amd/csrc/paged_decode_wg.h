@@ -156,10 +156,11 @@ struct PagePv {
   float alpha;
   bool fresh;          // the state had seen no live token (m = -inf): its accumulators are +0
   uint2 pb;            // P, bf16, B operand of the PV MFMAs
+  uint2 rest;          // WIDE: what P's upper 16 bits leave of it
   uint2 va[D / 16];    // V^T operands (row = dim (D/16)·r + c, k = token 4g+i)
 };
 
-template <int D, typename Sees>
+template <int D, bool WIDE = false, typename Sees>
 __device__ __forceinline__ void softmax_phase_if(WaveState<D>& st, PagePv<D>& ph, f32x4_t s,
                                                  const RowSlice<D> (&v)[4], int tok0, Sees sees, float scale_log2) {
   constexpr int VD = D / 16;
@@ -185,8 +186,21 @@ __device__ __forceinline__ void softmax_phase_if(WaveState<D>& st, PagePv<D>& ph
   for (int i = 0; i < 4; ++i) p[i] = fast_exp2(sv[i] - m_ref);
   st.l = __builtin_fmaf(st.l, ph.alpha, (p[0] + p[1]) + (p[2] + p[3]));
   st.m = m_new;
-  ph.pb.x = pack_bf16x2_hw(p[0], p[1]);
-  ph.pb.y = pack_bf16x2_hw(p[2], p[3]);
+  if constexpr (WIDE) {
+    // P as two operands, 16 bits in all: its upper half, and the rest, which is at least 2^-126 so that an infinite V
+    // meets no 0 there (P itself is its upper half where its lower bits are 0).
+    ph.pb.x = pick_halves(__float_as_uint(p[0]), __float_as_uint(p[1]), 1);
+    ph.pb.y = pick_halves(__float_as_uint(p[2]), __float_as_uint(p[3]), 1);
+    float rest[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      rest[i] = fmaxf(p[i] - __uint_as_float(__float_as_uint(p[i]) & 0xffff0000u), 0x1p-126f);
+    ph.rest.x = pack_bf16x2_hw(rest[0], rest[1]);
+    ph.rest.y = pack_bf16x2_hw(rest[2], rest[3]);
+  } else {
+    ph.pb.x = pack_bf16x2_hw(p[0], p[1]);
+    ph.pb.y = pack_bf16x2_hw(p[2], p[3]);
+  }
   constexpr int VW = VD / 2;  // dwords per V row slice
   uint32_t vv[4][VW];
 #pragma unroll
@@ -216,10 +230,14 @@ __device__ __forceinline__ void rescale_phase(WaveState<D>& st, const PagePv<D>&
   }
 }
 
-template <int D>
+template <int D, bool WIDE = false>
 __device__ __forceinline__ void pv_phase(WaveState<D>& st, const PagePv<D>& ph) {
 #pragma unroll
   for (int c = 0; c < D / 16; ++c) st.acc[c] = mfma_16x16x16(ph.va[c], ph.pb, st.acc[c]);
+  if constexpr (WIDE) {
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) st.acc[c] = mfma_16x16x16(ph.va[c], ph.rest, st.acc[c]);
+  }
 }
 
 template <int D>

@@ -74,6 +74,9 @@ int64_t prefill_work_groups(const PrefillArgs& a, int columns);
 // own, as the decode work-groups do (paged_decode_wg.h). The states meet in LDS: every wave
 // writes its sums of the heads there are, and each (head, 4 dims) is added up in wave order.
 // The result of a run that is not the whole row is an fp32 (o, lse), added by window_merge_kernel.
+// Weights meet V as two bf16 operands, 16 bits: bound by memory, the rows have room for the second product
+// (64 rows of 1028 keys, 28 / 4 heads of 128: 24.0 us with one operand, 24.1 with two, in one run; error against 64 bits
+// 2.10e-3 -> 1.66e-3, as fp32 weights give; one row of 260 keys at D = 64 5.15 -> 5.31).
 
 // Runs of a row of n pages: `per` pages each, `live` of them not empty (one of an empty row).
 struct Runs {
@@ -131,10 +134,10 @@ __device__ __forceinline__ void window_row(const DecodeArgs& a, int b, int row, 
   auto page_work = [&](const PageRegs<D>& r, int k) __attribute__((always_inline)) {
     const f32x4_t scores = register_scores<D>(r, qb, tile, n, g);
     PagePv<D> ph;
-    softmax_phase_if<D>(st, ph, scores, r.v, 16 * page(first + NW * k) + 4 * g,
-                        [&](int tok) { return view.sees(tok); }, a.scale_log2);
+    softmax_phase_if<D, true>(st, ph, scores, r.v, 16 * page(first + NW * k) + 4 * g,
+                              [&](int tok) { return view.sees(tok); }, a.scale_log2);
     rescale_phase<D>(st, ph);
-    pv_phase<D>(st, ph);
+    pv_phase<D, true>(st, ph);
   };
 
   for (int base = 0; base < cnt; base += 64) {

@@ -493,7 +493,8 @@ BVLLM_API int bvllm_qk_norm_rope_append(const void* q, int64_t q_stride_t, int64
  * bvllm_window_workspace_bytes() of the same num_ranges (0 without ranges) and row_runs says how much,
  * and may be 0. bvllm_window_plan writes the four to use, from host sizes alone (plan[0..3]: columns, split_tiles,
  * num_ranges, row_runs; partials of either kind are at most 64 MiB). They steer the choice only: results agree
- * within the rounding of fp32 sums in another order.
+ * within the rounding of fp32 sums in another order and of the weights: scores, statistics and sums are fp32, the
+ * weights of single queries keep 16 bits, those of the blocks are rounded to bf16 (as bvllm_paged_prefill's).
  */
 BVLLM_API int bvllm_window_plan(int32_t num_seqs, int32_t num_tokens, int32_t max_query_len,
                      int32_t single_query_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
