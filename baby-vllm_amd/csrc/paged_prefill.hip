@@ -181,7 +181,11 @@ __attribute__((noinline)) __device__ void window_block_rows(WindowLaunch launch,
 // some row of the block sees (BlockWalk), put together to tiles whatever lies between them; keys
 // that a column does not see are masked by their place in the walk. A key that some columns of a
 // block see and others do not is in a tile of all of them, where a weight of 0 leaves the product's
-// 0·V: a block whose sums are not finite is computed again, row by row (window_row).
+// 0·V: a block whose sums are not finite is computed again, row by row (window_row). P is rounded to bf16 as in the
+// other forms, so that a window of everything gives what no window does to the same roundings (error against 64 bits
+// 2.2e-3 to 2.3e-3, with fp32 weights 1.65e-3). P as two bf16 operands gives the latter and takes, 28 / 4 heads of 128 (14 / 2 of
+// 64): 77 rows behind 16,000, 4096 + 4 keys, in 32 columns 22.8 -> 23.5 us (16.5 -> 17.0), 24 rows and 6 prompts of 65 to 1001,
+// 512 + 16 keys, 35.3 -> 38.6 (17.0 -> 18.8), 8192 tokens, 1024 + 4 keys, 142 -> 177 (61.6 -> 72.9).
 template <int D, int NW, int QT, bool MB, int KS, bool SPL = false, bool CTX = false, bool WIN = false>
 __global__ __launch_bounds__(NW * 64, 2) void paged_prefill_kernel(PrefillArgs a, int n_blocks_bound, int dense_qb,
                                                                   int xcd_group, int per_xcd,
