@@ -83,6 +83,8 @@ def paged_window_attention(q, kv_cache, md, scale, window, sinks=0):
     qsl, seq_lens, ctx_lens = md.query_start_loc.contiguous(), md.seq_lens.contiguous(), md.context_lens.contiguous()
     h = _lib.lib()
     single = _single_query_seqs(md, num_seqs) if max_query_len > 1 and host_lists else -1
+    if single >= 0 and md.query_start_loc_cpu[-1] > num_tokens:
+        single = -1  # another step's list: this one leaves rows out
     with torch.cuda.device(q.device):
         plan = (ctypes.c_int32 * 4)()
         _lib.check(h.bvllm_window_plan(num_seqs, num_tokens, max_query_len, single, num_heads, num_kv_heads, head_dim,

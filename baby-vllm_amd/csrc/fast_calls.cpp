@@ -845,6 +845,7 @@ PyObject* fast_window(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (i > 0 && at - last == 1) ++single;
       last = at;
     }
+    if (last > tokens) single = -1;  // another step's list: this one leaves rows out
   }
   const int32_t w = (int32_t)std::min<int64_t>(window, INT32_MAX), first = (int32_t)std::min<int64_t>(sinks, INT32_MAX);
   int32_t plan[4];  // columns, split_tiles, num_ranges, row_runs

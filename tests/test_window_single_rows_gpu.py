@@ -56,3 +56,19 @@ def test_a_request_of_which_the_step_has_one_row(native, monkeypatch):
         torch.cuda.synchronize()
         del spoilt
         check(paged_window_attention(q, cache, md, 0.1, 4096, 4), want)
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("rows", [1, 2, 5, 6])
+def test_host_lists_of_more_rows_than_the_step_has(rows, native, monkeypatch):
+    if not native:
+        python_path(monkeypatch)
+    # Requests of 5, 1, 1 and 1 new tokens, a step of fewer rows.
+    new, ctx = [5, 1, 1, 1], [1500, 40, 300, 900]
+    full, cache, whole = build(list(zip(ctx, new)), 2, 7, 64, 1000, 4)
+    held = [whole.block_tables[s, :-(-(c + n) // 16)] for s, (c, n) in enumerate(zip(ctx, new))]
+    t = build_step_tables(i32(new), i32(ctx), torch.cat(held), rows, whole.block_tables.shape[1])
+    md = AttentionMetadata(t.slot_mapping, t.block_tables, t.query_start_loc, t.seq_lens, i32(ctx), [0, 5, 6, 7, 8],
+                           [c + n for c, n in zip(ctx, new)], ctx, 5, 1505)
+    q = full[:rows].contiguous()
+    check(paged_window_attention(q, cache, md, 0.1, 1000, 4), formula(q, cache, md, 0.1, 1000, 4))
