@@ -125,6 +125,8 @@ def paged_prefill_attention(q, kv_cache, md, scale):
         raise ValueError("K and V halves of kv_cache must share a layout with unit last stride")
     num_seqs = seq_lens.shape[0]
     single = _single_query_seqs(md, num_seqs)
+    if single >= 0 and md.query_start_loc_cpu[-1] > num_tokens:
+        single = -1  # another step's list: this one leaves rows out
     split_tiles = _split_tiles(md, num_seqs, num_tokens, single, num_heads, num_kv_heads, head_dim, bt.shape[1])
     args = (
         q.data_ptr(), q.stride(0), q.stride(1),

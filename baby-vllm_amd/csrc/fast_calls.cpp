@@ -400,6 +400,7 @@ PyObject* fast_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     }
     prev = v;
   }
+  if (prev > tokens) return none();  // another step's list: this one leaves rows out
   if (!PyLong_CheckExact(a[8]) || !PyFloat_CheckExact(a[9])) return none();
   const int64_t max_q = clamped(a[8]);
   const float scale = (float)PyFloat_AsDouble(a[9]);
